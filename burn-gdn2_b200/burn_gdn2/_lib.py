@@ -82,6 +82,18 @@ class PrologueArgs(ctypes.Structure):
                 ("w", ctypes.c_void_p), ("g", ctypes.c_void_p)]
 
 
+class ScanArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("seq_len", ctypes.c_int32), ("channels", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("g_dtype", ctypes.c_int32), ("complement", ctypes.c_int32),
+                ("cu_seqlens", ctypes.c_void_p), ("x", View), ("g", View), ("state_in", ctypes.c_void_p),
+                ("carry", ctypes.c_void_p)]
+
+
+class ScanBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", ScanArgs), ("d_h", View), ("d_state_out", ctypes.c_void_p), ("dx", View), ("dg", View),
+                ("d_state_in", ctypes.c_void_p)]
+
+
 class Config(ctypes.Structure):
     _fields_ = [("hidden_size", ctypes.c_int64), ("num_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
                 ("expand_v", ctypes.c_float), ("num_v_heads", ctypes.c_int64), ("use_short_conv", ctypes.c_int32),
@@ -96,7 +108,7 @@ EXPORTS = (
     "gdn2_last_error", "gdn2_last_cuda_error", "gdn2_abi_version", "gdn2_read_device_errors",
     "gdn2_selftest_umma", "gdn2_chunk_fwd_noalloc", "gdn2_project_activations", "gdn2_selftest_wait",
     "gdn2_set_reserved_sms", "gdn2_recurrent_bwd_workspace_bytes", "gdn2_recurrent_bwd",
-    "gdn2_chunk_trajectory",
+    "gdn2_chunk_trajectory", "gdn2_gated_scan", "gdn2_gated_scan_bwd",
 )
 
 
@@ -123,6 +135,10 @@ def _load():
     lib.gdn2_recurrent_bwd.restype = ctypes.c_int
     lib.gdn2_chunk_trajectory.argtypes = [P(RecurrentArgs), i32, vp, View, vp]
     lib.gdn2_chunk_trajectory.restype = ctypes.c_int
+    lib.gdn2_gated_scan.argtypes = [P(ScanArgs), View, vp, vp]
+    lib.gdn2_gated_scan.restype = ctypes.c_int
+    lib.gdn2_gated_scan_bwd.argtypes = [P(ScanBwdArgs), vp]
+    lib.gdn2_gated_scan_bwd.restype = ctypes.c_int
     lib.gdn2_short_conv.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     lib.gdn2_short_conv.restype = ctypes.c_int
     lib.gdn2_rms_norm_gate.argtypes = [P(Dims), i32, View, View, vp, f32, View, vp]

@@ -1,0 +1,184 @@
+"""Sequence operators around a gated recurrence, for training and serving.
+
+  gated_scan        the diagonal gated linear recurrence h_t = e^{g_t} h_{t-1} + s_t x_t
+
+Every operator takes CUDA tensors on any device and launches on that device's
+current stream; it is differentiable where an input requires a gradient, and
+deterministic.  Sequences come as a dense batch [B,T,C], or packed: one
+buffer [1,R,C] with ``cu_seqlens`` (int32 [N+1], ascending from 0), sequence n
+in the rows cu_seqlens[n] .. cu_seqlens[n+1].  A ``cu_seqlens`` on the CPU is
+checked and copied to the device; one on the device is taken as it is (the
+kernels stay inside the buffers whatever it holds).  Rows behind the last
+sequence come out as zero, in outputs and gradients.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import LIB, check
+from .ops import _DT, dtype_code
+
+SCAN_CARRY = 16  # tokens between the states that gated_scan keeps for its backward
+
+_NOTHING = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device as the current one for a launch (free when it is already)."""
+    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _same_device(what: str, device: torch.device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _check_input(what: str, x: torch.Tensor):
+    if not x.is_cuda:
+        raise RuntimeError(f"{what} runs on the B200 CUDA kernels only; got a CPU tensor")
+    if x.dtype not in _DT:
+        raise TypeError(f"{what}: unsupported dtype {x.dtype}; use float32 or bfloat16")
+
+
+def _cu_seqlens(what: str, cu: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """Packed offsets on x's device, int32; the values are checked where they are on the host."""
+    if x.shape[0] != 1:
+        raise ValueError(f"{what}: packed sequences come as one buffer [1,R,C], got a batch of {x.shape[0]}")
+    if cu.dim() != 1 or cu.numel() < 2 or cu.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: cu_seqlens must be int32 [N+1] with N >= 1, got {cu.dtype} {list(cu.shape)}")
+    if not cu.is_cuda:
+        steps = cu[1:] - cu[:-1]
+        if int(cu[0]) != 0 or int(steps.min()) < 0 or int(cu[-1]) > x.shape[1]:
+            raise ValueError(f"{what}: cu_seqlens must ascend from 0 to at most {x.shape[1]} rows, got {cu.tolist()}")
+        return cu.to(device=x.device, dtype=torch.int32)
+    _same_device(what, x.device, cu)
+    if cu.dtype != torch.int32:
+        raise ValueError(f"{what}: cu_seqlens on the device must be int32, got {cu.dtype}")
+    return cu.contiguous()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous channels and no broadcast over them."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _view3(t: Optional[torch.Tensor]) -> _lib.View:
+    """[B,T,C] as the library's [B,T,1,C] view."""
+    if t is None:
+        return _lib.View()
+    s = t.stride()
+    return _lib.View(t.data_ptr(), s[0], s[1], 0)
+
+
+def _f32(what: str, name: str, t: Optional[torch.Tensor], shape) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
+    return t.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+# -- gated scan ----------------------------------------------------------------
+
+
+def _scan_args(x, g, state, cu, complement, carry):
+    return _lib.ScanArgs(x.shape[0] if cu is None else cu.numel() - 1, x.shape[1], x.shape[2], _DT[x.dtype],
+                         _DT[g.dtype], int(complement), _ptr(cu), _view3(x), _view3(g), _ptr(state), _ptr(carry))
+
+
+def _scan_forward(x, g, state, cu, complement, state_out, keep):
+    B, T, C = x.shape
+    h = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
+    carry = torch.empty((B, -(-T // SCAN_CARRY), C), dtype=torch.float32, device=x.device) if keep else None
+    a = _scan_args(x, g, state, cu, complement, carry)
+    with _on(x.device):
+        check(LIB.gdn2_gated_scan(ctypes.byref(a), _view3(h), _ptr(state_out), _stream(x.device)))
+    return h, carry
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, g, state, cu, complement):
+        n = x.shape[0] if cu is None else cu.numel() - 1
+        last = torch.empty((n, x.shape[2]), dtype=torch.float32, device=x.device)
+        h, carry = _scan_forward(x, g, state, cu, complement, last, True)
+        ctx.save_for_backward(x, g, state, cu, carry)
+        ctx.complement = complement
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_h, d_last):
+        x, g, state, cu, carry = ctx.saved_tensors
+        d_h = torch.zeros_like(x) if d_h is None else _rows(d_h)
+        d_last = None if d_last is None else d_last.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dg = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[2] else None
+        a = _lib.ScanBwdArgs(_scan_args(x, g, state, cu, ctx.complement, carry), _view3(d_h), _ptr(d_last),
+                             _view3(dx), _view3(dg), _ptr(d_state))
+        with _on(x.device):
+            check(LIB.gdn2_gated_scan_bwd(ctypes.byref(a), _stream(x.device)))
+        return dx, dg, d_state, None, None
+
+
+def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
+               inplace: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The diagonal gated linear recurrence h_t = e^{g_t} h_{t-1} + s_t x_t.
+
+    x [B,T,C] (f32 or bf16); g [B,T,C], the log decay, f32 or x's dtype;
+    state [B,C] f32, the state before the first token (None: zeros).  s_t = 1,
+    or 1 - e^{g_t} with ``complement`` (a leaky average of x).  Returns
+    (h [B,T,C] in x's dtype, the state after the last token [B,C] f32); the
+    arithmetic is f32.  Packed: x, g [1,R,C], state [N,C] (see the module).
+
+    T = 1 is the decode step.  ``inplace`` writes the new state over ``state``
+    and returns it (serving; no gradients).  g may be anything whose
+    exponential is wanted: -inf cuts off what came before.  Differentiable
+    in x, g and state, once.
+    """
+    what = "gated_scan"
+    _check_input(what, x)
+    if x.dim() != 3 or x.shape != g.shape:
+        raise ValueError(f"{what}: x and g must both be [B,T,C], got {list(x.shape)} and {list(g.shape)}")
+    if g.dtype != torch.float32 and g.dtype != x.dtype:
+        raise TypeError(f"{what}: g must be float32 or x's dtype {x.dtype}, got {g.dtype}")
+    _same_device(what, x.device, g, state)
+    cu = None if cu_seqlens is None else _cu_seqlens(what, cu_seqlens, x)
+    B, T, C = x.shape
+    n = B if cu is None else cu.numel() - 1
+    given, state = state, _f32(what, "state", state, (n, C))
+    x, g = _rows(x), _rows(g)
+    grads = torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (state is not None and state.requires_grad))
+    if inplace:
+        if given is None:
+            raise ValueError(f"{what}: inplace needs a state")
+        if grads:
+            raise ValueError(f"{what}: inplace does not go with gradients; detach the inputs or use torch.no_grad()")
+        if state is not given:
+            raise ValueError(f"{what}: inplace needs a contiguous state")
+    if n == 0 or C == 0 or (T == 0 and cu is None):  # nothing to launch: no token, or nothing in it
+        last = torch.zeros((n, C), dtype=torch.float32, device=x.device) if state is None else state
+        return x + g.to(x.dtype), last if inplace else last.clone()
+    if grads:
+        return _GatedScan.apply(x, g, state, cu, bool(complement))
+    last = state if inplace else torch.empty((n, C), dtype=torch.float32, device=x.device)
+    h, _ = _scan_forward(x, g, state, cu, complement, last, False)
+    return h, last

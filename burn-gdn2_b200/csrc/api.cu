@@ -50,6 +50,8 @@ int launch_short_conv(int B, int Tn, int C, int dtype, const void* x, const floa
 int launch_rms_norm_gate(const gdn2_dims& d, int dtype, const gdn2_view& o, const gdn2_view& gate, const float* w,
                          float eps, const gdn2_view& out, cudaStream_t st);
 int launch_project_activations(const gdn2_prologue_args* a, cudaStream_t st);
+int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, cudaStream_t st);
+int launch_scan_bwd(const gdn2_scan_bwd_args* a, cudaStream_t st);
 
 static int check_dims(const gdn2_dims& d, const char* fn) {
   if (d.batch <= 0 || d.seq_len <= 0 || d.num_heads <= 0 || d.num_v_heads <= 0 || d.head_k_dim <= 0 ||
@@ -402,6 +404,14 @@ int gdn2_rms_norm_gate(const gdn2_dims* dims, int32_t dtype, gdn2_view o, gdn2_v
     return set_error(GDN2_EINVAL, "gdn2_rms_norm_gate: unknown dtype %d", dtype);
   if (!o.data || !gate.data || !weight || !out.data) return set_error(GDN2_EINVAL, "gdn2_rms_norm_gate: null pointer");
   return launch_rms_norm_gate(*dims, dtype, o, gate, weight, eps, out, (cudaStream_t)stream);
+}
+
+int gdn2_gated_scan(const gdn2_scan_args* a, gdn2_view h, float* state_out, void* stream) {
+  return launch_scan_fwd(a, h, state_out, (cudaStream_t)stream);
+}
+
+int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* a, void* stream) {
+  return launch_scan_bwd(a, (cudaStream_t)stream);
 }
 
 int gdn2_config_validate(const gdn2_config* c, char* msg, size_t msg_len) {

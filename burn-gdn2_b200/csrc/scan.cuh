@@ -1,0 +1,106 @@
+// Pieces shared by the sequence operators (gated scan, short conv, group
+// norm): vector access to rows of channels, packed-sequence lookup and the
+// decay's exponential.
+#pragma once
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace gdn2 {
+
+// VEC consecutive elements of T as one memory access of sizeof(T) * VEC bytes.
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<2> { typedef unsigned short type; };
+template <>
+struct RawOf<4> { typedef unsigned type; };
+template <>
+struct RawOf<8> { typedef uint2 type; };
+template <>
+struct RawOf<16> { typedef uint4 type; };
+
+template <typename T, int VEC>
+struct Vec {
+  typedef typename RawOf<(int)sizeof(T) * VEC>::type Raw;
+  static __device__ __forceinline__ Raw load(const T* p) { return __ldcs(reinterpret_cast<const Raw*>(p)); }
+  static __device__ __forceinline__ void unpack(Raw r, float (&f)[VEC]) {
+    T e[VEC];
+    memcpy(e, &r, sizeof(r));
+    #pragma unroll
+    for (int v = 0; v < VEC; ++v) f[v] = to_f32<T>(e[v]);
+  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[VEC]) {
+    T e[VEC];
+    #pragma unroll
+    for (int v = 0; v < VEC; ++v) e[v] = from_f32<T>(f[v]);
+    Raw r;
+    memcpy(&r, e, sizeof(r));
+    return r;
+  }
+  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+    __stcs(reinterpret_cast<Raw*>(p), pack(f));
+  }
+};
+
+template <int VEC>
+__device__ __forceinline__ void load_f32(const float* p, float (&f)[VEC]) {
+  #pragma unroll
+  for (int v = 0; v < VEC; ++v) f[v] = p[v];
+}
+template <int VEC>
+__device__ __forceinline__ void store_f32(float* p, const float (&f)[VEC]) {
+  #pragma unroll
+  for (int v = 0; v < VEC; ++v) p[v] = f[v];
+}
+
+// Sequence of packed row t: the n with cu[n] <= t < cu[n + 1], or -1 for a
+// row outside every sequence.  Reads cu[0..N] only, whatever it holds, and
+// takes at most 32 halvings.
+__device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int N, int t) {
+  int lo = 0, hi = N + 1;  // first index whose entry is above t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(cu + mid) <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo >= 1 && lo <= N ? lo - 1 : -1;
+}
+
+// a = e^g and m = e^g - 1 of two log decays.  Argument reduction by powers of
+// two (Cody and Waite): g = n ln 2 + r with |r| <= ln 2 / 2, p = e^r - 1 by its
+// Taylor polynomial to r^7 (its first dropped term is below 2^-25 of p), then
+// a = 2^n (1 + p), m = 2^n p + (2^n - 1).  For n = 0 (the slow channels, whose
+// decay is applied thousands of times) a is 1 + p rounded once and m is p
+// itself, without the cancellation of 1 - a: an ulp of bias in a would grow
+// by the length of the channel's memory.  Valid for |g| <= 87; NaN stays NaN.
+__device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& m) {
+  const f32x2 kLog2e = f2pk(1.44269504088896f, 1.44269504088896f);
+  const f32x2 kMagic = f2pk(12582912.f, 12582912.f);  // 1.5 * 2^23: its sum rounds to a whole number
+  const f32x2 kOne = f2pk(1.f, 1.f), kMinus = f2pk(-1.f, -1.f);
+  const f32x2 t = f2fma(g, kLog2e, kMagic);
+  const f32x2 n = f2fma(kMagic, kMinus, t);
+  f32x2 r = f2fma(n, f2pk(-0.693145751953125f, -0.693145751953125f), g);
+  r = f2fma(n, f2pk(-1.42860677e-6f, -1.42860677e-6f), r);
+  f32x2 q = f2fma(r, f2pk(1.f / 5040, 1.f / 5040), f2pk(1.f / 720, 1.f / 720));
+  q = f2fma(q, r, f2pk(1.f / 120, 1.f / 120));
+  q = f2fma(q, r, f2pk(1.f / 24, 1.f / 24));
+  q = f2fma(q, r, f2pk(1.f / 6, 1.f / 6));
+  q = f2fma(q, r, f2pk(0.5f, 0.5f));
+  const f32x2 p = f2fma(f2mul(r, r), q, r);
+  float t0, t1;
+  f2un(t, t0, t1);
+  const f32x2 s = f2pk(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
+                       __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
+  a = f2fma(s, p, s);
+  m = f2fma(s, p, f2fma(s, kOne, kMinus));
+}
+__device__ __forceinline__ void exp_pair(float g0, float g1, float& a0, float& a1, float& m0, float& m1) {
+  f32x2 a, m;
+  exp_pair(f2pk(g0, g1), a, m);
+  f2un(a, a0, a1);
+  f2un(m, m0, m1);
+}
+constexpr float kExpRange = 87.f;
+
+}  // namespace gdn2

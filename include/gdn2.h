@@ -319,6 +319,57 @@ GDN2_API int gdn2_short_conv(int32_t batch, int32_t seq_len, int32_t channels, i
 GDN2_API int gdn2_rms_norm_gate(const gdn2_dims* dims, int32_t dtype, gdn2_view o, gdn2_view gate,
                        const float* weight, float eps, gdn2_view out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Gated scan: the diagonal gated linear recurrence, one state per channel
+ * (no counterpart in the reference, whose state is a K x V matrix per head):
+ *
+ *   h_t = e^{g_t} h_{t-1} + s_t x_t     s_t = 1, or 1 - e^{g_t} (complement)
+ *
+ *   x, h : [B, T, 1, C] views (dtype), channels contiguous, stride0 between
+ *          sequences, stride1 between tokens, stride2 unused
+ *   g    : the same, f32 or (with bf16 x) bf16: the log decay, any value
+ *          whose exponential is wanted (-inf cuts off what came before)
+ * Packed sequences: cu_seqlens (device, int32 [batch + 1], ascending from 0)
+ * gives sequence n the rows cu[n] .. cu[n+1] of one buffer of seq_len rows
+ * (stride0 unused); offsets beyond the buffer count as its end.  An empty
+ * sequence hands its state on.  Rows outside every sequence are not read
+ * into any result and come out as zero.
+ *   state_in  : [batch, C] f32 or NULL (zeros)
+ *   state_out : [batch, C] f32 or NULL; may be state_in
+ *   carry     : [batch (1 when packed), ceil(seq_len / 16), C] f32 or NULL:
+ *               the state before every 16th token, kept for the backward
+ * f32 arithmetic; h is rounded once.  No workspace, no atomics: results do
+ * not vary from call to call.
+ *
+ * gdn2_gated_scan_bwd: the adjoint.  fwd as it was given to the forward,
+ * with the carry that it wrote; d_h (dtype) and d_state_out (NULL = zeros)
+ * are the gradients of h and state_out; dx (dtype), dg (g_dtype) and
+ * d_state_in (f32, or NULL) are written.
+ * ---------------------------------------------------------------------- */
+typedef struct gdn2_scan_args {
+  int32_t batch;    /* sequences */
+  int32_t seq_len;  /* tokens of each, or rows of the packed buffer */
+  int32_t channels;
+  int32_t dtype;
+  int32_t g_dtype;
+  int32_t complement;
+  const int32_t* cu_seqlens; /* NULL: dense */
+  gdn2_view x, g;
+  const float* state_in;
+  float* carry;
+} gdn2_scan_args;
+
+typedef struct gdn2_scan_bwd_args {
+  gdn2_scan_args fwd;
+  gdn2_view d_h;
+  const float* d_state_out;
+  gdn2_view dx, dg;
+  float* d_state_in;
+} gdn2_scan_bwd_args;
+
+GDN2_API int gdn2_gated_scan(const gdn2_scan_args* args, gdn2_view h, float* state_out, void* stream);
+GDN2_API int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* args, void* stream);
+
 /* Mirror of Gdn2Config (src/config.rs:24-58) and its validate()
  * (src/config.rs:71-111).  num_v_heads < 0 means None; min_decay < 0
  * means None; mode 0 = FusedRecurrent, 1 = Chunk. */

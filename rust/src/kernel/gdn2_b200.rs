@@ -171,6 +171,35 @@ pub struct Gdn2PrologueArgs {
     pub g: *mut f32,
 }
 
+/// Gated scan (`gdn2_gated_scan`): x, g are `[B, T, 1, C]` views, or one packed buffer of `seq_len` rows with
+/// `cu_seqlens` on the device.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2ScanArgs {
+    pub batch: i32,
+    pub seq_len: i32,
+    pub channels: i32,
+    pub dtype: i32,
+    pub g_dtype: i32,
+    pub complement: i32,
+    pub cu_seqlens: *const i32,
+    pub x: Gdn2View,
+    pub g: Gdn2View,
+    pub state_in: *const f32,
+    pub carry: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2ScanBwdArgs {
+    pub fwd: Gdn2ScanArgs,
+    pub d_h: Gdn2View,
+    pub d_state_out: *const f32,
+    pub dx: Gdn2View,
+    pub dg: Gdn2View,
+    pub d_state_in: *mut f32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct Gdn2Config {
@@ -208,6 +237,8 @@ extern "C" {
                            stream: *mut c_void) -> i32;
     pub fn gdn2_rms_norm_gate(dims: *const Gdn2Dims, dtype: i32, o: Gdn2View, gate: Gdn2View, weight: *const f32,
                               eps: f32, out: Gdn2View, stream: *mut c_void) -> i32;
+    pub fn gdn2_gated_scan(args: *const Gdn2ScanArgs, h: Gdn2View, state_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn gdn2_gated_scan_bwd(args: *const Gdn2ScanBwdArgs, stream: *mut c_void) -> i32;
     pub fn gdn2_config_validate(cfg: *const Gdn2Config, msg: *mut c_char, msg_len: usize) -> i32;
     pub fn gdn2_read_device_errors(flags: *mut u32) -> i32;
     pub fn gdn2_selftest_umma(test: i32, a: *const f32, b: *const f32, d: *mut f32, stream: *mut c_void) -> i32;

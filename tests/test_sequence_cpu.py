@@ -1,0 +1,93 @@
+"""CPU: what the sequence operators refuse, before any launch, and their C
+entries' argument errors."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _fake(*shape, dtype=torch.float32):
+    """A tensor that says it is on a device: shapes and types without a GPU."""
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def test_refuses_cpu_tensors():
+    import burn_gdn2 as bg
+
+    x = torch.zeros(1, 4, 8)
+    with pytest.raises(RuntimeError, match="CPU tensor"):
+        bg.gated_scan(x, x)
+
+
+def test_packed_offsets_are_checked_on_the_host():
+    from burn_gdn2 import sequence
+
+    x = _fake(1, 10, 4)
+    for bad in ([1, 5], [0, 7, 3], [0, 11], [0, 4, 3, 9]):
+        with pytest.raises(ValueError, match="ascend"):
+            sequence._cu_seqlens("op", torch.tensor(bad, dtype=torch.int32), x)
+    for bad in (torch.tensor([0], dtype=torch.int32), torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([0.0, 1.0])):
+        with pytest.raises(ValueError, match="int32"):
+            sequence._cu_seqlens("op", bad, x)
+    with pytest.raises(ValueError, match="one buffer"):
+        sequence._cu_seqlens("op", torch.tensor([0, 3], dtype=torch.int32), _fake(2, 10, 4))
+
+
+def _scan_args(**over):
+    from burn_gdn2 import _lib
+
+    fake = 1 << 20  # never dereferenced: validation fails first
+    v = _lib.View(fake, 64, 8, 0)
+    a = _lib.ScanArgs(2, 8, 8, 0, 0, 0, None, v, v, None, None)
+    for k, val in over.items():
+        setattr(a, k, val)
+    return a
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(batch=0), 1), (dict(seq_len=-1), 1), (dict(seq_len=0), 1), (dict(channels=0), 1), (dict(dtype=7), 1),
+    (dict(g_dtype=-1), 1), (dict(g_dtype=1), 2), (dict(seq_len=(1 << 30) + 1), 2),
+])
+def test_scan_argument_errors(over, status):
+    from burn_gdn2 import LIB, _lib
+
+    out = _lib.View(1 << 20, 64, 8, 0)
+    a = _scan_args(**over)
+    assert LIB.gdn2_gated_scan(ctypes.byref(a), out, None, None) == status
+    assert LIB.gdn2_last_error().decode().startswith("gdn2_gated_scan:")
+    b = _lib.ScanBwdArgs(a, out, None, out, out, None)
+    assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None) == status
+
+
+def test_scan_null_pointers():
+    from burn_gdn2 import LIB, _lib
+
+    out, none = _lib.View(1 << 20, 64, 8, 0), _lib.View()
+    assert LIB.gdn2_gated_scan(None, out, None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan_bwd(None, None) == _lib.GDN2_EINVAL
+    a = _scan_args()
+    assert LIB.gdn2_gated_scan(ctypes.byref(a), none, None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan(ctypes.byref(_scan_args(x=none)), out, None, None) == _lib.GDN2_EINVAL
+    for args in ((a, none, out, out), (a, out, none, out), (a, out, out, none), (a, out, out, out)):  # the last: no carry
+        b = _lib.ScanBwdArgs(args[0], args[1], None, args[2], args[3], None)
+        assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None) == _lib.GDN2_EINVAL
+
+
+def test_struct_layouts_match_header(tmp_path):
+    import os
+    import subprocess
+
+    from burn_gdn2 import _lib
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {"gdn2_scan_args": _lib.ScanArgs, "gdn2_scan_bwd_args": _lib.ScanBwdArgs}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "gdn2.h"', "int main() {"]
+    for c, s in names.items():
+        lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
+        lines += [f'printf("{c} {f} %zu\\n", offsetof({c}, {f}));' for f, _ in s._fields_]
+    src, exe = tmp_path / "p.c", tmp_path / "p"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        c, f, v = line.split()
+        assert int(v) == (ctypes.sizeof(names[c]) if f == "size" else getattr(names[c], f).offset), (c, f)
