@@ -94,6 +94,20 @@ class ScanBwdArgs(ctypes.Structure):
                 ("d_state_in", ctypes.c_void_p)]
 
 
+class GroupNormArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("groups", ctypes.c_int32), ("width", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("center", ctypes.c_int32), ("weight_shared", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64),
+                ("gate", ctypes.c_void_p), ("ld_gate", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p)]
+
+
+class GroupNormBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", GroupNormArgs), ("d_y", ctypes.c_void_p), ("ld_dy", ctypes.c_int64),
+                ("dx", ctypes.c_void_p), ("d_gate", ctypes.c_void_p), ("d_weight", ctypes.c_void_p),
+                ("d_bias", ctypes.c_void_p)]
+
+
 class Config(ctypes.Structure):
     _fields_ = [("hidden_size", ctypes.c_int64), ("num_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
                 ("expand_v", ctypes.c_float), ("num_v_heads", ctypes.c_int64), ("use_short_conv", ctypes.c_int32),
@@ -109,6 +123,7 @@ EXPORTS = (
     "gdn2_selftest_umma", "gdn2_chunk_fwd_noalloc", "gdn2_project_activations", "gdn2_selftest_wait",
     "gdn2_set_reserved_sms", "gdn2_recurrent_bwd_workspace_bytes", "gdn2_recurrent_bwd",
     "gdn2_chunk_trajectory", "gdn2_gated_scan", "gdn2_gated_scan_bwd",
+    "gdn2_group_norm_gate", "gdn2_group_norm_gate_bwd_workspace_bytes", "gdn2_group_norm_gate_bwd",
 )
 
 
@@ -139,6 +154,12 @@ def _load():
     lib.gdn2_gated_scan.restype = ctypes.c_int
     lib.gdn2_gated_scan_bwd.argtypes = [P(ScanBwdArgs), vp]
     lib.gdn2_gated_scan_bwd.restype = ctypes.c_int
+    lib.gdn2_group_norm_gate.argtypes = [P(GroupNormArgs), vp, vp]
+    lib.gdn2_group_norm_gate.restype = ctypes.c_int
+    lib.gdn2_group_norm_gate_bwd_workspace_bytes.argtypes = [P(GroupNormBwdArgs)]
+    lib.gdn2_group_norm_gate_bwd_workspace_bytes.restype = sz
+    lib.gdn2_group_norm_gate_bwd.argtypes = [P(GroupNormBwdArgs), vp, sz, vp]
+    lib.gdn2_group_norm_gate_bwd.restype = ctypes.c_int
     lib.gdn2_short_conv.argtypes = [i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]
     lib.gdn2_short_conv.restype = ctypes.c_int
     lib.gdn2_rms_norm_gate.argtypes = [P(Dims), i32, View, View, vp, f32, View, vp]

@@ -1,6 +1,7 @@
 """Sequence operators around a gated recurrence, for training and serving.
 
   gated_scan        the diagonal gated linear recurrence h_t = e^{g_t} h_{t-1} + s_t x_t
+  group_norm_gate   the norm of each token's channel groups behind it, with an affine map and a SiLU
 
 Every operator takes CUDA tensors on any device and launches on that device's
 current stream; it is differentiable where an input requires a gradient, and
@@ -182,3 +183,86 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
     last = state if inplace else torch.empty((n, C), dtype=torch.float32, device=x.device)
     h, _ = _scan_forward(x, g, state, cu, complement, last, False)
     return h, last
+
+
+# -- group norm ----------------------------------------------------------------
+
+
+def _norm_args(x, gate, weight, bias, groups, eps, center):
+    rows, chan = x.shape
+    shared = weight is not None and weight.numel() != chan
+    return _lib.GroupNormArgs(rows, groups, chan // groups, _DT[x.dtype], int(center), int(shared), eps, x.data_ptr(),
+                              x.stride(0), _ptr(gate), 0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias))
+
+
+def _norm_forward(x, gate, weight, bias, groups, eps, center):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.shape[0]:
+        a = _norm_args(x, gate, weight, bias, groups, eps, center)
+        with _on(x.device):
+            check(LIB.gdn2_group_norm_gate(ctypes.byref(a), y.data_ptr(), _stream(x.device)))
+    return y
+
+
+class _GroupNormGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, weight, bias, groups, eps, center):
+        ctx.save_for_backward(x, gate, weight, bias)
+        ctx.rest = (groups, eps, center)
+        return _norm_forward(x, gate, weight, bias, groups, eps, center)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_y):
+        x, gate, weight, bias = ctx.saved_tensors
+        d_y = _rows(d_y)
+        new = lambda k, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if ctx.needs_input_grad[k] else None
+        dx, d_gate, d_weight, d_bias = (new(k, t) for k, t in enumerate((x, gate, weight, bias)))
+        if not x.shape[0]:
+            return (dx, d_gate, *(None if t is None else t.zero_() for t in (d_weight, d_bias)), None, None, None)
+        a = _lib.GroupNormBwdArgs(_norm_args(x, gate, weight, bias, *ctx.rest), d_y.data_ptr(), d_y.stride(0),
+                                  _ptr(dx), _ptr(d_gate), _ptr(d_weight), _ptr(d_bias))
+        with _on(x.device):
+            size = LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(a))
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            check(LIB.gdn2_group_norm_gate_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
+        return dx, d_gate, d_weight, d_bias, None, None, None
+
+
+def group_norm_gate(x, gate=None, weight=None, bias=None, *, num_groups: int, eps: float = 1e-5, center: bool = True):
+    """Norm of each token's channel groups, an affine map and a SiLU.
+
+    x [..., C] (f32 or bf16, channels last): each token's C channels are
+    num_groups groups of C / num_groups, each brought to mean 0 and variance 1
+    (``center=False``: to root mean square 1), z = n weight + bias, and
+    y = z silu(gate), or silu(z) without a gate.  gate: x's shape and dtype.
+    weight, bias: f32 [C], or [C / num_groups] for all groups alike, or None.
+    With ``center=False``, a gate and a weight per head this is
+    rms_norm_gate_per_head on [..., HV*V], with gradients.  f32 arithmetic;
+    differentiable in x, gate, weight and bias, once.
+    """
+    what = "group_norm_gate"
+    _check_input(what, x)
+    if x.dim() < 1 or num_groups < 1 or x.shape[-1] == 0 or x.shape[-1] % num_groups:
+        raise ValueError(f"{what}: the {x.shape[-1] if x.dim() else 0} channels do not split into {num_groups} groups")
+    if not eps > 0:
+        raise ValueError(f"{what}: eps must be > 0, got {eps}")
+    _same_device(what, x.device, gate, weight, bias)
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        raise ValueError(f"{what}: gate must be {list(x.shape)} {x.dtype}, got {list(gate.shape)} {gate.dtype}")
+    shape, chan = x.shape, x.shape[-1]
+    width = chan // num_groups
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.dim() != 1 or t.numel() not in (chan, width)):
+            raise ValueError(f"{what}: {name} must be [{chan}] or [{width}], got {list(t.shape)}")
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
+    if bias is not None and (weight is None or weight.shape != bias.shape):
+        raise ValueError(f"{what}: a bias goes with a weight of its shape")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    flat = lambda t: None if t is None else _rows(t.reshape(-1, chan))
+    args = (flat(x), flat(gate), weight, bias, int(num_groups), float(eps), bool(center))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias)):
+        return _GroupNormGate.apply(*args).reshape(shape)
+    return _norm_forward(*args).reshape(shape)

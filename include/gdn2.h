@@ -370,6 +370,58 @@ typedef struct gdn2_scan_bwd_args {
 GDN2_API int gdn2_gated_scan(const gdn2_scan_args* args, gdn2_view h, float* state_out, void* stream);
 GDN2_API int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Group norm of each token's channels with an affine map and a SiLU, and
+ * its backward; gdn2_rms_norm_gate (rms_norm_gate_per_head,
+ * src/module.rs:501-517) is the case center = 0 with weight_shared = 1:
+ *
+ *   n = (x - mean) / sqrt(mean((x - mean)^2) + eps)   over each group of
+ *       `width` channels of a row; center = 0: mean taken as 0
+ *   z = n weight + bias,   y = z silu(gate),  or silu(z) when gate is NULL
+ *
+ *   x, gate : [rows][ld_*] (dtype), channel c of a row at column c
+ *   weight, bias : [groups * width] f32, or [width] for all groups with
+ *             weight_shared = 1; NULL = 1 and 0
+ *   y       : [rows][groups * width] contiguous (dtype)
+ * Up to 1024 * v channels a group, v = 4, 2 or 1 the most elements that width,
+ * pointers and pitches are multiples of.
+ * Backward: d_y [rows][ld_dy]; dx, d_gate contiguous (dtype), d_weight and
+ * d_bias f32 as the weights, each NULL where it is not wanted.  The
+ * workspace (16-byte aligned, gdn2_group_norm_gate_bwd_workspace_bytes; 0
+ * without d_weight and d_bias) holds partial sums of the weights' gradients,
+ * added in a fixed order.
+ * ---------------------------------------------------------------------- */
+typedef struct gdn2_group_norm_args {
+  int64_t rows;
+  int32_t groups;
+  int32_t width;
+  int32_t dtype;
+  int32_t center;
+  int32_t weight_shared;
+  float eps;
+  const void* x;
+  int64_t ld_x;
+  const void* gate;
+  int64_t ld_gate;
+  const float* weight;
+  const float* bias;
+} gdn2_group_norm_args;
+
+typedef struct gdn2_group_norm_bwd_args {
+  gdn2_group_norm_args fwd;
+  const void* d_y;
+  int64_t ld_dy;
+  void* dx;
+  void* d_gate;
+  float* d_weight;
+  float* d_bias;
+} gdn2_group_norm_bwd_args;
+
+GDN2_API int gdn2_group_norm_gate(const gdn2_group_norm_args* args, void* y, void* stream);
+GDN2_API size_t gdn2_group_norm_gate_bwd_workspace_bytes(const gdn2_group_norm_bwd_args* args);
+GDN2_API int gdn2_group_norm_gate_bwd(const gdn2_group_norm_bwd_args* args, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
 /* Mirror of Gdn2Config (src/config.rs:24-58) and its validate()
  * (src/config.rs:71-111).  num_v_heads < 0 means None; min_decay < 0
  * means None; mode 0 = FusedRecurrent, 1 = Chunk. */

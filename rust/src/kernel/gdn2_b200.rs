@@ -200,6 +200,37 @@ pub struct Gdn2ScanBwdArgs {
     pub d_state_in: *mut f32,
 }
 
+/// Group norm with SiLU (`gdn2_group_norm_gate`), statistics per row and group of `width` channels.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2GroupNormArgs {
+    pub rows: i64,
+    pub groups: i32,
+    pub width: i32,
+    pub dtype: i32,
+    pub center: i32,
+    pub weight_shared: i32,
+    pub eps: f32,
+    pub x: *const c_void,
+    pub ld_x: i64,
+    pub gate: *const c_void,
+    pub ld_gate: i64,
+    pub weight: *const f32,
+    pub bias: *const f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2GroupNormBwdArgs {
+    pub fwd: Gdn2GroupNormArgs,
+    pub d_y: *const c_void,
+    pub ld_dy: i64,
+    pub dx: *mut c_void,
+    pub d_gate: *mut c_void,
+    pub d_weight: *mut f32,
+    pub d_bias: *mut f32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct Gdn2Config {
@@ -239,6 +270,10 @@ extern "C" {
                               eps: f32, out: Gdn2View, stream: *mut c_void) -> i32;
     pub fn gdn2_gated_scan(args: *const Gdn2ScanArgs, h: Gdn2View, state_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn gdn2_gated_scan_bwd(args: *const Gdn2ScanBwdArgs, stream: *mut c_void) -> i32;
+    pub fn gdn2_group_norm_gate(args: *const Gdn2GroupNormArgs, y: *mut c_void, stream: *mut c_void) -> i32;
+    pub fn gdn2_group_norm_gate_bwd_workspace_bytes(args: *const Gdn2GroupNormBwdArgs) -> usize;
+    pub fn gdn2_group_norm_gate_bwd(args: *const Gdn2GroupNormBwdArgs, workspace: *mut c_void, workspace_bytes: usize,
+                                    stream: *mut c_void) -> i32;
     pub fn gdn2_config_validate(cfg: *const Gdn2Config, msg: *mut c_char, msg_len: usize) -> i32;
     pub fn gdn2_read_device_errors(flags: *mut u32) -> i32;
     pub fn gdn2_selftest_umma(test: i32, a: *const f32, b: *const f32, d: *mut f32, stream: *mut c_void) -> i32;

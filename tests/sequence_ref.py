@@ -74,6 +74,73 @@ def scan(x, g, state, lens, comp, d_h=None, d_state=None):
     return out, tol
 
 
+def silu_parts(t):
+    """sigmoid, silu, silu' and the absolute errors of the last two for an exact t: the fast exponential is within
+    (4 + 2 |t|) EPS, the fast division within 4 EPS, relative."""
+    sig = torch.sigmoid(t)
+    act, slope = t * sig, sig * (1 + t * (1 - sig))
+    rel = (16 + 2 * t.abs()) * EPS
+    return act, slope, rel * act.abs(), rel * sig * (1 + 2 * t.abs())
+
+
+def group_norm(x, gate, weight, bias, groups, eps, center, d=None):
+    """[R,C] group norm with SiLU and its adjoint, with bounds.
+
+    Sums over a group run at most 50 deep (16 values a lane, then trees), so a mean is off by 50 EPS of the mean
+    size A.  A deviation is off by that and its own rounding; rstd, relative, by half the variance's error (twice
+    the deviations' over sigma, and the sum's) and the root's 4 EPS.  Weight gradients are sums over the rows, at
+    most one addition a row deep."""
+    f64 = lambda t: None if t is None else t.double()
+    x, gate, weight, bias, d = (f64(t) for t in (x, gate, weight, bias, d))
+    rows, chan = x.shape
+    per = lambda t: t.reshape(rows, groups, -1)
+    wide = lambda t, default: torch.full((1, 1), default, dtype=torch.float64) if t is None else t.reshape(-1, chan // groups)
+    v, w, b = per(x), wide(weight, 1.0), wide(bias, 0.0)
+    A = v.abs().mean(-1, keepdim=True)
+    dev = v - v.mean(-1, keepdim=True) if center else v
+    e_dev = (50 * EPS * A if center else 0) + 2 * EPS * dev.abs()
+    rstd = ((dev * dev).mean(-1, keepdim=True) + eps).rsqrt()
+    rel_r = (50 * A * rstd if center else 0) * EPS + 31 * EPS
+    n = dev * rstd
+    e_n = rstd * e_dev + n.abs() * (rel_r + EPS)
+    z = n * w + b
+    e_z = w.abs() * e_n + 2 * EPS * ((n * w).abs() + b.abs())
+    t = z if gate is None else per(gate)
+    act, slope, e_act, e_slope = silu_parts(t)
+    if gate is None:
+        y, e_y = act, e_act + 1.1 * e_z + EPS * act.abs()
+    else:
+        y, e_y = z * act, z.abs() * e_act + act.abs() * e_z + 2 * EPS * (z * act).abs()
+    flat = lambda t: t.reshape(rows, chan)
+    out, tol = {"y": flat(y)}, {"y": flat(e_y)}
+    if d is None:
+        return out, tol
+    d = per(d)
+    if gate is None:
+        dz, e_dz = d * slope, d.abs() * (e_slope + 0.5 * e_z) + EPS * (d * slope).abs()
+    else:
+        dz, e_dz = d * act, d.abs() * e_act + EPS * (d * act).abs()
+        out["d_gate"] = flat(d * z * slope)
+        tol["d_gate"] = flat(d.abs() * (e_z * slope.abs() + z.abs() * e_slope) + 3 * EPS * (d * z * slope).abs())
+    dn = dz * w
+    e_dn = w.abs() * e_dz + EPS * dn.abs()
+    mean = lambda t: t.mean(-1, keepdim=True)
+    m0, e_m0 = (mean(dn), mean(e_dn) + 50 * EPS * mean(dn.abs())) if center else (0, 0)
+    m1 = mean(dn * n)
+    e_m1 = mean(e_dn * n.abs() + dn.abs() * e_n) + 50 * EPS * mean((dn * n).abs())
+    dx = rstd * (dn - m0 - n * m1)
+    size = dn.abs() + (m0.abs() if center else 0) + (n * m1).abs()
+    out["dx"] = flat(dx)
+    tol["dx"] = flat(rstd * (e_dn + e_m0 + n.abs() * e_m1 + e_n * m1.abs() + 3 * EPS * size) + dx.abs() * (rel_r + EPS))
+    for name, given, g, e in (("d_weight", weight, dz * n, e_dz * n.abs() + dz.abs() * e_n), ("d_bias", bias, dz, e_dz)):
+        if given is not None:
+            over = (0,) if given.numel() == chan else (0, 1)
+            deep = (rows if given.numel() == chan else rows * groups) + 8
+            out[name] = g.sum(over).reshape(given.shape)
+            tol[name] = (e.sum(over) + deep * EPS * g.abs().sum(over)).reshape(given.shape)
+    return out, tol
+
+
 def check(got, want, bound, what):
     """got (any dtype) within the bound of f32 arithmetic plus one rounding to its dtype."""
     assert got.shape == want.shape, (what, got.shape, want.shape)

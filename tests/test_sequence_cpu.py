@@ -80,7 +80,8 @@ def test_struct_layouts_match_header(tmp_path):
     from burn_gdn2 import _lib
 
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    names = {"gdn2_scan_args": _lib.ScanArgs, "gdn2_scan_bwd_args": _lib.ScanBwdArgs}
+    names = {"gdn2_scan_args": _lib.ScanArgs, "gdn2_scan_bwd_args": _lib.ScanBwdArgs,
+             "gdn2_group_norm_args": _lib.GroupNormArgs, "gdn2_group_norm_bwd_args": _lib.GroupNormBwdArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "gdn2.h"', "int main() {"]
     for c, s in names.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
@@ -91,3 +92,51 @@ def test_struct_layouts_match_header(tmp_path):
     for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
         c, f, v = line.split()
         assert int(v) == (ctypes.sizeof(names[c]) if f == "size" else getattr(names[c], f).offset), (c, f)
+
+
+def _norm_args(**over):
+    from burn_gdn2 import _lib
+
+    fake = 1 << 20
+    a = _lib.GroupNormArgs(4, 2, 16, 0, 1, 0, 1e-5, fake, 32, fake, 32, fake, fake)
+    for k, val in over.items():
+        setattr(a, k, val)
+    return a
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(rows=0), 1), (dict(groups=0), 1), (dict(width=-4), 1), (dict(dtype=2), 1), (dict(eps=0.0), 1),
+    (dict(eps=float("nan")), 1), (dict(x=None), 1), (dict(width=4100), 2), (dict(width=1025), 2),
+    (dict(groups=1 << 20, width=1 << 12), 2),
+])
+def test_group_norm_argument_errors(over, status):
+    from burn_gdn2 import LIB, _lib
+
+    fake = 1 << 20
+    a = _norm_args(**over)
+    assert LIB.gdn2_group_norm_gate(ctypes.byref(a), fake, None) == status
+    assert LIB.gdn2_last_error().decode().startswith("gdn2_group_norm_gate:")
+    b = _lib.GroupNormBwdArgs(a, fake, 32, fake, fake, fake, fake)
+    assert LIB.gdn2_group_norm_gate_bwd(ctypes.byref(b), fake, 1 << 30, None) == status
+    assert LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(b)) == 0
+
+
+def test_group_norm_null_pointers_and_workspace():
+    from burn_gdn2 import LIB, _lib
+
+    fake = 1 << 20
+    assert LIB.gdn2_group_norm_gate(None, fake, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_group_norm_gate(ctypes.byref(_norm_args()), None, None) == _lib.GDN2_EINVAL
+    bwd = lambda a, *rest: _lib.GroupNormBwdArgs(a, *rest)
+    call = lambda b, ws=None, n=0: LIB.gdn2_group_norm_gate_bwd(ctypes.byref(b), ws, n, None)
+    assert LIB.gdn2_group_norm_gate_bwd(None, None, 0, None) == _lib.GDN2_EINVAL
+    assert call(bwd(_norm_args(), None, 32, fake, fake, None, None)) == _lib.GDN2_EINVAL
+    for absent, rest in ((dict(gate=None), (fake, fake, None, None)), (dict(weight=None), (fake, None, fake, None)),
+                         (dict(bias=None), (fake, None, None, fake))):
+        assert call(bwd(_norm_args(**absent), fake, 32, *rest)) == _lib.GDN2_EINVAL
+    b = bwd(_norm_args(), fake, 32, fake, fake, fake, fake)
+    need = LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(b))
+    assert need > 0 and need % (2 * 32 * 4) == 0
+    assert call(b, fake, need - 1) == _lib.GDN2_EWORKSPACE
+    assert call(b) == _lib.GDN2_EWORKSPACE
+    assert LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(bwd(_norm_args(), fake, 32, fake, fake, None, None))) == 0
