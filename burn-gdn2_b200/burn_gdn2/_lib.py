@@ -94,6 +94,17 @@ class ScanBwdArgs(ctypes.Structure):
                 ("d_state_in", ctypes.c_void_p)]
 
 
+class ConvArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("seq_len", ctypes.c_int32), ("channels", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("cu_seqlens", ctypes.c_void_p), ("x", View), ("weight", ctypes.c_void_p),
+                ("cache_in", ctypes.c_void_p)]
+
+
+class ConvBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", ConvArgs), ("d_y", View), ("d_cache_out", ctypes.c_void_p), ("dx", View),
+                ("d_weight", ctypes.c_void_p), ("d_cache_in", ctypes.c_void_p)]
+
+
 class GroupNormArgs(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("groups", ctypes.c_int32), ("width", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("center", ctypes.c_int32), ("weight_shared", ctypes.c_int32),
@@ -124,6 +135,7 @@ EXPORTS = (
     "gdn2_set_reserved_sms", "gdn2_recurrent_bwd_workspace_bytes", "gdn2_recurrent_bwd",
     "gdn2_chunk_trajectory", "gdn2_gated_scan", "gdn2_gated_scan_bwd",
     "gdn2_group_norm_gate", "gdn2_group_norm_gate_bwd_workspace_bytes", "gdn2_group_norm_gate_bwd",
+    "gdn2_causal_conv", "gdn2_causal_conv_bwd_workspace_bytes", "gdn2_causal_conv_bwd",
 )
 
 
@@ -154,6 +166,12 @@ def _load():
     lib.gdn2_gated_scan.restype = ctypes.c_int
     lib.gdn2_gated_scan_bwd.argtypes = [P(ScanBwdArgs), vp]
     lib.gdn2_gated_scan_bwd.restype = ctypes.c_int
+    lib.gdn2_causal_conv.argtypes = [P(ConvArgs), View, vp, vp]
+    lib.gdn2_causal_conv.restype = ctypes.c_int
+    lib.gdn2_causal_conv_bwd_workspace_bytes.argtypes = [P(ConvBwdArgs)]
+    lib.gdn2_causal_conv_bwd_workspace_bytes.restype = sz
+    lib.gdn2_causal_conv_bwd.argtypes = [P(ConvBwdArgs), vp, sz, vp]
+    lib.gdn2_causal_conv_bwd.restype = ctypes.c_int
     lib.gdn2_group_norm_gate.argtypes = [P(GroupNormArgs), vp, vp]
     lib.gdn2_group_norm_gate.restype = ctypes.c_int
     lib.gdn2_group_norm_gate_bwd_workspace_bytes.argtypes = [P(GroupNormBwdArgs)]

@@ -1,6 +1,7 @@
 """Sequence operators around a gated recurrence, for training and serving.
 
   gated_scan        the diagonal gated linear recurrence h_t = e^{g_t} h_{t-1} + s_t x_t
+  causal_conv_silu  the 4-tap causal convolution with SiLU in front of it
   group_norm_gate   the norm of each token's channel groups behind it, with an affine map and a SiLU
 
 Every operator takes CUDA tensors on any device and launches on that device's
@@ -22,7 +23,7 @@ import torch
 
 from . import _lib
 from ._lib import LIB, check
-from .ops import _DT, dtype_code
+from .ops import SHORT_CONV_CACHE, SHORT_CONV_KERNEL, _DT
 
 SCAN_CARRY = 16  # tokens between the states that gated_scan keeps for its backward
 
@@ -183,6 +184,79 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
     last = state if inplace else torch.empty((n, C), dtype=torch.float32, device=x.device)
     h, _ = _scan_forward(x, g, state, cu, complement, last, False)
     return h, last
+
+
+# -- causal convolution --------------------------------------------------------
+
+
+def _conv_args(x, weight, cache, cu):
+    return _lib.ConvArgs(x.shape[0] if cu is None else cu.numel() - 1, x.shape[1], x.shape[2], _DT[x.dtype], _ptr(cu),
+                         _view3(x), weight.data_ptr(), _ptr(cache))
+
+
+def _conv_forward(x, weight, cache, cu):
+    n = x.shape[0] if cu is None else cu.numel() - 1
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    new = torch.empty((n, SHORT_CONV_CACHE, x.shape[2]), dtype=torch.float32, device=x.device)
+    a = _conv_args(x, weight, cache, cu)
+    with _on(x.device):
+        check(LIB.gdn2_causal_conv(ctypes.byref(a), _view3(y), new.data_ptr(), _stream(x.device)))
+    return y, new
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, cache, cu):
+        ctx.save_for_backward(x, weight, cache, cu)
+        ctx.set_materialize_grads(False)
+        return _conv_forward(x, weight, cache, cu)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_y, d_new):
+        x, weight, cache, cu = ctx.saved_tensors
+        d_y = torch.zeros_like(x) if d_y is None else _rows(d_y)
+        d_new = None if d_new is None else d_new.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        d_cache = torch.empty_like(cache) if cache is not None and ctx.needs_input_grad[2] else None
+        a = _lib.ConvBwdArgs(_conv_args(x, weight, cache, cu), _view3(d_y), _ptr(d_new), _view3(dx), _ptr(d_weight),
+                             _ptr(d_cache))
+        with _on(x.device):
+            size = LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(a))
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            check(LIB.gdn2_causal_conv_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
+        return dx, d_weight, d_cache, None
+
+
+def causal_conv_silu(x, weight, cache=None, *, cu_seqlens=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """short_conv_1d with gradients and packed sequences: the causal depthwise
+    convolution of 4 taps and its SiLU, y_t = silu(sum_j w[:, j] x_{t-3+j}).
+
+    x [B,T,C] (f32 or bf16); weight [C,4] f32; cache [B,3,C] f32, the three
+    values before each sequence, or None: copies of its first token
+    (src/short_conv.rs:42-54).  Returns (y [B,T,C], the new cache [B,3,C] f32:
+    the last three values).  Packed: x [1,R,C], caches [N,3,C] (see the
+    module); an empty sequence keeps its cache (zeros without one).  T = 1 is
+    the decode step.  f32 arithmetic; differentiable in x, weight and cache,
+    once.
+    """
+    what = "causal_conv_silu"
+    _check_input(what, x)
+    if x.dim() != 3:
+        raise ValueError(f"{what}: x must be [B,T,C], got {list(x.shape)}")
+    _same_device(what, x.device, weight, cache)
+    cu = None if cu_seqlens is None else _cu_seqlens(what, cu_seqlens, x)
+    B, T, C = x.shape
+    n = B if cu is None else cu.numel() - 1
+    weight = _f32(what, "weight", weight, (C, SHORT_CONV_KERNEL))
+    cache = _f32(what, "cache", cache, (n, SHORT_CONV_CACHE, C))
+    x = _rows(x)
+    if n == 0 or C == 0 or (T == 0 and cu is None):  # nothing to launch: no token, or nothing in it
+        return x * weight[:, 0], torch.zeros((n, SHORT_CONV_CACHE, C), device=x.device) if cache is None else cache.clone()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, cache)):
+        return _CausalConv.apply(x, weight, cache, cu)
+    return _conv_forward(x, weight, cache, cu)
 
 
 # -- group norm ----------------------------------------------------------------

@@ -52,6 +52,9 @@ int launch_rms_norm_gate(const gdn2_dims& d, int dtype, const gdn2_view& o, cons
 int launch_project_activations(const gdn2_prologue_args* a, cudaStream_t st);
 int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, cudaStream_t st);
 int launch_scan_bwd(const gdn2_scan_bwd_args* a, cudaStream_t st);
+int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_out, cudaStream_t st);
+size_t conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* a);
+int launch_conv_bwd(const gdn2_conv_bwd_args* a, void* ws, size_t ws_bytes, cudaStream_t st);
 int launch_group_norm(const gdn2_group_norm_args* a, void* y, cudaStream_t st);
 size_t group_norm_bwd_workspace_bytes(const gdn2_group_norm_bwd_args* a);
 int launch_group_norm_bwd(const gdn2_group_norm_bwd_args* a, void* ws, size_t ws_bytes, cudaStream_t st);
@@ -415,6 +418,16 @@ int gdn2_gated_scan(const gdn2_scan_args* a, gdn2_view h, float* state_out, void
 
 int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* a, void* stream) {
   return launch_scan_bwd(a, (cudaStream_t)stream);
+}
+
+int gdn2_causal_conv(const gdn2_conv_args* a, gdn2_view y, float* cache_out, void* stream) {
+  return launch_conv_fwd(a, y, cache_out, (cudaStream_t)stream);
+}
+
+size_t gdn2_causal_conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* a) { return conv_bwd_workspace_bytes(a); }
+
+int gdn2_causal_conv_bwd(const gdn2_conv_bwd_args* a, void* ws, size_t ws_bytes, void* stream) {
+  return launch_conv_bwd(a, ws, ws_bytes, (cudaStream_t)stream);
 }
 
 int gdn2_group_norm_gate(const gdn2_group_norm_args* a, void* y, void* stream) {

@@ -371,6 +371,50 @@ GDN2_API int gdn2_gated_scan(const gdn2_scan_args* args, gdn2_view h, float* sta
 GDN2_API int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Causal depthwise convolution of 4 taps with SiLU, with its backward and
+ * packed sequences; gdn2_short_conv (src/short_conv.rs:22-65) is its dense
+ * forward on contiguous tensors:
+ *
+ *   y_t = silu(sum_j weight[c][j] x_{t-3+j})
+ *
+ *   x, y   : [B, T, 1, C] views (dtype), packed with cu_seqlens as
+ *            gdn2_gated_scan's (rows outside every sequence come out as zero)
+ *   weight : [C, 4] f32
+ *   cache_in  : [batch, 3, C] f32, the three values before each sequence, or
+ *               NULL: copies of its first token (src/short_conv.rs:42-54)
+ *   cache_out : [batch, 3, C] f32 or NULL: its last three values; an empty
+ *               sequence hands cache_in on (zeros without one).  May be
+ *               cache_in for a dense call of at most 16 tokens.
+ * Backward: d_y and d_cache_out (NULL = zeros) in; dx (dtype), d_weight f32
+ * or NULL, d_cache_in f32 or NULL out.  The workspace
+ * (gdn2_causal_conv_bwd_workspace_bytes; 0 without d_weight) holds partial
+ * sums of d_weight, added in a fixed order.
+ * ---------------------------------------------------------------------- */
+typedef struct gdn2_conv_args {
+  int32_t batch;   /* sequences */
+  int32_t seq_len; /* tokens of each, or rows of the packed buffer */
+  int32_t channels;
+  int32_t dtype;
+  const int32_t* cu_seqlens; /* NULL: dense */
+  gdn2_view x;
+  const float* weight;
+  const float* cache_in;
+} gdn2_conv_args;
+
+typedef struct gdn2_conv_bwd_args {
+  gdn2_conv_args fwd;
+  gdn2_view d_y;
+  const float* d_cache_out;
+  gdn2_view dx;
+  float* d_weight;
+  float* d_cache_in;
+} gdn2_conv_bwd_args;
+
+GDN2_API int gdn2_causal_conv(const gdn2_conv_args* args, gdn2_view y, float* cache_out, void* stream);
+GDN2_API size_t gdn2_causal_conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* args);
+GDN2_API int gdn2_causal_conv_bwd(const gdn2_conv_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Group norm of each token's channels with an affine map and a SiLU, and
  * its backward; gdn2_rms_norm_gate (rms_norm_gate_per_head,
  * src/module.rs:501-517) is the case center = 0 with weight_shared = 1:

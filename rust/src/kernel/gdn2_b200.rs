@@ -200,6 +200,31 @@ pub struct Gdn2ScanBwdArgs {
     pub d_state_in: *mut f32,
 }
 
+/// Causal convolution of 4 taps with SiLU (`gdn2_causal_conv`), views and packing as [`Gdn2ScanArgs`].
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2ConvArgs {
+    pub batch: i32,
+    pub seq_len: i32,
+    pub channels: i32,
+    pub dtype: i32,
+    pub cu_seqlens: *const i32,
+    pub x: Gdn2View,
+    pub weight: *const f32,
+    pub cache_in: *const f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2ConvBwdArgs {
+    pub fwd: Gdn2ConvArgs,
+    pub d_y: Gdn2View,
+    pub d_cache_out: *const f32,
+    pub dx: Gdn2View,
+    pub d_weight: *mut f32,
+    pub d_cache_in: *mut f32,
+}
+
 /// Group norm with SiLU (`gdn2_group_norm_gate`), statistics per row and group of `width` channels.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -270,6 +295,10 @@ extern "C" {
                               eps: f32, out: Gdn2View, stream: *mut c_void) -> i32;
     pub fn gdn2_gated_scan(args: *const Gdn2ScanArgs, h: Gdn2View, state_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn gdn2_gated_scan_bwd(args: *const Gdn2ScanBwdArgs, stream: *mut c_void) -> i32;
+    pub fn gdn2_causal_conv(args: *const Gdn2ConvArgs, y: Gdn2View, cache_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn gdn2_causal_conv_bwd_workspace_bytes(args: *const Gdn2ConvBwdArgs) -> usize;
+    pub fn gdn2_causal_conv_bwd(args: *const Gdn2ConvBwdArgs, workspace: *mut c_void, workspace_bytes: usize,
+                                stream: *mut c_void) -> i32;
     pub fn gdn2_group_norm_gate(args: *const Gdn2GroupNormArgs, y: *mut c_void, stream: *mut c_void) -> i32;
     pub fn gdn2_group_norm_gate_bwd_workspace_bytes(args: *const Gdn2GroupNormBwdArgs) -> usize;
     pub fn gdn2_group_norm_gate_bwd(args: *const Gdn2GroupNormBwdArgs, workspace: *mut c_void, workspace_bytes: usize,

@@ -141,6 +141,64 @@ def group_norm(x, gate, weight, bias, groups, eps, center, d=None):
     return out, tol
 
 
+def conv(x, weight, cache, lens, d_y=None, d_cache=None):
+    """Sequences of lens rows each of [R,C] through the 4-tap causal convolution with SiLU, and its adjoint, with
+    bounds: a sum of n products is off by at most (n + 1) EPS of the sum of their sizes."""
+    R, C = x.shape
+    N = len(lens)
+    x, w = x.double(), weight.double()
+    train = d_y is not None
+    out = {"y": torch.zeros(R, C, dtype=torch.float64), "cache": torch.zeros(N, 3, C, dtype=torch.float64)}
+    if train:
+        out.update(dx=torch.zeros(R, C, dtype=torch.float64), d_weight=torch.zeros(C, 4, dtype=torch.float64))
+        if cache is not None:
+            out["d_cache"] = torch.zeros(N, 3, C, dtype=torch.float64)
+    tol = {k: torch.zeros_like(v) for k, v in out.items()}
+    dw_size = torch.zeros(C, 4, dtype=torch.float64)
+    at = 0
+    for n, length in enumerate(lens):
+        s = slice(at, at + length)
+        at += length
+        seq = x[s]
+        if cache is not None:
+            front = cache[n].double()
+        else:
+            front = seq[:1].expand(3, C) if length else torch.zeros(3, C, dtype=torch.float64)
+        line = torch.cat((front, seq))
+        out["cache"][n] = line[length:]
+        taps = torch.stack([line[j:j + length] for j in range(4)], -1)  # [T,C,4]
+        pre = (taps * w).sum(-1)
+        e_pre = 5 * EPS * (taps * w).abs().sum(-1)
+        act, slope, e_act, e_slope = silu_parts(pre)
+        out["y"][s], tol["y"][s] = act, e_act + 1.1 * e_pre
+        if not train:
+            continue
+        d = d_y.double()[s]
+        dp, e_dp = d * slope, d.abs() * (e_slope + 0.5 * e_pre) + EPS * (d * slope).abs()
+        d_line, e_line, size = (torch.zeros(length + 3, C, dtype=torch.float64) for _ in range(3))
+        for j in range(4):
+            d_line[j:j + length] += dp * w[:, j]
+            e_line[j:j + length] += e_dp * w[:, j].abs()
+            size[j:j + length] += (dp * w[:, j]).abs()
+        if d_cache is not None:
+            d_line[length:] += d_cache[n].double()
+            size[length:] += d_cache[n].double().abs()
+        out["dx"][s], tol["dx"][s] = d_line[3:], e_line[3:]
+        count = 6 * size
+        if cache is not None:
+            out["d_cache"][n], tol["d_cache"][n] = d_line[:3], e_line[:3] + EPS * count[:3]
+        elif length:  # copies of the first token: four values' sums come together
+            out["dx"][s][0] += d_line[:3].sum(0)
+            tol["dx"][s][0] += e_line[:3].sum(0) + 16 * EPS * size[:4].sum(0)
+        tol["dx"][s] += EPS * count[3:]
+        out["d_weight"] += (dp[..., None] * taps).sum(0)
+        tol["d_weight"] += (e_dp[..., None] * taps.abs()).sum(0)
+        dw_size += (dp[..., None] * taps).abs().sum(0)
+    if train:
+        tol["d_weight"] += (R + 8) * EPS * dw_size
+    return out, tol
+
+
 def check(got, want, bound, what):
     """got (any dtype) within the bound of f32 arithmetic plus one rounding to its dtype."""
     assert got.shape == want.shape, (what, got.shape, want.shape)

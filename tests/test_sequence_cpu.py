@@ -81,7 +81,8 @@ def test_struct_layouts_match_header(tmp_path):
 
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     names = {"gdn2_scan_args": _lib.ScanArgs, "gdn2_scan_bwd_args": _lib.ScanBwdArgs,
-             "gdn2_group_norm_args": _lib.GroupNormArgs, "gdn2_group_norm_bwd_args": _lib.GroupNormBwdArgs}
+             "gdn2_group_norm_args": _lib.GroupNormArgs, "gdn2_group_norm_bwd_args": _lib.GroupNormBwdArgs,
+             "gdn2_conv_args": _lib.ConvArgs, "gdn2_conv_bwd_args": _lib.ConvBwdArgs}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "gdn2.h"', "int main() {"]
     for c, s in names.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
@@ -140,3 +141,49 @@ def test_group_norm_null_pointers_and_workspace():
     assert call(b, fake, need - 1) == _lib.GDN2_EWORKSPACE
     assert call(b) == _lib.GDN2_EWORKSPACE
     assert LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(bwd(_norm_args(), fake, 32, fake, fake, None, None))) == 0
+
+
+def _conv_args(**over):
+    from burn_gdn2 import _lib
+
+    fake = 1 << 20
+    a = _lib.ConvArgs(2, 40, 8, 0, None, _lib.View(fake, 320, 8, 0), fake, None)
+    for k, val in over.items():
+        setattr(a, k, val)
+    return a
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(batch=0), 1), (dict(seq_len=0), 1), (dict(seq_len=-2), 1), (dict(channels=0), 1), (dict(dtype=3), 1),
+    (dict(weight=None), 1), (dict(seq_len=(1 << 30) + 1), 2),
+])
+def test_conv_argument_errors(over, status):
+    from burn_gdn2 import LIB, _lib
+
+    out = _lib.View(1 << 20, 320, 8, 0)
+    a = _conv_args(**over)
+    assert LIB.gdn2_causal_conv(ctypes.byref(a), out, None, None) == status
+    assert LIB.gdn2_last_error().decode().startswith("gdn2_causal_conv:")
+    b = _lib.ConvBwdArgs(a, out, None, out, 1 << 20, None)
+    assert LIB.gdn2_causal_conv_bwd(ctypes.byref(b), 1 << 20, 1 << 30, None) == status
+    assert LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(b)) == 0
+
+
+def test_conv_null_pointers_and_workspace():
+    from burn_gdn2 import LIB, _lib
+
+    fake = 1 << 20
+    out, none = _lib.View(fake, 320, 8, 0), _lib.View()
+    assert LIB.gdn2_causal_conv(None, out, None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_causal_conv(ctypes.byref(_conv_args()), none, None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_causal_conv(ctypes.byref(_conv_args(x=none)), out, None, None) == _lib.GDN2_EINVAL
+    call = lambda *rest, ws=None, n=0: LIB.gdn2_causal_conv_bwd(ctypes.byref(_lib.ConvBwdArgs(_conv_args(), *rest)), ws, n, None)
+    assert LIB.gdn2_causal_conv_bwd(None, None, 0, None) == _lib.GDN2_EINVAL
+    assert call(none, None, out, None, None) == _lib.GDN2_EINVAL
+    assert call(out, None, none, None, None) == _lib.GDN2_EINVAL
+    assert call(out, None, out, None, fake) == _lib.GDN2_EINVAL  # d_cache_in without a cache
+    b = _lib.ConvBwdArgs(_conv_args(), out, None, out, fake, None)
+    need = LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(b))
+    assert need > 0 and need % (8 * 4 * 4) == 0
+    assert call(out, None, out, fake, None, ws=fake, n=need - 1) == _lib.GDN2_EWORKSPACE
+    assert call(out, None, out, fake, None) == _lib.GDN2_EWORKSPACE
