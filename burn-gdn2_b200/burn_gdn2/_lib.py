@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_HERE, "libgdn2_b200.so")
 GDN2_OK, GDN2_EINVAL, GDN2_EUNSUPPORTED, GDN2_ECUDA, GDN2_EWORKSPACE = range(5)
 GDN2_DTYPE_F32, GDN2_DTYPE_BF16 = 0, 1
 GDN2_PRECISION_F32, GDN2_PRECISION_BF16 = 0, 1
+GDN2_MAX_STATE_ROWS = 4096
 
 _STATUS = {1: "EINVAL", 2: "EUNSUPPORTED", 3: "ECUDA", 4: "EWORKSPACE"}
 
@@ -119,6 +120,10 @@ class GroupNormBwdArgs(ctypes.Structure):
                 ("d_bias", ctypes.c_void_p)]
 
 
+class StateRows(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("row_bytes", ctypes.c_int64)]
+
+
 class Config(ctypes.Structure):
     _fields_ = [("hidden_size", ctypes.c_int64), ("num_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
                 ("expand_v", ctypes.c_float), ("num_v_heads", ctypes.c_int64), ("use_short_conv", ctypes.c_int32),
@@ -136,6 +141,7 @@ EXPORTS = (
     "gdn2_chunk_trajectory", "gdn2_gated_scan", "gdn2_gated_scan_bwd",
     "gdn2_group_norm_gate", "gdn2_group_norm_gate_bwd_workspace_bytes", "gdn2_group_norm_gate_bwd",
     "gdn2_causal_conv", "gdn2_causal_conv_bwd_workspace_bytes", "gdn2_causal_conv_bwd",
+    "gdn2_move_state_rows",
 )
 
 
@@ -172,6 +178,8 @@ def _load():
     lib.gdn2_causal_conv_bwd_workspace_bytes.restype = sz
     lib.gdn2_causal_conv_bwd.argtypes = [P(ConvBwdArgs), vp, sz, vp]
     lib.gdn2_causal_conv_bwd.restype = ctypes.c_int
+    lib.gdn2_move_state_rows.argtypes = [P(StateRows), i32, vp, i32, i32, vp]
+    lib.gdn2_move_state_rows.restype = ctypes.c_int
     lib.gdn2_group_norm_gate.argtypes = [P(GroupNormArgs), vp, vp]
     lib.gdn2_group_norm_gate.restype = ctypes.c_int
     lib.gdn2_group_norm_gate_bwd_workspace_bytes.argtypes = [P(GroupNormBwdArgs)]
@@ -203,7 +211,8 @@ LIB = _load()
 
 
 def read_device_errors() -> int:
-    """Device error bits since the last call (bit 0: a bounded wait gave up)."""
+    """Device error bits since the last call (bit 0: a bounded wait gave up;
+    bit 1: a row number outside a state pool)."""
     v = ctypes.c_uint32(0)
     check(LIB.gdn2_read_device_errors(ctypes.byref(v)))
     return int(v.value)

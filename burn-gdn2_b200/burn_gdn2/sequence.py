@@ -3,6 +3,8 @@
   gated_scan        the diagonal gated linear recurrence h_t = e^{g_t} h_{t-1} + s_t x_t
   causal_conv_silu  the 4-tap causal convolution with SiLU in front of it
   group_norm_gate   the norm of each token's channel groups behind it, with an affine map and a SiLU
+  reorder_states    forking, compacting and freeing the rows of the state pool of a serving batch, in place
+  select_states     the same into a new pool of another size
 
 Every operator takes CUDA tensors on any device and launches on that device's
 current stream; it is differentiable where an input requires a gradient, and
@@ -17,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import dataclasses
 from typing import Optional, Tuple
 
 import torch
@@ -340,3 +343,116 @@ def group_norm_gate(x, gate=None, weight=None, bias=None, *, num_groups: int, ep
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias)):
         return _GroupNormGate.apply(*args).reshape(shape)
     return _norm_forward(*args).reshape(shape)
+
+
+# -- state pools ---------------------------------------------------------------
+
+
+def _pool_tensors(what: str, states) -> list:
+    """The tensors of a tensor, a state (its fields), or a sequence of either."""
+    if isinstance(states, torch.Tensor):
+        return [states]
+    if dataclasses.is_dataclass(states):
+        return [getattr(states, f.name) for f in dataclasses.fields(states)]
+    if isinstance(states, (list, tuple)):
+        return [t for s in states for t in _pool_tensors(what, s)]
+    raise TypeError(f"{what}: a pool is tensors, states or sequences of them, got {type(states).__name__}")
+
+
+def _pool_like(states, new):
+    """The structure of states, filled from the iterator new."""
+    if isinstance(states, torch.Tensor):
+        return next(new)
+    if dataclasses.is_dataclass(states):
+        return dataclasses.replace(states, **{f.name: next(new) for f in dataclasses.fields(states)})
+    return type(states)([_pool_like(s, new) for s in states])
+
+
+def _checked_pool(what: str, states):
+    tensors = _pool_tensors(what, states)
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} runs on the B200 CUDA kernels only; got a CPU tensor")
+        if t.dim() < 1 or t.shape[0] != tensors[0].shape[0]:
+            raise ValueError(f"{what}: every tensor of a pool has its rows first and as many, got {[list(t.shape) for t in tensors]}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what}: the tensors of a pool must be contiguous")
+        if t.requires_grad:
+            raise ValueError(f"{what}: the rows of a pool move without gradients; detach its tensors")
+        _same_device(what, tensors[0].device, t)
+    if tensors and tensors[0].shape[0] > _lib.GDN2_MAX_STATE_ROWS:
+        raise ValueError(f"{what}: {tensors[0].shape[0]} rows, at most {_lib.GDN2_MAX_STATE_ROWS}")
+    return tensors
+
+
+def _pool_index(what: str, index, rows: int, device) -> torch.Tensor:
+    """Row numbers on the device, int32; checked where they come from the host."""
+    if not isinstance(index, torch.Tensor):
+        index = torch.tensor(index, dtype=torch.int64)
+    if index.dim() != 1 or index.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: index must be a vector of int32 or int64, got {index.dtype} {list(index.shape)}")
+    if index.shape[0] > _lib.GDN2_MAX_STATE_ROWS:
+        raise ValueError(f"{what}: {index.shape[0]} rows, at most {_lib.GDN2_MAX_STATE_ROWS}")
+    if not index.is_cuda:
+        if index.numel() and (int(index.min()) < -1 or int(index.max()) >= rows):
+            raise ValueError(f"{what}: row numbers must be -1 to {rows - 1}, got {index.tolist()}")
+        return index.to(device=device, dtype=torch.int32)
+    _same_device(what, device, index)
+    if index.dtype == torch.int64:  # as far as 32 bits tell a number inside the pool from one outside
+        index = index.clamp(-2, rows).int()
+    return index.contiguous()
+
+
+def _move_rows(pairs, index, src_rows):
+    pairs = [(s, d) for s, d in pairs if s.numel() or d.numel()]
+    if not pairs or not index.numel():
+        return
+    device = index.device
+    rows = (_lib.StateRows * len(pairs))(*((s.data_ptr(), d.data_ptr(), d.numel() // d.shape[0] * d.element_size())
+                                           for s, d in pairs))
+    with _on(device):
+        check(LIB.gdn2_move_state_rows(rows, len(pairs), index.data_ptr(), src_rows, index.shape[0], _stream(device)))
+
+
+def reorder_states(states, index) -> None:
+    """Move the rows of a state pool, in place and in one launch: in every
+    tensor row d becomes what row index[d] was, -1 a row of zeros (a freed or
+    a fresh sequence); a row's own number leaves it alone.  All rows at once:
+    a fork names one source several times, a compaction moves the last live
+    rows into the holes, swaps need no third row.
+
+    states: a Gdn2State, a tensor (a scan's state, a convolution's cache), or a
+    sequence of them (the layers of a model); rows come first, contiguous, at
+    most 4096.  index: one number a row, on the host (checked) or on the device
+    (int32 or int64; read by the kernel, so a captured call follows it).  On
+    the device a number outside the pool leaves its row as it was and sets bit
+    1 of ``read_device_errors()``.
+    """
+    what = "reorder_states"
+    tensors = _checked_pool(what, states)
+    if not tensors:
+        return
+    rows = tensors[0].shape[0]
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{what}: a tensor (or a part of one) comes twice")
+    index = _pool_index(what, index, rows, tensors[0].device)
+    if index.shape[0] != rows:
+        raise ValueError(f"{what}: {index.shape[0]} row numbers for {rows} rows")
+    _move_rows([(t, t) for t in tensors], index, rows)
+
+
+def select_states(states, index):
+    """A new pool of len(index) rows, row d a copy of row index[d] of states
+    (-1: zeros): a batch that grows, or is split for another device step.  The
+    result has the structure of ``states``; numbers as in reorder_states, but a
+    row whose number on the device is outside the pool is zeros."""
+    what = "select_states"
+    tensors = _checked_pool(what, states)
+    if not tensors:
+        return _pool_like(states, iter(()))
+    rows = tensors[0].shape[0]
+    index = _pool_index(what, index, rows, tensors[0].device)
+    new = [torch.empty((index.shape[0], *t.shape[1:]), dtype=t.dtype, device=t.device) for t in tensors]
+    _move_rows([(t, n) for t, n in zip(tensors, new)], index, rows)
+    return _pool_like(states, iter(new))

@@ -43,6 +43,7 @@ unsigned read_device_errors_intra_tc();
 unsigned read_device_errors_inter_tc();
 unsigned read_device_errors_intra_x3();
 unsigned read_device_errors_inter_x3();
+unsigned read_device_errors_state_rows();
 int selftest_umma(int test, const float* A, const float* B, float* D, cudaStream_t st);
 int selftest_wait(unsigned spins, int arrive, int* completed);
 int launch_short_conv(int B, int Tn, int C, int dtype, const void* x, const float* w, const float* cin, float* cout,
@@ -52,6 +53,8 @@ int launch_rms_norm_gate(const gdn2_dims& d, int dtype, const gdn2_view& o, cons
 int launch_project_activations(const gdn2_prologue_args* a, cudaStream_t st);
 int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, cudaStream_t st);
 int launch_scan_bwd(const gdn2_scan_bwd_args* a, cudaStream_t st);
+int launch_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* index, int32_t src_rows,
+                      int32_t dst_rows, cudaStream_t st);
 int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_out, cudaStream_t st);
 size_t conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* a);
 int launch_conv_bwd(const gdn2_conv_bwd_args* a, void* ws, size_t ws_bytes, cudaStream_t st);
@@ -259,7 +262,7 @@ int gdn2_read_device_errors(uint32_t* flags) {
   int rc = check_cuda(cudaDeviceSynchronize(), "gdn2_read_device_errors");
   if (rc) return rc;
   *flags = read_device_errors_recurrent() | read_device_errors_selftest() | read_device_errors_intra_tc() |
-           read_device_errors_inter_tc() | read_device_errors_intra_x3() | read_device_errors_inter_x3();
+           read_device_errors_inter_tc() | read_device_errors_intra_x3() | read_device_errors_inter_x3() | read_device_errors_state_rows();
   return GDN2_OK;
 }
 
@@ -418,6 +421,11 @@ int gdn2_gated_scan(const gdn2_scan_args* a, gdn2_view h, float* state_out, void
 
 int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* a, void* stream) {
   return launch_scan_bwd(a, (cudaStream_t)stream);
+}
+
+int gdn2_move_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* index, int32_t src_rows,
+                         int32_t dst_rows, void* stream) {
+  return launch_state_rows(t, count, index, src_rows, dst_rows, (cudaStream_t)stream);
 }
 
 int gdn2_causal_conv(const gdn2_conv_args* a, gdn2_view y, float* cache_out, void* stream) {

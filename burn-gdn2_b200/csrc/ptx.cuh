@@ -10,6 +10,7 @@ namespace gdn2 {
 // Device error bits, read and cleared by gdn2_read_device_errors().
 enum : unsigned {
   DEVERR_MBAR_TIMEOUT = 1u,  // a bounded mbarrier wait gave up
+  DEVERR_STATE_INDEX = 2u,   // a row number outside a state pool
 };
 // One copy per translation unit (no relocatable device code); each unit
 // that launches kernels exposes a host reader (see gdn2_read_device_errors).

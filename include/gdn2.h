@@ -466,6 +466,31 @@ GDN2_API size_t gdn2_group_norm_gate_bwd_workspace_bytes(const gdn2_group_norm_b
 GDN2_API int gdn2_group_norm_gate_bwd(const gdn2_group_norm_bwd_args* args, void* workspace, size_t workspace_bytes,
                                       void* stream);
 
+/* ------------------------------------------------------------------------
+ * Rows of a state pool moved on the device: the recurrent states, caches and
+ * scan states of a batch of running sequences, forked, compacted and freed
+ * (no counterpart in the reference, which keeps one state per call).  In
+ * every tensor row d becomes what row index[d] was, all rows at once: swaps,
+ * several copies of one row and chains of moves are all right in one call.
+ * index[d] = -1 sets the row to zero; in place, index[d] = d leaves it alone.
+ * src = dst in every tensor (in place, src_rows = dst_rows), or in none
+ * (rows gathered into another pool; the two must not overlap).  index:
+ * device, int32 [dst_rows]; a number outside -1 .. src_rows - 1 sets bit 1 of
+ * the device error bits (gdn2_read_device_errors) and leaves its row as it
+ * was in place, zero in another pool.  At most GDN2_MAX_STATE_ROWS rows a call; up to
+ * 16 tensors are one launch.  No tensor may appear twice.
+ * ---------------------------------------------------------------------- */
+#define GDN2_MAX_STATE_ROWS 4096
+
+typedef struct gdn2_state_rows {
+  const void* src;   /* [src_rows] rows of row_bytes each, contiguous */
+  void* dst;         /* [dst_rows] */
+  int64_t row_bytes; /* any; multiples of 16 move fastest */
+} gdn2_state_rows;
+
+GDN2_API int gdn2_move_state_rows(const gdn2_state_rows* tensors, int32_t count, const int32_t* index,
+                                  int32_t src_rows, int32_t dst_rows, void* stream);
+
 /* Mirror of Gdn2Config (src/config.rs:24-58) and its validate()
  * (src/config.rs:71-111).  num_v_heads < 0 means None; min_decay < 0
  * means None; mode 0 = FusedRecurrent, 1 = Chunk. */
@@ -490,7 +515,8 @@ GDN2_API int gdn2_config_validate(const gdn2_config* cfg, char* msg, size_t msg_
 /* Device-side error bits accumulated since the last call (and cleared):
  * bit 0 = a bounded wait inside a kernel gave up (a bulk copy that never
  * completed); the kernel finished without hanging but its results are
- * invalid.  Synchronises the current device. */
+ * invalid; bit 1 = gdn2_move_state_rows met a row number outside its pool.
+ * Synchronises the current device. */
 GDN2_API int gdn2_read_device_errors(uint32_t* flags);
 
 /* Diagnostic (no counterpart in the reference): one tcgen05 MMA tile,

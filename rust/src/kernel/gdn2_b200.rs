@@ -256,6 +256,17 @@ pub struct Gdn2GroupNormBwdArgs {
     pub d_bias: *mut f32,
 }
 
+pub const GDN2_MAX_STATE_ROWS: i32 = 4096;
+
+/// One tensor of a state pool for `gdn2_move_state_rows`.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Gdn2StateRows {
+    pub src: *const c_void,
+    pub dst: *mut c_void,
+    pub row_bytes: i64,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct Gdn2Config {
@@ -303,6 +314,8 @@ extern "C" {
     pub fn gdn2_group_norm_gate_bwd_workspace_bytes(args: *const Gdn2GroupNormBwdArgs) -> usize;
     pub fn gdn2_group_norm_gate_bwd(args: *const Gdn2GroupNormBwdArgs, workspace: *mut c_void, workspace_bytes: usize,
                                     stream: *mut c_void) -> i32;
+    pub fn gdn2_move_state_rows(tensors: *const Gdn2StateRows, count: i32, index: *const i32, src_rows: i32,
+                                dst_rows: i32, stream: *mut c_void) -> i32;
     pub fn gdn2_config_validate(cfg: *const Gdn2Config, msg: *mut c_char, msg_len: usize) -> i32;
     pub fn gdn2_read_device_errors(flags: *mut u32) -> i32;
     pub fn gdn2_selftest_umma(test: i32, a: *const f32, b: *const f32, d: *mut f32, stream: *mut c_void) -> i32;

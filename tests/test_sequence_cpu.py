@@ -82,7 +82,7 @@ def test_struct_layouts_match_header(tmp_path):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     names = {"gdn2_scan_args": _lib.ScanArgs, "gdn2_scan_bwd_args": _lib.ScanBwdArgs,
              "gdn2_group_norm_args": _lib.GroupNormArgs, "gdn2_group_norm_bwd_args": _lib.GroupNormBwdArgs,
-             "gdn2_conv_args": _lib.ConvArgs, "gdn2_conv_bwd_args": _lib.ConvBwdArgs}
+             "gdn2_conv_args": _lib.ConvArgs, "gdn2_conv_bwd_args": _lib.ConvBwdArgs, "gdn2_state_rows": _lib.StateRows}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "gdn2.h"', "int main() {"]
     for c, s in names.items():
         lines.append(f'printf("{c} size %zu\\n", sizeof({c}));')
@@ -187,3 +187,46 @@ def test_conv_null_pointers_and_workspace():
     assert need > 0 and need % (8 * 4 * 4) == 0
     assert call(out, None, out, fake, None, ws=fake, n=need - 1) == _lib.GDN2_EWORKSPACE
     assert call(out, None, out, fake, None) == _lib.GDN2_EWORKSPACE
+
+
+def test_state_rows_argument_errors():
+    from burn_gdn2 import LIB, _lib
+
+    fake = 1 << 20
+    idx = ctypes.c_void_p(fake)
+
+    def call(pairs, index=idx, src=4, dst=4, count=None):
+        t = (_lib.StateRows * max(1, len(pairs)))(*pairs)
+        return LIB.gdn2_move_state_rows(t, len(pairs) if count is None else count, index, src, dst, None)
+
+    good = (fake, fake, 64)
+    assert call([good], count=-1) == _lib.GDN2_EINVAL
+    assert call([good], src=-1) == _lib.GDN2_EINVAL and call([good], dst=-1) == _lib.GDN2_EINVAL
+    assert call([], count=0) == _lib.GDN2_OK and call([good], dst=0, src=0) == _lib.GDN2_OK  # nothing to do
+    assert call([good], index=None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_move_state_rows(None, 1, idx, 4, 4, None) == _lib.GDN2_EINVAL
+    for bad in ((None, fake, 64), (fake, None, 64), (fake, fake, 0), (fake, fake, -16)):
+        assert call([bad]) == _lib.GDN2_EINVAL
+    assert call([good], src=4097, dst=4097) == _lib.GDN2_EUNSUPPORTED
+    assert call([good], src=5, dst=4) == _lib.GDN2_EINVAL  # in place, rows differ
+    assert call([good, (fake, fake + (1 << 16), 64)]) == _lib.GDN2_EINVAL  # in place and not
+    assert call([(fake, fake + 3 * 64, 64)]) == _lib.GDN2_EINVAL  # overlap
+    assert call([(fake + 3 * 64, fake, 64)]) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_last_error().decode().startswith("gdn2_move_state_rows:")
+
+
+def test_pool_structures():
+    import burn_gdn2 as bg
+    from burn_gdn2 import sequence
+
+    t = [torch.zeros(2, k + 1) for k in range(6)]
+    state = bg.Gdn2State(*t[:4])
+    nested = [state, (t[4], [t[5]])]
+    flat = sequence._pool_tensors("op", nested)
+    assert [a is b for a, b in zip(flat, t)] == [True] * 6 and len(flat) == 6
+    again = sequence._pool_like(nested, iter(flat))
+    assert isinstance(again[0], bg.Gdn2State) and again[0].conv_v is t[3] and again[1][1][0] is t[5]
+    with pytest.raises(TypeError):
+        sequence._pool_tensors("op", {"a": 1})
+    with pytest.raises(RuntimeError, match="CPU tensor"):
+        bg.reorder_states(state, [0, 1])
