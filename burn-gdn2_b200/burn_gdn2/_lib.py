@@ -138,7 +138,7 @@ EXPORTS = (
     "gdn2_last_error", "gdn2_last_cuda_error", "gdn2_abi_version", "gdn2_read_device_errors",
     "gdn2_selftest_umma", "gdn2_chunk_fwd_noalloc", "gdn2_project_activations", "gdn2_selftest_wait",
     "gdn2_set_reserved_sms", "gdn2_recurrent_bwd_workspace_bytes", "gdn2_recurrent_bwd",
-    "gdn2_chunk_trajectory", "gdn2_gated_scan", "gdn2_gated_scan_bwd",
+    "gdn2_chunk_trajectory", "gdn2_gated_scan_workspace_bytes", "gdn2_gated_scan", "gdn2_gated_scan_bwd_workspace_bytes", "gdn2_gated_scan_bwd",
     "gdn2_group_norm_gate", "gdn2_group_norm_gate_bwd_workspace_bytes", "gdn2_group_norm_gate_bwd",
     "gdn2_causal_conv", "gdn2_causal_conv_bwd_workspace_bytes", "gdn2_causal_conv_bwd",
     "gdn2_move_state_rows",
@@ -168,9 +168,13 @@ def _load():
     lib.gdn2_recurrent_bwd.restype = ctypes.c_int
     lib.gdn2_chunk_trajectory.argtypes = [P(RecurrentArgs), i32, vp, View, vp]
     lib.gdn2_chunk_trajectory.restype = ctypes.c_int
-    lib.gdn2_gated_scan.argtypes = [P(ScanArgs), View, vp, vp]
+    lib.gdn2_gated_scan_workspace_bytes.argtypes = [P(ScanArgs), View]
+    lib.gdn2_gated_scan_workspace_bytes.restype = sz
+    lib.gdn2_gated_scan.argtypes = [P(ScanArgs), View, vp, vp, sz, vp]
     lib.gdn2_gated_scan.restype = ctypes.c_int
-    lib.gdn2_gated_scan_bwd.argtypes = [P(ScanBwdArgs), vp]
+    lib.gdn2_gated_scan_bwd_workspace_bytes.argtypes = [P(ScanBwdArgs)]
+    lib.gdn2_gated_scan_bwd_workspace_bytes.restype = sz
+    lib.gdn2_gated_scan_bwd.argtypes = [P(ScanBwdArgs), vp, sz, vp]
     lib.gdn2_gated_scan_bwd.restype = ctypes.c_int
     lib.gdn2_causal_conv.argtypes = [P(ConvArgs), View, vp, vp]
     lib.gdn2_causal_conv.restype = ctypes.c_int

@@ -95,6 +95,10 @@ def _f32(what: str, name: str, t: Optional[torch.Tensor], shape) -> Optional[tor
     return t.contiguous()
 
 
+def _workspace(size: int, device: torch.device):
+    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -111,9 +115,10 @@ def _scan_forward(x, g, state, cu, complement, state_out, keep):
     B, T, C = x.shape
     h = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
     carry = torch.empty((B, -(-T // SCAN_CARRY), C), dtype=torch.float32, device=x.device) if keep else None
-    a = _scan_args(x, g, state, cu, complement, carry)
+    a, out = _scan_args(x, g, state, cu, complement, carry), _view3(h)
     with _on(x.device):
-        check(LIB.gdn2_gated_scan(ctypes.byref(a), _view3(h), _ptr(state_out), _stream(x.device)))
+        ws, size = _workspace(LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(a), out), x.device)
+        check(LIB.gdn2_gated_scan(ctypes.byref(a), out, _ptr(state_out), _ptr(ws), size, _stream(x.device)))
     return h, carry
 
 
@@ -140,7 +145,8 @@ class _GatedScan(torch.autograd.Function):
         a = _lib.ScanBwdArgs(_scan_args(x, g, state, cu, ctx.complement, carry), _view3(d_h), _ptr(d_last),
                              _view3(dx), _view3(dg), _ptr(d_state))
         with _on(x.device):
-            check(LIB.gdn2_gated_scan_bwd(ctypes.byref(a), _stream(x.device)))
+            ws, size = _workspace(LIB.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(a)), x.device)
+            check(LIB.gdn2_gated_scan_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
         return dx, dg, d_state, None, None
 
 
@@ -226,8 +232,7 @@ class _CausalConv(torch.autograd.Function):
         a = _lib.ConvBwdArgs(_conv_args(x, weight, cache, cu), _view3(d_y), _ptr(d_new), _view3(dx), _ptr(d_weight),
                              _ptr(d_cache))
         with _on(x.device):
-            size = LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(a))
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            ws, size = _workspace(LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(a)), x.device)
             check(LIB.gdn2_causal_conv_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
         return dx, d_weight, d_cache, None
 
@@ -300,8 +305,7 @@ class _GroupNormGate(torch.autograd.Function):
         a = _lib.GroupNormBwdArgs(_norm_args(x, gate, weight, bias, *ctx.rest), d_y.data_ptr(), d_y.stride(0),
                                   _ptr(dx), _ptr(d_gate), _ptr(d_weight), _ptr(d_bias))
         with _on(x.device):
-            size = LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(a))
-            ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+            ws, size = _workspace(LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(a)), x.device)
             check(LIB.gdn2_group_norm_gate_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
         return dx, d_gate, d_weight, d_bias, None, None, None
 

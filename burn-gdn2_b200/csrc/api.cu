@@ -51,8 +51,11 @@ int launch_short_conv(int B, int Tn, int C, int dtype, const void* x, const floa
 int launch_rms_norm_gate(const gdn2_dims& d, int dtype, const gdn2_view& o, const gdn2_view& gate, const float* w,
                          float eps, const gdn2_view& out, cudaStream_t st);
 int launch_project_activations(const gdn2_prologue_args* a, cudaStream_t st);
-int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, cudaStream_t st);
-int launch_scan_bwd(const gdn2_scan_bwd_args* a, cudaStream_t st);
+int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, void* ws, size_t ws_bytes,
+                    cudaStream_t st);
+int launch_scan_bwd(const gdn2_scan_bwd_args* a, void* ws, size_t ws_bytes, cudaStream_t st);
+size_t scan_workspace_bytes(const gdn2_scan_args* a, const gdn2_view& h);
+size_t scan_bwd_workspace_bytes(const gdn2_scan_bwd_args* a);
 int launch_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* index, int32_t src_rows,
                       int32_t dst_rows, cudaStream_t st);
 int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_out, cudaStream_t st);
@@ -415,12 +418,16 @@ int gdn2_rms_norm_gate(const gdn2_dims* dims, int32_t dtype, gdn2_view o, gdn2_v
   return launch_rms_norm_gate(*dims, dtype, o, gate, weight, eps, out, (cudaStream_t)stream);
 }
 
-int gdn2_gated_scan(const gdn2_scan_args* a, gdn2_view h, float* state_out, void* stream) {
-  return launch_scan_fwd(a, h, state_out, (cudaStream_t)stream);
+size_t gdn2_gated_scan_workspace_bytes(const gdn2_scan_args* a, gdn2_view h) { return scan_workspace_bytes(a, h); }
+
+int gdn2_gated_scan(const gdn2_scan_args* a, gdn2_view h, float* state_out, void* ws, size_t ws_bytes, void* stream) {
+  return launch_scan_fwd(a, h, state_out, ws, ws_bytes, (cudaStream_t)stream);
 }
 
-int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* a, void* stream) {
-  return launch_scan_bwd(a, (cudaStream_t)stream);
+size_t gdn2_gated_scan_bwd_workspace_bytes(const gdn2_scan_bwd_args* a) { return scan_bwd_workspace_bytes(a); }
+
+int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* a, void* ws, size_t ws_bytes, void* stream) {
+  return launch_scan_bwd(a, ws, ws_bytes, (cudaStream_t)stream);
 }
 
 int gdn2_move_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* index, int32_t src_rows,

@@ -7,147 +7,171 @@
 //   l_t = dh_t + e^{g_{t+1}} l_{t+1},  dx_t = s_t l_t,
 //   dg_t = e^{g_t} (h_{t-1} [- x_t]) l_t,  dstate = e^{g_0} l_0.
 //
-// Both are bound by HBM: a forward reads x and g and writes h once, a
-// backward reads x, g and dh and writes dx and dg, some ten flops per byte.
-// So each value is read once into registers and every step of the scan
-// happens there: a warp holds RUN tokens of 32 * VEC neighbouring channels (all
-// its loads in flight at once), reduces them to the affine map
-// c -> A c + H of the run, and the maps of a tile's runs are joined through
-// shared memory and those of the cluster's tiles through distributed shared
-// memory.  A cluster walks its channels' whole time axis, CL tiles a step,
-// so one pass over the data suffices and the carry never leaves the chip.
-// The cluster is wider the fewer chains there are.  The joining order is
-// fixed: results do not depend on timing.
+// Both are bound by HBM with the issue rate close behind (some twenty
+// instructions for 8 to 14 bytes a value): a forward reads x and g and writes
+// h, a backward reads x, g and dh and writes dx and dg.  So each value is
+// read once and its decay computed once, between the load and the store, in
+// packed pairs of channels: a warp holds RUN tokens of 32 * VEC channels in
+// registers, reduces them to the affine map c -> A c + H of the run, the maps of
+// a block's runs are joined through shared memory, and the block walks its
+// channels' time axis, the loads of the next step in flight meanwhile.
+//
+// With few chains (sequences times sets of channels) the time axis is cut
+// into segments as well: a first launch reduces every segment to its map, the
+// second starts each segment from the maps before it.  That reads the inputs
+// twice, and pays below about 100 chains, where one block each would leave
+// the memory system idle.  The joining order is fixed by the sizes: results
+// do not depend on timing.
 #include "scan.cuh"
 
 namespace gdn2 {
 
 constexpr int RUN = 16;  // tokens of a warp's run; also the spacing of the states a backward starts from
-constexpr int MAX_CL = 8;
+constexpr int STAGES = 2;
+constexpr int MAX_SEGMENTS = 128;
 
 struct ScanParams {
-  int B, T, C;     // dense: B sequences of T; packed: N sequences in T rows
-  int tiles, steps;
-  int sets;        // sets of 32 * VEC channels
+  int B, T, C;      // dense: B sequences of T; packed: N sequences in T rows
+  int sets;         // sets of 32 * VEC channels
+  int steps;        // tiles of a segment
+  int segments;
   const int* cu;
-  DView x, g, h;   // forward: h out.  backward: h = dh
+  DView x, g, h;    // forward: h out.  backward: h = dh
   DView dx, dg;
   const float* state_in;
   float* state_out;
   const float* d_state_out;
   float* d_state_in;
-  float* carry;    // [B or 1][ceil(T / RUN)][C]: state before every RUN-th token
+  float* carry;     // [B or 1][ceil(T / RUN)][C]: state before every RUN-th token
+  float2* maps;     // [chain][segment][CH] maps of the segments, or null (one segment)
+  int* map_cuts;    // [chain][segment]: a sequence begins (adjoint: ends) in the segment
 };
 
-// A product of decays that a sequence start cuts is the negative zero: no
-// decay is negative, so the sign marks "take nothing from before", also
-// where what is before holds an infinity or NaN of another sequence.
-__device__ __forceinline__ bool is_cut(float A) { return __float_as_uint(A) == 0x80000000u; }
-
-template <bool PACKED>
-__device__ __forceinline__ float carry_on(float A, float H, float c) {
-  return PACKED && is_cut(A) ? H : fmaf(A, c, H);
-}
-// The product of the decays A, then a; a cut stays one, whatever follows.
-template <bool PACKED>
-__device__ __forceinline__ float chain(float A, float a) {
-  if (PACKED && is_cut(A)) return A;
-  return PACKED && is_cut(a) ? a : A * a;
-}
-
-// The maps of a step, [run][channel] of this tile and [tile][channel] of the cluster, twice for alternating steps.
-template <int NW, int CH>
-struct ScanShared {
-  float2 run[2][NW][CH];
-  float2 tile[2][MAX_CL][CH];
-};
-
-// Joins the runs' maps: from the state `c` before the step's first token (or
-// after its last, in the reverse direction), the state before this warp's
-// run; c becomes the state after the step.  Run and tile order is the
-// direction of the scan.
-template <int NW, int VEC, bool PACKED>
-__device__ __forceinline__ void join(ScanShared<NW, 32 * VEC>& sh, int buf, int CL, int rank, int warp, int lane,
-                                     const float (&A)[VEC], const float (&H)[VEC], float (&c)[VEC],
-                                     float (&cin)[VEC]) {
-  constexpr int CH = 32 * VEC;
-  const int ch = lane * VEC;
-  #pragma unroll
-  for (int v = 0; v < VEC; ++v) sh.run[buf][warp][ch + v] = make_float2(A[v], H[v]);
-  __syncthreads();
-  if (CL == 1) {
-    #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+// One warp's staged rows, [RUN][32 * VEC] of T.  Copied 16 bytes a lane over
+// several rows where rows allow it (COOP: few instructions; lanes read what
+// others copied), else each lane its own values.
+template <typename T, int VEC, bool COOP>
+struct Rows {
+  static constexpr int ROW = 32 * VEC * (int)sizeof(T), BYTES = RUN * ROW;
+  unsigned char* base;
+  // rows t0 .. of p (its lane 0 channel), those below T, channels below `left`
+  __device__ __forceinline__ void fetch(const T* p, int64_t stride, int t0, int T_, int left, int lane) const {
+    if constexpr (COOP) {
+      constexpr int LANES = ROW / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
+      const int c = lane % LANES * (16 / (int)sizeof(T)), r = lane / LANES;
+      const T* q = p + (int64_t)(t0 + r) * stride + c;
       #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (w == warp) cin[v] = c[v];
-        const float2 m = sh.run[buf][w][ch + v];
-        c[v] = carry_on<PACKED>(m.x, m.y, c[v]);
+      for (int i = 0; i < RUN; i += AT_ONCE) {
+        const bool in = c < left && t0 + r + i < T_;
+        cp_async_zfill<16>(base + (i + r) * ROW + lane % LANES * 16, in ? q : p, in);
+        q += AT_ONCE * stride;
+      }
+    } else {
+      typedef typename Vec<T, VEC>::Raw Raw;
+      const T* q = p + (int64_t)t0 * stride + lane * VEC;
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        const bool in = lane * VEC < left && t0 + i < T_;
+        Raw* to = reinterpret_cast<Raw*>(base + i * ROW) + lane;
+        if constexpr (sizeof(Raw) >= 4) cp_async_zfill<(int)sizeof(Raw)>(to, in ? q : p, in);
+        else *to = in ? Vec<T, VEC>::load(q) : Raw{};
+        q += stride;
       }
     }
-    return;
   }
-  for (int e = threadIdx.x; e < CH; e += 32 * NW) {
-    float2 t = sh.run[buf][0][e];
-    #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      const float2 m = sh.run[buf][w][e];
-      t.y = carry_on<PACKED>(m.x, m.y, t.y);
-      t.x = chain<PACKED>(t.x, m.x);
-    }
-    for (int r = 0; r < CL; ++r) {
-      const uint32_t at = cluster_addr(&sh.tile[buf][rank][e], r);
-      st_cluster_f32(at, t.x);
-      st_cluster_f32(at + 4, t.y);
-    }
+  // a lane's channels of row i as a pair (the second zero for VEC = 1)
+  __device__ __forceinline__ f32x2 get(int i, int lane) const {
+    float f[2] = {0.f, 0.f};
+    const T* p = reinterpret_cast<const T*>(base + i * ROW) + lane * VEC;
+    if constexpr (VEC == 2) Vec<T, 2>::unpack(*reinterpret_cast<const typename Vec<T, 2>::Raw*>(p), f);
+    else f[0] = to_f32<T>(*p);
+    return f2pk(f[0], f[1]);
   }
-  cluster_sync_all();
-  #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    float s = c[v];
-    for (int r = 0; r < CL; ++r) {
-      if (r == rank) cin[v] = s;
-      const float2 m = sh.tile[buf][r][ch + v];
-      s = carry_on<PACKED>(m.x, m.y, s);
-    }
-    c[v] = s;
-    for (int w = 0; w < warp; ++w) {
-      const float2 m = sh.run[buf][w][ch + v];
-      cin[v] = carry_on<PACKED>(m.x, m.y, cin[v]);
-    }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* p, f32x2 v) {
+  float f[2];
+  f2un(v, f[0], f[1]);
+  if constexpr (VEC == 2) Vec<T, 2>::store(p, f);
+  else {
+    float one[1] = {f[0]};
+    Vec<T, 1>::store(p, one);
   }
 }
+template <int VEC>
+__device__ __forceinline__ f32x2 get_f32(const float* p) {
+  return f2pk(p[0], VEC == 2 ? p[VEC - 1] : 0.f);
+}
+template <int VEC>
+__device__ __forceinline__ void put_f32(float* p, f32x2 v) {
+  float f0, f1;
+  f2un(v, f0, f1);
+  p[0] = f0;
+  if (VEC == 2) p[VEC - 1] = f1;
+}
 
-// Decays of a run: raw g to a = e^g and m = e^g - 1.
-template <typename TG, int VEC>
-__device__ __forceinline__ void decays(const typename Vec<TG, VEC>::Raw (&gr)[RUN], float (&a)[RUN][VEC],
-                                       float (&m)[RUN][VEC]) {
-  float g[RUN][VEC];
+// The maps of a step's runs, twice for alternating steps.  cut: a sequence
+// begins (adjoint: ends) in the run, so that nothing from before it comes
+// through, not even an infinity or NaN times zero.
+template <int NW>
+struct ScanMaps {
+  ulonglong2 run[2][NW][32];  // (A, H) pairs
+  int cut[2][NW];
+};
+
+// From the state `c` before the step's first token (after its last, in the
+// adjoint), the state before this warp's run; c becomes the state after the
+// step, and the maps join to `A` of the whole (with SUM).
+template <int NW, bool PACKED, bool SUM>
+__device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int lane, f32x2 A, f32x2 H, bool cut,
+                                      f32x2& c, f32x2& all, bool& any_cut) {
+  sh.run[buf][warp][lane] = make_ulonglong2(A, H);
+  if (PACKED && lane == 0) sh.cut[buf][warp] = cut;
+  __syncthreads();
+  f32x2 cin = c;
+  #pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w == warp) cin = c;
+    const ulonglong2 m = sh.run[buf][w][lane];
+    const bool cuts = PACKED && sh.cut[buf][w];
+    c = cuts ? m.y : f2fma(m.x, c, m.y);
+    if (SUM) {
+      all = f2mul(all, m.x);
+      any_cut |= cuts;
+    }
+  }
+  return cin;
+}
+
+// Decays of a run: a = e^g, and k = 1 - e^g where it is wanted.
+template <typename G, bool COMP>
+__device__ __forceinline__ void decays(const G& rows, int lane, f32x2 (&a)[RUN], f32x2 (&k)[RUN]) {
   float far = 0.f;
   #pragma unroll
   for (int i = 0; i < RUN; ++i) {
-    Vec<TG, VEC>::unpack(gr[i], g[i]);
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) far = fmaxf(far, fabsf(g[i][v]));
-  }
-  if constexpr (VEC == 1) {
-    #pragma unroll
-    for (int i = 0; i < RUN; i += 2) exp_pair(g[i][0], g[i + 1][0], a[i][0], a[i + 1][0], m[i][0], m[i + 1][0]);
-  } else {
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i)
-      #pragma unroll
-      for (int v = 0; v < VEC; v += 2) exp_pair(g[i][v], g[i][v + 1], a[i][v], a[i][v + 1], m[i][v], m[i][v + 1]);
+    const f32x2 g = rows.get(i, lane);
+    float g0, g1;
+    f2un(g, g0, g1);
+    far = fmaxf(far, fmaxf(fabsf(g0), fabsf(g1)));
+    exp_pair<COMP>(g, a[i], k[i]);
   }
   if (far > kExpRange) {  // a reset (-inf), a decay below every f32, or growth
     #pragma unroll
-    for (int i = 0; i < RUN; ++i)
+    for (int i = 0; i < RUN; ++i) {
+      float g[2], e[2], m[2];
+      f2un(rows.get(i, lane), g[0], g[1]);
+      f2un(a[i], e[0], e[1]);
+      if (COMP) f2un(k[i], m[0], m[1]);
       #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (fabsf(g[i][v]) > kExpRange) {
-          a[i][v] = expf(g[i][v]);
-          m[i][v] = expm1f(g[i][v]);
+      for (int v = 0; v < 2; ++v)
+        if (fabsf(g[v]) > kExpRange) {
+          e[v] = expf(g[v]);
+          m[v] = -expm1f(g[v]);
         }
+      a[i] = f2pk(e[0], e[1]);
+      if (COMP) k[i] = f2pk(m[0], m[1]);
+    }
   }
 }
 
@@ -162,6 +186,7 @@ __device__ __forceinline__ bool is_empty(const int* __restrict__ cu, int n, int 
 struct RunMasks {
   unsigned start, last, valid;
   int seq;
+  __device__ __forceinline__ int sequence(int i) const { return __shfl_sync(0xffffffffu, seq, i); }
 };
 __device__ __forceinline__ RunMasks run_masks(const int* __restrict__ cu, int N, int T, int t0, int lane) {
   RunMasks k;
@@ -181,264 +206,267 @@ __device__ __forceinline__ RunMasks run_masks(const int* __restrict__ cu, int N,
   return k;
 }
 
-template <typename TX, typename TG, int VEC, int NW, bool COMP, bool PACKED>
-__global__ void __launch_bounds__(32 * NW) k_scan_fwd(ScanParams p, int CL) {
-  constexpr int CH = 32 * VEC;
-  __shared__ ScanShared<NW, CH> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = CL == 1 ? 0 : (int)(blockIdx.x % CL);
-  const int64_t chain = blockIdx.x / CL;
-  const int b = (int)(chain / p.sets);
-  const int c0 = (int)(chain % p.sets) * CH + lane * VEC;
-  const bool on = c0 < p.C;
-  const TX* x = static_cast<const TX*>(p.x.p) + (PACKED ? 0 : (int64_t)b * p.x.s0) + c0;
-  const TG* g = static_cast<const TG*>(p.g.p) + (PACKED ? 0 : (int64_t)b * p.g.s0) + c0;
-  TX* h = static_cast<TX*>(const_cast<void*>(p.h.p)) + (PACKED ? 0 : (int64_t)b * p.h.s0) + c0;
-
-  if (PACKED && p.state_out && rank == 0) {  // empty sequences keep their state
-    for (int n0 = warp * 32; n0 < p.B; n0 += 32 * NW) {
-      const int n = n0 + lane;
-      unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
-      while (empty) {
-        const int j = n0 + __ffs(empty) - 1;
-        empty &= empty - 1;
-        if (on) {
-          float s[VEC] = {};
-          if (p.state_in) load_f32<VEC>(p.state_in + (int64_t)j * p.C + c0, s);
-          store_f32<VEC>(p.state_out + (int64_t)j * p.C + c0, s);
-        }
-      }
+// Empty sequences hand their state (its gradient) through.
+template <int VEC>
+__device__ __forceinline__ void pass_empty(const ScanParams& p, const float* from, float* to, int c0, bool on) {
+  const int lane = threadIdx.x & 31;
+  for (int n0 = (int)threadIdx.x - lane; n0 < p.B; n0 += blockDim.x) {
+    const int n = n0 + lane;
+    unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
+    while (empty) {
+      const int64_t at = (int64_t)(n0 + __ffs(empty) - 1) * p.C + c0;
+      empty &= empty - 1;
+      if (on) put_f32<VEC>(to + at, from ? get_f32<VEC>(from + at) : f2pk(0.f, 0.f));
     }
   }
+}
 
-  if (CL > 1) cluster_sync_all();  // every CTA of the cluster runs before its memory is written
+// The state before segment `seg` (adjoint: after it): `c` through the maps of
+// the segments before (after) it.
+template <bool PACKED>
+__device__ __forceinline__ f32x2 through_segments(const ScanParams& p, int64_t chain, int seg, int lane, f32x2 c) {
+  const ulonglong2* m = reinterpret_cast<const ulonglong2*>(p.maps) + chain * p.segments * 32 + lane;
+  const int* cut = p.map_cuts + chain * p.segments;
+  #pragma unroll 8
+  for (int s = 0; s < seg; ++s) {
+    const ulonglong2 v = m[s * 32];
+    c = PACKED && cut[s] ? v.y : f2fma(v.x, c, v.y);
+  }
+  return c;
+}
+template <bool PACKED>
+__device__ __forceinline__ void write_map(const ScanParams& p, int64_t chain, int seg, f32x2 A, f32x2 H, bool cut) {
+  if (threadIdx.x < 32) reinterpret_cast<ulonglong2*>(p.maps)[(chain * p.segments + seg) * 32 + threadIdx.x] = make_ulonglong2(A, H);
+  if (PACKED && threadIdx.x == 0) p.map_cuts[chain * p.segments + seg] = cut;
+}
 
-  float c[VEC] = {};
-  if (!PACKED && p.state_in && on) load_f32<VEC>(p.state_in + (int64_t)b * p.C + c0, c);
+// MAPS: only the segment's map, for the first of two launches.
+template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED, bool MAPS>
+__global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
+  typedef Rows<TX, VEC, COOP> RX;
+  typedef Rows<TG, VEC, COOP> RG;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ ScanMaps<NW> sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int seg = (int)(blockIdx.x % p.segments);
+  const int64_t chain = blockIdx.x / p.segments;
+  const int b = PACKED ? 0 : (int)(chain / p.sets);
+  const int base = (int)(chain % p.sets) * 32 * VEC, c0 = base + lane * VEC;
+  const bool on = c0 < p.C;
+  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
+  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
+  TX* h = static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + c0;
+  const int runs = (p.T + RUN - 1) / RUN;
 
-  for (int step = 0; step < p.steps; ++step) {
-    const int t0 = ((step * CL + rank) * NW + warp) * RUN;
-    typename Vec<TX, VEC>::Raw xr[RUN];
-    typename Vec<TG, VEC>::Raw gr[RUN];
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      const bool in = on && t0 + i < p.T;
-      xr[i] = typename Vec<TX, VEC>::Raw{};
-      gr[i] = typename Vec<TG, VEC>::Raw{};
-      if (in) {
-        xr[i] = Vec<TX, VEC>::load(x + (int64_t)(t0 + i) * p.x.s1);
-        gr[i] = Vec<TG, VEC>::load(g + (int64_t)(t0 + i) * p.g.s1);
-      }
+  if (PACKED && !MAPS && p.state_out && seg == 0) pass_empty<VEC>(p, p.state_in, p.state_out, c0, on);
+  if (!p.steps) return;
+  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
+  bool any_cut = false;
+  if (!MAPS) {
+    if (!PACKED && p.state_in && on) c = get_f32<VEC>(p.state_in + (int64_t)b * p.C + c0);
+    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
+  }
+
+  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * (RX::BYTES + RG::BYTES); };
+  auto run_at = [&](int step) { return ((seg * p.steps + step) * NW + warp) * RUN; };
+  auto fetch = [&](int step) {
+    if (step < p.steps) {
+      RX{stage(step)}.fetch(x, p.x.s1, run_at(step), p.T, p.C - base, lane);
+      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, run_at(step), p.T, p.C - base, lane);
     }
+    cp_async_commit();
+  };
+  for (int step = 0; step < STAGES - 1; ++step) fetch(step);
+  for (int step = 0; step < p.steps; ++step) {
+    __syncwarp();
+    fetch(step + STAGES - 1);
+    const int t0 = run_at(step);
     RunMasks k;
     if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const RX xs{stage(step)};
 
-    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run
-    float a[RUN][VEC], u[RUN][VEC], A[VEC], H[VEC];
-    decays<TG, VEC>(gr, a, u);
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; H[v] = 0.f; }
+    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run (after the
+    // run's last cut, a[i] has no meaning)
+    f32x2 a[RUN], u[RUN], A = f2pk(1.f, 1.f), H = f2pk(0.f, 0.f);
+    decays<RG, COMP>(RG{stage(step) + RX::BYTES}, lane, a, u);
+    const unsigned cuts = PACKED ? (k.start | ~k.valid) & ((1u << RUN) - 1) : 0;
     #pragma unroll
     for (int i = 0; i < RUN; ++i) {
-      float xf[VEC];
-      Vec<TX, VEC>::unpack(xr[i], xf);
-      float st[VEC] = {};
-      bool opens = false, out = false;
-      if (PACKED) {
-        opens = (k.start >> i) & 1;
-        out = !((k.valid >> i) & 1);
-        const int n = __shfl_sync(0xffffffffu, k.seq, i);
-        if (opens && p.state_in && on) load_f32<VEC>(p.state_in + (int64_t)n * p.C + c0, st);
-      }
-      #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float in = COMP ? -u[i][v] * xf[v] : xf[v];
-        if (PACKED && (opens || out)) {
-          H[v] = out ? 0.f : fmaf(a[i][v], st[v], in);
-          A[v] = -0.f;
+      const f32x2 in = COMP ? f2mul(u[i], xs.get(i, lane)) : xs.get(i, lane);
+      if (PACKED && ((cuts >> i) & 1)) {
+        const int n = k.sequence(i);
+        f32x2 st = f2pk(0.f, 0.f);
+        if ((k.start >> i) & 1) {
+          if (p.state_in && on) st = get_f32<VEC>(p.state_in + (int64_t)n * p.C + c0);
+          H = f2fma(a[i], st, in);
         } else {
-          H[v] = fmaf(a[i][v], H[v], in);
-          A[v] = PACKED && is_cut(A[v]) ? A[v] : A[v] * a[i][v];
+          H = st;
         }
-        a[i][v] = A[v];
-        u[i][v] = H[v];
+      } else {
+        H = f2fma(a[i], H, in);
+        A = f2mul(A, a[i]);
       }
+      a[i] = A;
+      u[i] = H;
     }
-    float cin[VEC];
-    join<NW, VEC, PACKED>(sh, step & 1, CL, rank, warp, lane, A, H, c, cin);
+    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cuts != 0, c, all, any_cut);
+    if (MAPS) continue;
 
+    const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
     if (on && t0 < p.T) {
-      if (p.carry)
-        store_f32<VEC>(p.carry + ((PACKED ? 0 : (int64_t)b * ((p.T + RUN - 1) / RUN)) + t0 / RUN) * p.C + c0, cin);
+      if (p.carry) put_f32<VEC>(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + c0, cin);
+      TX* out = h + (int64_t)t0 * p.h.s1;
       #pragma unroll
       for (int i = 0; i < RUN; ++i) {
-        #pragma unroll
-        for (int v = 0; v < VEC; ++v) u[i][v] = carry_on<PACKED>(a[i][v], u[i][v], cin[v]);
-        if (t0 + i < p.T) Vec<TX, VEC>::store(h + (int64_t)(t0 + i) * p.h.s1, u[i]);
+        if (!PACKED || i < first_cut) u[i] = f2fma(a[i], cin, u[i]);
+        if (t0 + i < p.T) put<TX, VEC>(out, u[i]);
+        out += p.h.s1;
       }
     }
     if (PACKED && p.state_out && k.last) {
       #pragma unroll
       for (int i = 0; i < RUN; ++i) {
         if (!((k.last >> i) & 1)) continue;
-        const int n = __shfl_sync(0xffffffffu, k.seq, i);
-        if (on) store_f32<VEC>(p.state_out + (int64_t)n * p.C + c0, u[i]);
+        const int n = k.sequence(i);
+        if (on) put_f32<VEC>(p.state_out + (int64_t)n * p.C + c0, u[i]);
       }
     }
   }
-  if (!PACKED && p.state_out && rank == 0 && warp == 0 && on) store_f32<VEC>(p.state_out + (int64_t)b * p.C + c0, c);
+  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
+  else if (!PACKED && p.state_out && seg == p.segments - 1 && warp == 0 && on)
+    put_f32<VEC>(p.state_out + (int64_t)b * p.C + c0, c);
 }
 
-// The adjoint, walked from the last tile to the first; warp 0 of rank 0 takes
-// a step's latest run.  States inside a run are rebuilt from the state that
-// the forward kept before it.
-template <typename TX, typename TG, int VEC, int NW, bool COMP, bool PACKED>
-__global__ void __launch_bounds__(32 * NW) k_scan_bwd(ScanParams p, int CL) {
-  constexpr int CH = 32 * VEC;
-  __shared__ ScanShared<NW, CH> sh;
+// The adjoint, walked from the last tile to the first; warp 0 takes a step's
+// latest run, segment 0 the latest segment.  States inside a run are rebuilt
+// from the state that the forward kept before it.
+template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED, bool MAPS>
+__global__ void __launch_bounds__(32 * NW) k_scan_bwd(const ScanParams p) {
+  typedef Rows<TX, VEC, COOP> RX;
+  typedef Rows<TG, VEC, COOP> RG;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ ScanMaps<NW> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rank = CL == 1 ? 0 : (int)(blockIdx.x % CL);
-  const int64_t chain = blockIdx.x / CL;
-  const int b = (int)(chain / p.sets);
-  const int c0 = (int)(chain % p.sets) * CH + lane * VEC;
+  const int seg = (int)(blockIdx.x % p.segments);
+  const int64_t chain = blockIdx.x / p.segments;
+  const int b = PACKED ? 0 : (int)(chain / p.sets);
+  const int base = (int)(chain % p.sets) * 32 * VEC, c0 = base + lane * VEC;
   const bool on = c0 < p.C;
-  const TX* x = static_cast<const TX*>(p.x.p) + (PACKED ? 0 : (int64_t)b * p.x.s0) + c0;
-  const TG* g = static_cast<const TG*>(p.g.p) + (PACKED ? 0 : (int64_t)b * p.g.s0) + c0;
-  const TX* dh = static_cast<const TX*>(p.h.p) + (PACKED ? 0 : (int64_t)b * p.h.s0) + c0;
-  TX* dx = static_cast<TX*>(const_cast<void*>(p.dx.p)) + (PACKED ? 0 : (int64_t)b * p.dx.s0) + c0;
-  TG* dg = static_cast<TG*>(const_cast<void*>(p.dg.p)) + (PACKED ? 0 : (int64_t)b * p.dg.s0) + c0;
+  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
+  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
+  const TX* dh = static_cast<const TX*>(p.h.p) + b * p.h.s0 + base;
+  TX* dx = static_cast<TX*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + c0;
+  TG* dg = static_cast<TG*>(const_cast<void*>(p.dg.p)) + b * p.dg.s0 + c0;
+  const int runs = (p.T + RUN - 1) / RUN;
 
-  if (PACKED && p.d_state_in && rank == 0) {  // an empty sequence hands its state's gradient through
-    for (int n0 = warp * 32; n0 < p.B; n0 += 32 * NW) {
-      const int n = n0 + lane;
-      unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
-      while (empty) {
-        const int j = n0 + __ffs(empty) - 1;
-        empty &= empty - 1;
-        if (on) {
-          float s[VEC] = {};
-          if (p.d_state_out) load_f32<VEC>(p.d_state_out + (int64_t)j * p.C + c0, s);
-          store_f32<VEC>(p.d_state_in + (int64_t)j * p.C + c0, s);
-        }
-      }
-    }
+  if (PACKED && !MAPS && p.d_state_in && seg == 0) pass_empty<VEC>(p, p.d_state_out, p.d_state_in, c0, on);
+  if (!p.steps) return;
+  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
+  bool any_cut = false;
+  if (!MAPS) {
+    if (!PACKED && p.d_state_out && on) c = get_f32<VEC>(p.d_state_out + (int64_t)b * p.C + c0);
+    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
   }
 
-  if (CL > 1) cluster_sync_all();
-
-  float c[VEC] = {};
-  if (!PACKED && p.d_state_out && on) load_f32<VEC>(p.d_state_out + (int64_t)b * p.C + c0, c);
-
-  for (int step = 0; step < p.steps; ++step) {
-    const int t0 = (p.steps * CL * NW - 1 - ((step * CL + rank) * NW + warp)) * RUN;
-    typename Vec<TX, VEC>::Raw xr[RUN], dr[RUN];
-    typename Vec<TG, VEC>::Raw gr[RUN];
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      const bool in = on && t0 + i < p.T;
-      xr[i] = dr[i] = typename Vec<TX, VEC>::Raw{};
-      gr[i] = typename Vec<TG, VEC>::Raw{};
-      if (in) {
-        xr[i] = Vec<TX, VEC>::load(x + (int64_t)(t0 + i) * p.x.s1);
-        gr[i] = Vec<TG, VEC>::load(g + (int64_t)(t0 + i) * p.g.s1);
-        dr[i] = Vec<TX, VEC>::load(dh + (int64_t)(t0 + i) * p.h.s1);
-      }
+  constexpr int STAGE = 2 * RX::BYTES + RG::BYTES;
+  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
+  auto run_at = [&](int step) { return ((p.segments * p.steps - 1 - (seg * p.steps + step)) * NW + NW - 1 - warp) * RUN; };
+  f32x2 next_state = f2pk(0.f, 0.f);  // state before the next step's run
+  auto fetch = [&](int step) {
+    if (step < p.steps) {
+      const int t0 = run_at(step);
+      RX{stage(step)}.fetch(dh, p.h.s1, t0, p.T, p.C - base, lane);
+      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, t0, p.T, p.C - base, lane);
+      if (!MAPS) RX{stage(step) + RX::BYTES + RG::BYTES}.fetch(x, p.x.s1, t0, p.T, p.C - base, lane);
+      if (!MAPS && on && t0 < p.T) next_state = get_f32<VEC>(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + c0);
     }
-    float hp[VEC] = {};  // state before the run
-    if (on && t0 < p.T)
-      load_f32<VEC>(p.carry + ((PACKED ? 0 : (int64_t)b * ((p.T + RUN - 1) / RUN)) + t0 / RUN) * p.C + c0, hp);
+    cp_async_commit();
+  };
+  static_assert(STAGES == 2, "next_state is one step ahead");
+  fetch(0);
+  for (int step = 0; step < p.steps; ++step) {
+    __syncwarp();
+    f32x2 hp = next_state;
+    fetch(step + 1);
+    const int t0 = run_at(step);
     RunMasks k;
     if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const RX ds{stage(step)}, xs{stage(step) + RX::BYTES + RG::BYTES};
 
     // a[i]: decay of token i; w[i]: what dg multiplies, h_{i-1} or h_{i-1} - x_i
-    float a[RUN][VEC], m[RUN][VEC], w[RUN][VEC];
-    decays<TG, VEC>(gr, a, m);
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      float xf[VEC];
-      Vec<TX, VEC>::unpack(xr[i], xf);
-      if (PACKED && ((k.start >> i) & 1)) {
-        const int n = __shfl_sync(0xffffffffu, k.seq, i);
-        #pragma unroll
-        for (int v = 0; v < VEC; ++v) hp[v] = 0.f;
-        if (p.state_in && on) load_f32<VEC>(p.state_in + (int64_t)n * p.C + c0, hp);
-      }
+    f32x2 a[RUN], m[RUN], w[RUN];
+    decays<RG, COMP && !MAPS>(RG{stage(step) + RX::BYTES}, lane, a, m);
+    if (!MAPS) {
       #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        w[i][v] = COMP ? hp[v] - xf[v] : hp[v];
-        hp[v] = fmaf(a[i][v], hp[v], COMP ? -m[i][v] * xf[v] : xf[v]);
+      for (int i = 0; i < RUN; ++i) {
+        const f32x2 xf = xs.get(i, lane);
+        if (PACKED && ((k.start >> i) & 1)) {
+          const int n = k.sequence(i);
+          hp = p.state_in && on ? get_f32<VEC>(p.state_in + (int64_t)n * p.C + c0) : f2pk(0.f, 0.f);
+        }
+        w[i] = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
+        hp = f2fma(a[i], hp, COMP ? f2mul(m[i], xf) : xf);
       }
     }
     // the run's map from the adjoint after it to the adjoint before it
-    float A[VEC], M[VEC];
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; M[v] = 0.f; }
+    const unsigned cuts = PACKED ? (k.last | ~k.valid) & ((1u << RUN) - 1) : 0;
+    f32x2 A = f2pk(1.f, 1.f), M = f2pk(0.f, 0.f);
     #pragma unroll
     for (int i = RUN - 1; i >= 0; --i) {
-      float df[VEC];
-      Vec<TX, VEC>::unpack(dr[i], df);
-      bool closes = false, out = false;
-      float st[VEC] = {};
-      if (PACKED) {
-        closes = (k.last >> i) & 1;
-        out = !((k.valid >> i) & 1);
-        const int n = __shfl_sync(0xffffffffu, k.seq, i);
-        if (closes && p.d_state_out && on) load_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0, st);
-      }
-      #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (PACKED && (closes || out)) {
-          M[v] = out ? 0.f : a[i][v] * (df[v] + st[v]);
-          A[v] = -0.f;
-        } else {
-          M[v] = a[i][v] * (df[v] + M[v]);
-          A[v] = PACKED && is_cut(A[v]) ? A[v] : A[v] * a[i][v];
+      if (PACKED && ((cuts >> i) & 1)) {
+        const int n = k.sequence(i);
+        M = f2pk(0.f, 0.f);
+        if ((k.last >> i) & 1) {
+          if (p.d_state_out && on) M = get_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0);
+          M = f2mul(a[i], f2add(ds.get(i, lane), M));
         }
+      } else {
+        M = f2mul(a[i], f2add(ds.get(i, lane), M));
+        A = f2mul(A, a[i]);
       }
     }
-    float mu[VEC];
-    join<NW, VEC, PACKED>(sh, step & 1, CL, rank, warp, lane, A, M, c, mu);
+    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cuts != 0, c, all, any_cut);
+    if (MAPS) continue;
 
+    TX* ox = dx + (int64_t)(t0 + RUN - 1) * p.dx.s1;
+    TG* og = dg + (int64_t)(t0 + RUN - 1) * p.dg.s1;
     #pragma unroll
     for (int i = RUN - 1; i >= 0; --i) {
-      float df[VEC], ox[VEC], og[VEC];
-      Vec<TX, VEC>::unpack(dr[i], df);
-      bool out = false;
-      if (PACKED) {
-        out = !((k.valid >> i) & 1);
-        if ((k.last >> i) & 1) {
-          const int n = __shfl_sync(0xffffffffu, k.seq, i);
-          #pragma unroll
-          for (int v = 0; v < VEC; ++v) mu[v] = 0.f;
-          if (p.d_state_out && on) load_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0, mu);
-        }
+      const bool out = PACKED && !((k.valid >> i) & 1);
+      if (PACKED && ((k.last >> i) & 1)) {
+        const int n = k.sequence(i);
+        mu = p.d_state_out && on ? get_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0) : f2pk(0.f, 0.f);
       }
-      #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float l = df[v] + mu[v];
-        ox[v] = COMP ? -m[i][v] * l : l;
-        mu[v] = a[i][v] * l;
-        og[v] = mu[v] * w[i][v];
-        if (PACKED && out) ox[v] = og[v] = mu[v] = 0.f;
-      }
+      const f32x2 l = f2add(ds.get(i, lane), mu);
+      f32x2 vx = COMP ? f2mul(m[i], l) : l;
+      mu = f2mul(a[i], l);
+      f32x2 vg = f2mul(mu, w[i]);
+      if (out) vx = vg = mu = f2pk(0.f, 0.f);
       if (on && t0 + i < p.T) {
-        Vec<TX, VEC>::store(dx + (int64_t)(t0 + i) * p.dx.s1, ox);
-        Vec<TG, VEC>::store(dg + (int64_t)(t0 + i) * p.dg.s1, og);
+        put<TX, VEC>(ox, vx);
+        put<TG, VEC>(og, vg);
       }
+      ox -= p.dx.s1;
+      og -= p.dg.s1;
       if (PACKED && p.d_state_in && ((k.start >> i) & 1)) {
-        const int n = __shfl_sync(0xffffffffu, k.seq, i);
-        if (on) store_f32<VEC>(p.d_state_in + (int64_t)n * p.C + c0, mu);
+        const int n = k.sequence(i);
+        if (on) put_f32<VEC>(p.d_state_in + (int64_t)n * p.C + c0, mu);
       }
     }
   }
-  if (!PACKED && p.d_state_in && rank == 0 && warp == 0 && on)
-    store_f32<VEC>(p.d_state_in + (int64_t)b * p.C + c0, c);
+  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
+  else if (!PACKED && p.d_state_in && seg == p.segments - 1 && warp == 0 && on)
+    put_f32<VEC>(p.d_state_in + (int64_t)b * p.C + c0, c);
 }
 
 // One token per sequence, the decode step: elementwise, state read and
 // written once.  One thread per VEC channels of a sequence.
 template <typename TX, typename TG, int VEC, bool COMP>
-__global__ void __launch_bounds__(256) k_scan_step(ScanParams p) {
+__global__ void __launch_bounds__(256) k_scan_step(const ScanParams p) {
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per = p.C / VEC;
   if (e >= (int64_t)p.B * per) return;
@@ -456,80 +484,128 @@ __global__ void __launch_bounds__(256) k_scan_step(ScanParams p) {
 
 // ---- host ----
 
-static bool rows_ok(const gdn2_view& v, int vec, int elem) {
-  return (uintptr_t)v.data % (vec * elem) == 0 && v.stride0 % vec == 0 && v.stride1 % vec == 0;
+// Rows of v start on `bytes` boundaries.
+static bool rows_ok(const gdn2_view& v, int bytes, int elem) {
+  return (uintptr_t)v.data % bytes == 0 && v.stride0 * elem % bytes == 0 && v.stride1 * elem % bytes == 0;
 }
 
 static int elem_bytes(int dtype) { return dtype == GDN2_DTYPE_BF16 ? 2 : 4; }
 
-// Tiles per step (the cluster): enough CTAs to hold the memory system's
-// latency in flight, no more than the time axis has.
-static int cluster_size(int64_t chains, int tiles) {
-  int cl = 1;
-  while (cl < MAX_CL && chains * cl < 2 * 148 && 2 * cl <= tiles) cl *= 2;
-  return cl;
+// How a call is cut up: channels per lane, 16-byte copies, warps (runs) of a block, segments of the time axis.
+struct ScanPlan {
+  int vec;
+  bool coop;
+  int warps, sets, steps, segments;
+  int64_t chains;
+};
+
+static ScanPlan plan_scan(const gdn2_scan_args* a, bool pairs, bool coop) {
+  ScanPlan n;
+  n.vec = pairs ? 2 : 1;
+  n.coop = pairs && coop;
+  n.sets = (a->channels + 32 * n.vec - 1) / (32 * n.vec);
+  n.chains = (int64_t)n.sets * (a->cu_seqlens ? 1 : a->batch);
+  const int runs = (a->seq_len + RUN - 1) / RUN;
+  n.warps = runs <= 1 && !a->cu_seqlens ? 1 : 4;
+  int tiles = (runs + n.warps - 1) / n.warps;
+  n.segments = 1;
+  if (n.warps == 4 && n.chains < 100 && tiles > 1) {
+    int64_t want = 148 * 4 / n.chains;
+    if (want > MAX_SEGMENTS) want = MAX_SEGMENTS;
+    if (want > tiles) want = tiles;
+    n.steps = (int)((tiles + want - 1) / want);
+    n.segments = (tiles + n.steps - 1) / n.steps;
+  }
+  if (n.segments == 1) n.steps = tiles;
+  return n;
+}
+
+// Workspace of a cut time axis: the maps, their cut flags, and a copy of the
+// initial states for a call that writes the final ones over them.
+struct ScanSpace {
+  size_t cuts, states, bytes;
+};
+static ScanSpace scan_workspace(const ScanPlan& n, const gdn2_scan_args* a) {
+  ScanSpace w{};
+  if (n.segments == 1) return w;
+  w.cuts = (size_t)n.chains * n.segments * 32 * sizeof(ulonglong2);
+  w.states = w.cuts + ((size_t)n.chains * n.segments * sizeof(int) + 15) / 16 * 16;
+  w.bytes = w.states + (a->state_in ? (size_t)a->batch * a->channels * sizeof(float) : 0);
+  return w;
 }
 
 template <typename K>
-static int launch(K kernel, ScanParams& p, int64_t chains, int nw, cudaStream_t st, const char* fn) {
-  p.tiles = (p.T + nw * RUN - 1) / (nw * RUN);
-  const int cl = cluster_size(chains, p.tiles);
-  p.steps = (p.tiles + cl - 1) / cl;
-  if (chains * cl > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: %lld channel sets", fn, (long long)chains);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(chains * cl));
-  cfg.blockDim = dim3(32 * nw);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cl;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p, cl), fn);
+static int launch(K kernel, const ScanParams& p, const ScanPlan& n, int stage, cudaStream_t st, const char* fn) {
+  const int64_t grid = n.chains * n.segments;
+  if (grid > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: %lld blocks", fn, (long long)grid);
+  const int smem = STAGES * n.warps * stage;
+  int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
+  if (rc) return rc;
+  kernel<<<(unsigned)grid, 32 * n.warps, smem, st>>>(p);
+  return check_cuda(cudaGetLastError(), fn);
 }
 
-template <typename TX, typename TG, int VEC, bool COMP>
-static int run_fwd(ScanParams& p, cudaStream_t st, const char* fn) {
-  p.sets = (p.C + 32 * VEC - 1) / (32 * VEC);
-  if (p.cu) return launch(k_scan_fwd<TX, TG, VEC, 4, COMP, true>, p, p.sets, 4, st, fn);
-  const int64_t chains = (int64_t)p.B * p.sets;
-  if (p.T == 1 && !p.carry) {
-    const int64_t n = (int64_t)p.B * (p.C / VEC);
-    if ((n + 255) / 256 > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: too many channels", fn);
-    k_scan_step<TX, TG, VEC, COMP><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p);
+template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED>
+static int run_scan(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  const int rx = Rows<TX, VEC, COOP>::BYTES, rg = Rows<TG, VEC, COOP>::BYTES;
+  int rc = GDN2_OK;
+  if (bwd) {
+    if (NW > 1 && n.segments > 1)
+      rc = launch(k_scan_bwd<TX, TG, VEC, COOP, NW, COMP, PACKED, NW != 1>, p, n, 2 * rx + rg, st, fn);
+    return rc ? rc : launch(k_scan_bwd<TX, TG, VEC, COOP, NW, COMP, PACKED, false>, p, n, 2 * rx + rg, st, fn);
+  }
+  if (NW > 1 && n.segments > 1)
+    rc = launch(k_scan_fwd<TX, TG, VEC, COOP, NW, COMP, PACKED, NW != 1>, p, n, rx + rg, st, fn);
+  return rc ? rc : launch(k_scan_fwd<TX, TG, VEC, COOP, NW, COMP, PACKED, false>, p, n, rx + rg, st, fn);
+}
+
+template <typename TX, typename TG, int VEC, bool COOP, bool COMP>
+static int run_shape(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  if (p.cu) return run_scan<TX, TG, VEC, COOP, 4, COMP, true>(p, n, bwd, st, fn);
+  if (p.T == 1 && !p.carry && !bwd) {
+    const int64_t count = ((int64_t)p.B * (p.C / VEC) + 255) / 256;
+    if (count > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: too many channels", fn);
+    k_scan_step<TX, TG, VEC, COMP><<<(unsigned)count, 256, 0, st>>>(p);
     return check_cuda(cudaGetLastError(), fn);
   }
-  if (p.T <= RUN) return launch(k_scan_fwd<TX, TG, VEC, 1, COMP, false>, p, chains, 1, st, fn);
-  return launch(k_scan_fwd<TX, TG, VEC, 4, COMP, false>, p, chains, 4, st, fn);
-}
-
-template <typename TX, typename TG, int VEC, bool COMP>
-static int run_bwd(ScanParams& p, cudaStream_t st, const char* fn) {
-  p.sets = (p.C + 32 * VEC - 1) / (32 * VEC);
-  if (p.cu) return launch(k_scan_bwd<TX, TG, VEC, 4, COMP, true>, p, p.sets, 4, st, fn);
-  const int64_t chains = (int64_t)p.B * p.sets;
-  if (p.T <= RUN) return launch(k_scan_bwd<TX, TG, VEC, 1, COMP, false>, p, chains, 1, st, fn);
-  return launch(k_scan_bwd<TX, TG, VEC, 4, COMP, false>, p, chains, 4, st, fn);
-}
-
-template <typename TX, typename TG, int VEC>
-static int run_comp(ScanParams& p, bool comp, bool bwd, cudaStream_t st, const char* fn) {
-  if (bwd) return comp ? run_bwd<TX, TG, VEC, true>(p, st, fn) : run_bwd<TX, TG, VEC, false>(p, st, fn);
-  return comp ? run_fwd<TX, TG, VEC, true>(p, st, fn) : run_fwd<TX, TG, VEC, false>(p, st, fn);
+  if (n.warps == 1) return run_scan<TX, TG, VEC, COOP, 1, COMP, false>(p, n, bwd, st, fn);
+  return run_scan<TX, TG, VEC, COOP, 4, COMP, false>(p, n, bwd, st, fn);
 }
 
 template <typename TX, typename TG>
-static int run_vec(ScanParams& p, bool pairs, bool comp, bool bwd, cudaStream_t st, const char* fn) {
-  return pairs ? run_comp<TX, TG, 2>(p, comp, bwd, st, fn) : run_comp<TX, TG, 1>(p, comp, bwd, st, fn);
+static int run_vec(const ScanParams& p, const ScanPlan& n, bool comp, bool bwd, cudaStream_t st, const char* fn) {
+  if (n.coop)
+    return comp ? run_shape<TX, TG, 2, true, true>(p, n, bwd, st, fn)
+                : run_shape<TX, TG, 2, true, false>(p, n, bwd, st, fn);
+  if (n.vec == 2)
+    return comp ? run_shape<TX, TG, 2, false, true>(p, n, bwd, st, fn)
+                : run_shape<TX, TG, 2, false, false>(p, n, bwd, st, fn);
+  return comp ? run_shape<TX, TG, 1, false, true>(p, n, bwd, st, fn)
+              : run_shape<TX, TG, 1, false, false>(p, n, bwd, st, fn);
 }
 
-static int dispatch(ScanParams& p, const gdn2_scan_args* a, bool pairs, bool bwd, cudaStream_t st, const char* fn) {
+static int dispatch(ScanParams& p, const gdn2_scan_args* a, const ScanPlan& n, bool bwd, void* ws, size_t ws_bytes,
+                    cudaStream_t st, const char* fn) {
+  const ScanSpace w = scan_workspace(n, a);
+  if (w.bytes && (!ws || ws_bytes < w.bytes))
+    return set_error(GDN2_EWORKSPACE, "%s: workspace %zu bytes < required %zu", fn, ws ? ws_bytes : 0, w.bytes);
+  if (w.bytes && (uintptr_t)ws % 16) return set_error(GDN2_EINVAL, "%s: workspace must be 16-byte aligned", fn);
+  p.sets = n.sets; p.steps = n.steps; p.segments = n.segments;
+  if (w.bytes) {
+    char* at = static_cast<char*>(ws);
+    p.maps = reinterpret_cast<float2*>(at);
+    p.map_cuts = reinterpret_cast<int*>(at + w.cuts);
+    if (!bwd && p.state_in && p.state_in == p.state_out) {
+      int rc = check_cuda(cudaMemcpyAsync(at + w.states, p.state_in, (size_t)p.B * p.C * sizeof(float),
+                                          cudaMemcpyDeviceToDevice, st), fn);
+      if (rc) return rc;
+      p.state_in = reinterpret_cast<const float*>(at + w.states);
+    }
+  }
   const bool comp = a->complement != 0;
-  if (a->dtype == GDN2_DTYPE_F32) return run_vec<float, float>(p, pairs, comp, bwd, st, fn);
-  if (a->g_dtype == GDN2_DTYPE_F32) return run_vec<__nv_bfloat16, float>(p, pairs, comp, bwd, st, fn);
-  return run_vec<__nv_bfloat16, __nv_bfloat16>(p, pairs, comp, bwd, st, fn);
+  if (a->dtype == GDN2_DTYPE_F32) return run_vec<float, float>(p, n, comp, bwd, st, fn);
+  if (a->g_dtype == GDN2_DTYPE_F32) return run_vec<__nv_bfloat16, float>(p, n, comp, bwd, st, fn);
+  return run_vec<__nv_bfloat16, __nv_bfloat16>(p, n, comp, bwd, st, fn);
 }
 
 static int check_scan(const gdn2_scan_args* a, const char* fn) {
@@ -556,7 +632,31 @@ static void fill(ScanParams& p, const gdn2_scan_args* a) {
   p.carry = a->carry;
 }
 
-int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, cudaStream_t st) {
+// The plan by the rows' alignment; outputs need pairs, inputs 16 bytes for the copies.
+static ScanPlan plan_fwd(const gdn2_scan_args* a, const gdn2_view& h) {
+  const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
+  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * ex, ex) && rows_ok(a->g, 2 * eg, eg) && rows_ok(h, 2 * ex, ex);
+  return plan_scan(a, pairs, a->channels * ex % 16 == 0 && rows_ok(a->x, 16, ex) && rows_ok(a->g, 16, eg));
+}
+
+static ScanPlan plan_bwd(const gdn2_scan_bwd_args* q) {
+  const gdn2_scan_args* a = &q->fwd;
+  const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
+  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * ex, ex) && rows_ok(a->g, 2 * eg, eg) &&
+                     rows_ok(q->d_h, 2 * ex, ex) && rows_ok(q->dx, 2 * ex, ex) && rows_ok(q->dg, 2 * eg, eg);
+  return plan_scan(a, pairs, a->channels * ex % 16 == 0 && rows_ok(a->x, 16, ex) && rows_ok(a->g, 16, eg) &&
+                                 rows_ok(q->d_h, 16, ex));
+}
+
+size_t scan_workspace_bytes(const gdn2_scan_args* a, const gdn2_view& h) {
+  return check_scan(a, "gdn2_gated_scan_workspace_bytes") ? 0 : scan_workspace(plan_fwd(a, h), a).bytes;
+}
+size_t scan_bwd_workspace_bytes(const gdn2_scan_bwd_args* q) {
+  return !q || check_scan(&q->fwd, "gdn2_gated_scan_bwd_workspace_bytes") ? 0 : scan_workspace(plan_bwd(q), &q->fwd).bytes;
+}
+
+int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_out, void* ws, size_t ws_bytes,
+                    cudaStream_t st) {
   const char* fn = "gdn2_gated_scan";
   int rc = check_scan(a, fn);
   if (rc) return rc;
@@ -565,12 +665,10 @@ int launch_scan_fwd(const gdn2_scan_args* a, const gdn2_view& h, float* state_ou
   fill(p, a);
   p.h = make_dview(h);
   p.state_out = state_out;
-  const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2, ex) && rows_ok(a->g, 2, eg) && rows_ok(h, 2, ex);
-  return dispatch(p, a, pairs, false, st, fn);
+  return dispatch(p, a, plan_fwd(a, h), false, ws, ws_bytes, st, fn);
 }
 
-int launch_scan_bwd(const gdn2_scan_bwd_args* q, cudaStream_t st) {
+int launch_scan_bwd(const gdn2_scan_bwd_args* q, void* ws, size_t ws_bytes, cudaStream_t st) {
   const char* fn = "gdn2_gated_scan_bwd";
   if (!q) return set_error(GDN2_EINVAL, "%s: null args", fn);
   const gdn2_scan_args* a = &q->fwd;
@@ -584,10 +682,7 @@ int launch_scan_bwd(const gdn2_scan_bwd_args* q, cudaStream_t st) {
   p.dx = make_dview(q->dx); p.dg = make_dview(q->dg);
   p.d_state_out = q->d_state_out;
   p.d_state_in = q->d_state_in;
-  const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2, ex) && rows_ok(a->g, 2, eg) && rows_ok(q->d_h, 2, ex) &&
-                     rows_ok(q->dx, 2, ex) && rows_ok(q->dg, 2, eg);
-  return dispatch(p, a, pairs, true, st, fn);
+  return dispatch(p, a, plan_bwd(q), true, ws, ws_bytes, st, fn);
 }
 
 }  // namespace gdn2

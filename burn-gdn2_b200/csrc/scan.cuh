@@ -67,14 +67,15 @@ __device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int N, 
   return lo >= 1 && lo <= N ? lo - 1 : -1;
 }
 
-// a = e^g and m = e^g - 1 of two log decays.  Argument reduction by powers of
+// a = e^g and k = 1 - e^g of two log decays.  Argument reduction by powers of
 // two (Cody and Waite): g = n ln 2 + r with |r| <= ln 2 / 2, p = e^r - 1 by its
 // Taylor polynomial to r^7 (its first dropped term is below 2^-25 of p), then
-// a = 2^n (1 + p), m = 2^n p + (2^n - 1).  For n = 0 (the slow channels, whose
-// decay is applied thousands of times) a is 1 + p rounded once and m is p
+// a = 2^n (1 + p), k = (1 - 2^n) - 2^n p.  For n = 0 (the slow channels, whose
+// decay is applied thousands of times) a is 1 + p rounded once and k is -p
 // itself, without the cancellation of 1 - a: an ulp of bias in a would grow
 // by the length of the channel's memory.  Valid for |g| <= 87; NaN stays NaN.
-__device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& m) {
+template <bool WITH_K>
+__device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& k) {
   const f32x2 kLog2e = f2pk(1.44269504088896f, 1.44269504088896f);
   const f32x2 kMagic = f2pk(12582912.f, 12582912.f);  // 1.5 * 2^23: its sum rounds to a whole number
   const f32x2 kOne = f2pk(1.f, 1.f), kMinus = f2pk(-1.f, -1.f);
@@ -93,13 +94,7 @@ __device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& m) {
   const f32x2 s = f2pk(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
                        __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
   a = f2fma(s, p, s);
-  m = f2fma(s, p, f2fma(s, kOne, kMinus));
-}
-__device__ __forceinline__ void exp_pair(float g0, float g1, float& a0, float& a1, float& m0, float& m1) {
-  f32x2 a, m;
-  exp_pair(f2pk(g0, g1), a, m);
-  f2un(a, a0, a1);
-  f2un(m, m0, m1);
+  if constexpr (WITH_K) k = f2fma(f2mul(s, kMinus), p, f2fma(s, kMinus, kOne));
 }
 constexpr float kExpRange = 87.f;
 

@@ -338,8 +338,9 @@ GDN2_API int gdn2_rms_norm_gate(const gdn2_dims* dims, int32_t dtype, gdn2_view 
  *   state_out : [batch, C] f32 or NULL; may be state_in
  *   carry     : [batch (1 when packed), ceil(seq_len / 16), C] f32 or NULL:
  *               the state before every 16th token, kept for the backward
- * f32 arithmetic; h is rounded once.  No workspace, no atomics: results do
- * not vary from call to call.
+ * f32 arithmetic; h is rounded once; no atomics: results do not vary from
+ * call to call.  The workspace (16-byte aligned) holds the maps of the time
+ * axis's segments; 0 bytes when there are chains enough without them.
  *
  * gdn2_gated_scan_bwd: the adjoint.  fwd as it was given to the forward,
  * with the carry that it wrote; d_h (dtype) and d_state_out (NULL = zeros)
@@ -367,8 +368,11 @@ typedef struct gdn2_scan_bwd_args {
   float* d_state_in;
 } gdn2_scan_bwd_args;
 
-GDN2_API int gdn2_gated_scan(const gdn2_scan_args* args, gdn2_view h, float* state_out, void* stream);
-GDN2_API int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* args, void* stream);
+GDN2_API size_t gdn2_gated_scan_workspace_bytes(const gdn2_scan_args* args, gdn2_view h);
+GDN2_API int gdn2_gated_scan(const gdn2_scan_args* args, gdn2_view h, float* state_out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+GDN2_API size_t gdn2_gated_scan_bwd_workspace_bytes(const gdn2_scan_bwd_args* args);
+GDN2_API int gdn2_gated_scan_bwd(const gdn2_scan_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Causal depthwise convolution of 4 taps with SiLU, with its backward and

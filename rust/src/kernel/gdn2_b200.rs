@@ -304,8 +304,12 @@ extern "C" {
                            stream: *mut c_void) -> i32;
     pub fn gdn2_rms_norm_gate(dims: *const Gdn2Dims, dtype: i32, o: Gdn2View, gate: Gdn2View, weight: *const f32,
                               eps: f32, out: Gdn2View, stream: *mut c_void) -> i32;
-    pub fn gdn2_gated_scan(args: *const Gdn2ScanArgs, h: Gdn2View, state_out: *mut f32, stream: *mut c_void) -> i32;
-    pub fn gdn2_gated_scan_bwd(args: *const Gdn2ScanBwdArgs, stream: *mut c_void) -> i32;
+    pub fn gdn2_gated_scan_workspace_bytes(args: *const Gdn2ScanArgs, h: Gdn2View) -> usize;
+    pub fn gdn2_gated_scan(args: *const Gdn2ScanArgs, h: Gdn2View, state_out: *mut f32, workspace: *mut c_void,
+                           workspace_bytes: usize, stream: *mut c_void) -> i32;
+    pub fn gdn2_gated_scan_bwd_workspace_bytes(args: *const Gdn2ScanBwdArgs) -> usize;
+    pub fn gdn2_gated_scan_bwd(args: *const Gdn2ScanBwdArgs, workspace: *mut c_void, workspace_bytes: usize,
+                               stream: *mut c_void) -> i32;
     pub fn gdn2_causal_conv(args: *const Gdn2ConvArgs, y: Gdn2View, cache_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn gdn2_causal_conv_bwd_workspace_bytes(args: *const Gdn2ConvBwdArgs) -> usize;
     pub fn gdn2_causal_conv_bwd(args: *const Gdn2ConvBwdArgs, workspace: *mut c_void, workspace_bytes: usize,

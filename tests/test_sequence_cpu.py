@@ -53,24 +53,45 @@ def test_scan_argument_errors(over, status):
 
     out = _lib.View(1 << 20, 64, 8, 0)
     a = _scan_args(**over)
-    assert LIB.gdn2_gated_scan(ctypes.byref(a), out, None, None) == status
+    assert LIB.gdn2_gated_scan(ctypes.byref(a), out, None, None, 0, None) == status
     assert LIB.gdn2_last_error().decode().startswith("gdn2_gated_scan:")
     b = _lib.ScanBwdArgs(a, out, None, out, out, None)
-    assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None) == status
+    assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None, 0, None) == status
 
 
 def test_scan_null_pointers():
     from burn_gdn2 import LIB, _lib
 
     out, none = _lib.View(1 << 20, 64, 8, 0), _lib.View()
-    assert LIB.gdn2_gated_scan(None, out, None, None) == _lib.GDN2_EINVAL
-    assert LIB.gdn2_gated_scan_bwd(None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan(None, out, None, None, 0, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan_bwd(None, None, 0, None) == _lib.GDN2_EINVAL
     a = _scan_args()
-    assert LIB.gdn2_gated_scan(ctypes.byref(a), none, None, None) == _lib.GDN2_EINVAL
-    assert LIB.gdn2_gated_scan(ctypes.byref(_scan_args(x=none)), out, None, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan(ctypes.byref(a), none, None, None, 0, None) == _lib.GDN2_EINVAL
+    assert LIB.gdn2_gated_scan(ctypes.byref(_scan_args(x=none)), out, None, None, 0, None) == _lib.GDN2_EINVAL
     for args in ((a, none, out, out), (a, out, none, out), (a, out, out, none), (a, out, out, out)):  # the last: no carry
         b = _lib.ScanBwdArgs(args[0], args[1], None, args[2], args[3], None)
-        assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None) == _lib.GDN2_EINVAL
+        assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), None, 0, None) == _lib.GDN2_EINVAL
+
+
+def test_scan_workspace():
+    """Few chains over a long axis need one, many do not; too small a one is refused."""
+    from burn_gdn2 import LIB, _lib
+
+    out = _lib.View(1 << 20, 1 << 20, 8, 0)
+    long = _scan_args(batch=1, seq_len=4096)
+    need = LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(long), out)
+    assert need > 0
+    assert LIB.gdn2_gated_scan(ctypes.byref(long), out, None, None, 0, None) == _lib.GDN2_EWORKSPACE
+    assert LIB.gdn2_gated_scan(ctypes.byref(long), out, None, 1 << 20, need - 1, None) == _lib.GDN2_EWORKSPACE
+    assert LIB.gdn2_gated_scan(ctypes.byref(long), out, None, (1 << 20) + 4, need, None) == _lib.GDN2_EINVAL
+    long.carry = 1 << 20
+    b = _lib.ScanBwdArgs(long, out, None, out, out, None)
+    need = LIB.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(b))
+    assert need > 0
+    assert LIB.gdn2_gated_scan_bwd(ctypes.byref(b), 1 << 20, need - 1, None) == _lib.GDN2_EWORKSPACE
+    assert LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(_scan_args(batch=512, seq_len=4096)), out) == 0
+    assert LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(_scan_args(seq_len=0)), out) == 0
+    assert LIB.gdn2_gated_scan_workspace_bytes(None, out) == 0
 
 
 def test_struct_layouts_match_header(tmp_path):
