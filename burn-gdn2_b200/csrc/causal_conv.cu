@@ -6,22 +6,28 @@
 //
 // The three tokens before a sequence are its cache, or copies of its first
 // token (src/short_conv.rs:42-54).  Bound by HBM: x in and y out, or x and dy
-// in and dx out.  A warp takes RUN tokens of 32 * VEC channels with all their
-// rows in flight, and the three rows in front (behind too, in the adjoint)
-// once more, which neighbouring warps have just read.  The adjoint forms pre
-// again from x; each lane sums dw over the runs that its block walks, the
-// block adds its warps' sums and a second kernel the blocks', in a fixed
-// order.
+// in and dx out.  A warp walks a span of tokens of 32 * VEC channels in runs
+// that are copied to shared memory a run ahead; the three values before a
+// token stay in registers, so a span reads nothing twice but the three rows
+// in front of it.  In the adjoint the dx of the last three tokens stay in
+// registers as well until the tokens behind have added their parts, and a span
+// ends with the three tokens behind it (13 own tokens and those make its last
+// run).  Runs inside a sequence take a short path; those where one begins or
+// ends sort out caches and copies token by token.  Each lane sums dw over its
+// spans, the block adds its warps' sums and a second kernel the blocks', in a
+// fixed order.
 #include "scan.cuh"
 
 namespace gdn2 {
 
 constexpr int HALO = 3;  // taps before a token
-constexpr int CONV_RUN = 16, CONV_WARPS = 4;
+constexpr int CONV_WARPS = 4;
 
 struct ConvParams {
   int B, T, C;
-  int runs, sets;
+  int sets;   // sets of 32 * VEC channels
+  int span;   // tokens of a warp's span
+  int spans;  // spans of a sequence (of the packed buffer)
   const int* cu;
   DView x, y;  // y: out, or dy
   DView dx;
@@ -33,300 +39,328 @@ struct ConvParams {
   float* part;  // [gridDim.y][C][4]
 };
 
-// Where a token lies in its sequence: number and first row (dense: its batch row and 0).
-struct Place {
-  int seq, first, end;
+// What a run's tokens are: one bit a token; lane i holds the sequence and
+// the first row of token i.
+struct ConvRun {
+  unsigned start, last, valid;
+  int seq, first;
+  __device__ __forceinline__ bool inside() const { return !start && !last && valid == (1u << RUN) - 1; }
 };
 template <bool PACKED>
-__device__ __forceinline__ Place place_of(const ConvParams& p, int b, int t) {
-  if (!PACKED) return Place{t < p.T ? b : -1, 0, p.T};
-  Place q{-1, 0, 0};
-  if (t < p.T) {
-    q.seq = find_sequence(p.cu, p.B, t);
-    if (q.seq >= 0) {
-      q.first = __ldg(p.cu + q.seq);
-      q.end = __ldg(p.cu + q.seq + 1);
-      if (q.end > p.T) q.end = p.T;
+__device__ __forceinline__ ConvRun conv_run(const ConvParams& p, int b, int t0, int lane) {
+  const int t = t0 + lane;
+  ConvRun k{0, 0, 0, -1, 0};
+  bool l = false;
+  if (lane < RUN && t < p.T) {
+    if (PACKED) {
+      k.seq = find_sequence(p.cu, p.B, t);
+      if (k.seq >= 0) {
+        k.first = __ldg(p.cu + k.seq);
+        l = t + 1 == p.T || __ldg(p.cu + k.seq + 1) == t + 1;
+      }
+    } else {
+      k.seq = b;
+      l = t + 1 == p.T;
     }
   }
-  return q;
+  k.valid = __ballot_sync(0xffffffffu, k.seq >= 0);
+  k.start = __ballot_sync(0xffffffffu, k.seq >= 0 && k.first == t);
+  k.last = __ballot_sync(0xffffffffu, l);
+  return k;
 }
 
-template <int VEC>
-__device__ __forceinline__ const float* cache_row(const float* cache, int seq, int slot, int C, int c0) {
-  return cache + ((int64_t)seq * HALO + slot) * C + c0;
+// Row `slot` of a sequence's cache.
+__device__ __forceinline__ int64_t cache_at(const ConvParams& p, int seq, int slot, int c0) {
+  return ((int64_t)seq * HALO + slot) * p.C + c0;
 }
 
 // Empty sequences: the cache (its gradient) goes through; without one a new
 // cache is zero.
 template <int VEC>
-__device__ __forceinline__ void pass_empty(const ConvParams& p, const float* from, float* to, int c0, bool on,
-                                           int warp, int lane) {
-  for (int n0 = warp * 32; n0 < p.B; n0 += 32 * CONV_WARPS) {
+__device__ __forceinline__ void pass_empty(const ConvParams& p, const float* from, float* to, int c0, bool on) {
+  const int lane = threadIdx.x & 31;
+  for (int n0 = (int)threadIdx.x - lane; n0 < p.B; n0 += blockDim.x) {
     const int n = n0 + lane;
-    bool e = false;
-    if (n < p.B) {
-      const int a = __ldg(p.cu + n);
-      e = __ldg(p.cu + n + 1) <= a || a >= p.T;
-    }
-    unsigned empty = __ballot_sync(0xffffffffu, e);
+    unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
     while (empty) {
       const int j = n0 + __ffs(empty) - 1;
       empty &= empty - 1;
       if (!on) continue;
       #pragma unroll
-      for (int s = 0; s < HALO; ++s) {
-        float v[VEC] = {};
-        if (from) load_f32<VEC>(cache_row<VEC>(from, j, s, p.C, c0), v);
-        store_f32<VEC>(to + ((int64_t)j * HALO + s) * p.C + c0, v);
-      }
+      for (int s = 0; s < HALO; ++s)
+        put_f32<VEC>(to + cache_at(p, j, s, c0), from ? get_f32<VEC>(from + cache_at(p, j, s, c0)) : f2pk(0.f, 0.f));
     }
   }
 }
 
-// The three values before row t of a sequence, oldest first.
 template <typename T, int VEC>
-__device__ __forceinline__ void window_before(const ConvParams& p, const T* x, const Place& q, int t, int c0,
-                                              float (&win)[HALO][VEC]) {
+__device__ __forceinline__ f32x2 get(const T* p) {
+  float f[2] = {0.f, 0.f};
+  if constexpr (VEC == 2) Vec<T, 2>::unpack(Vec<T, 2>::load(p), f);
+  else f[0] = to_f32<T>(*p);
+  return f2pk(f[0], f[1]);
+}
+
+// The three values before row t of sequence seq that begins at row first, oldest first; x at this lane's channels.
+template <typename T, int VEC>
+__device__ __forceinline__ void window_before(const ConvParams& p, const T* x, int seq, int first, int t, int c0,
+                                              bool on, f32x2 (&win)[HALO]) {
   #pragma unroll
   for (int i = 0; i < HALO; ++i) {
     const int row = t - HALO + i;
-    if (row >= q.first)
-      Vec<T, VEC>::unpack(Vec<T, VEC>::load(x + (int64_t)row * p.x.s1), win[i]);
-    else if (p.cache_in)
-      load_f32<VEC>(cache_row<VEC>(p.cache_in, q.seq, row - q.first + HALO, p.C, c0), win[i]);
-    else
-      Vec<T, VEC>::unpack(Vec<T, VEC>::load(x + (int64_t)q.first * p.x.s1), win[i]);
+    win[i] = f2pk(0.f, 0.f);
+    if (!on) continue;
+    if (row >= first) win[i] = get<T, VEC>(x + (int64_t)row * p.x.s1);
+    else if (p.cache_in) win[i] = get_f32<VEC>(p.cache_in + cache_at(p, seq, row - first + HALO, c0));
+    else win[i] = get<T, VEC>(x + (int64_t)first * p.x.s1);
   }
 }
 
-template <typename T, int VEC, bool PACKED>
-__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(ConvParams p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chain = blockIdx.x;
-  const int b = (int)(chain / p.sets);
-  const int c0 = (int)(chain % p.sets) * 32 * VEC + lane * VEC;
-  const bool on = c0 < p.C;
-  const T* x = static_cast<const T*>(p.x.p) + (PACKED ? 0 : (int64_t)b * p.x.s0) + c0;
-  T* y = static_cast<T*>(const_cast<void*>(p.y.p)) + (PACKED ? 0 : (int64_t)b * p.y.s0) + c0;
-  if (PACKED && p.cache_out && blockIdx.y == 0) pass_empty<VEC>(p, p.cache_in, p.cache_out, c0, on, warp, lane);
+__device__ __forceinline__ f32x2 taps(const f32x2 (&win)[HALO], f32x2 x, const f32x2 (&w)[HALO + 1]) {
+  return f2fma(x, w[3], f2fma(win[2], w[2], f2fma(win[1], w[1], f2mul(win[0], w[0]))));
+}
+__device__ __forceinline__ void slide(f32x2 (&win)[HALO], f32x2 x) {
+  win[0] = win[1];
+  win[1] = win[2];
+  win[2] = x;
+}
+// sigmoid of a pair
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 t) {
+  float t0, t1;
+  f2un(t, t0, t1);
+  return f2pk(__fdividef(1.f, 1.f + __expf(-t0)), __fdividef(1.f, 1.f + __expf(-t1)));
+}
 
-  float w[VEC][HALO + 1];
+template <int VEC>
+__device__ __forceinline__ void load_taps(const ConvParams& p, int c0, bool on, f32x2 (&w)[HALO + 1]) {
   #pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    #pragma unroll
-    for (int j = 0; j <= HALO; ++j) w[v][j] = on ? __ldg(p.w + (int64_t)(c0 + v) * (HALO + 1) + j) : 0.f;
+  for (int j = 0; j <= HALO; ++j)
+    w[j] = on ? f2pk(__ldg(p.w + (int64_t)c0 * 4 + j), VEC == 2 ? __ldg(p.w + (int64_t)(c0 + VEC - 1) * 4 + j) : 0.f)
+              : f2pk(0.f, 0.f);
+}
 
-  for (int run = blockIdx.y * CONV_WARPS + warp; run < p.runs; run += gridDim.y * CONV_WARPS) {
-    const int t0 = run * CONV_RUN;
-    typename Vec<T, VEC>::Raw xr[CONV_RUN];
-    #pragma unroll
-    for (int i = 0; i < CONV_RUN; ++i) {
-      xr[i] = typename Vec<T, VEC>::Raw{};
-      if (on && t0 + i < p.T) xr[i] = Vec<T, VEC>::load(x + (int64_t)(t0 + i) * p.x.s1);
-    }
-    // lane i: the place of token i
-    const Place mine = place_of<PACKED>(p, b, lane < CONV_RUN ? t0 + lane : p.T);
-    const unsigned valid = __ballot_sync(0xffffffffu, mine.seq >= 0);
-    const unsigned start = __ballot_sync(0xffffffffu, mine.seq >= 0 && mine.first == t0 + lane);
-    const unsigned last = __ballot_sync(0xffffffffu, mine.seq >= 0 && mine.end == t0 + lane + 1);
-    float win[HALO][VEC] = {};
-    if (valid & 1) {
-      const Place q{__shfl_sync(0xffffffffu, mine.seq, 0), __shfl_sync(0xffffffffu, mine.first, 0), 0};
-      if (on) window_before<T, VEC>(p, x, q, t0, c0, win);
-    }
-    #pragma unroll
-    for (int i = 0; i < CONV_RUN; ++i) {
-      float xf[VEC], out[VEC];
-      Vec<T, VEC>::unpack(xr[i], xf);
-      if (PACKED && i && ((start >> i) & 1)) {
-        const Place q{__shfl_sync(0xffffffffu, mine.seq, i), t0 + i, 0};
-        if (on) window_before<T, VEC>(p, x, q, t0 + i, c0, win);
+template <typename T, int VEC, bool COOP, bool PACKED>
+__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p) {
+  typedef Rows<T, VEC, COOP> R;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = (int)blockIdx.x * 32 * VEC, c0 = base + lane * VEC;
+  const bool on = c0 < p.C;
+  if (PACKED && p.cache_out && blockIdx.y == 0) pass_empty<VEC>(p, p.cache_in, p.cache_out, c0, on);
+  f32x2 w[HALO + 1];
+  load_taps<VEC>(p, c0, on, w);
+
+  const int64_t units = (int64_t)p.spans * (PACKED ? 1 : p.B);
+  for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < units; unit += (int64_t)gridDim.y * CONV_WARPS) {
+    const int b = PACKED ? 0 : (int)(unit / p.spans);
+    const int s0 = (int)(PACKED ? unit : unit % p.spans) * p.span, s1 = s0 + p.span < p.T ? s0 + p.span : p.T;
+    const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
+    T* y = static_cast<T*>(const_cast<void*>(p.y.p)) + b * p.y.s0 + c0;
+    auto rows = [&](int run) { return R{smem + ((run % STAGES) * CONV_WARPS + warp) * R::BYTES}; };
+    auto fetch = [&](int run) {
+      if (s0 + run * RUN < s1) rows(run).fetch(x, p.x.s1, s0 + run * RUN, p.T, p.C - base, lane);
+      cp_async_commit();
+    };
+    __syncwarp();
+    fetch(0);
+    f32x2 win[HALO];
+    for (int run = 0, t0 = s0; t0 < s1; ++run, t0 += RUN) {
+      __syncwarp();
+      fetch(run + 1);
+      const ConvRun k = conv_run<PACKED>(p, b, t0, lane);
+      if (t0 == s0) {  // the tokens in front, of a span that begins inside a sequence
+        #pragma unroll
+        for (int i = 0; i < HALO; ++i) win[i] = f2pk(0.f, 0.f);
+        const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
+        if ((k.valid & 1) && !(k.start & 1)) window_before<T, VEC>(p, x + lane * VEC, seq, first, t0, c0, on, win);
       }
-      #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float s = win[0][v] * w[v][0];
-        s = fmaf(win[1][v], w[v][1], s);
-        s = fmaf(win[2][v], w[v][2], s);
-        s = fmaf(xf[v], w[v][3], s);
-        out[v] = !PACKED || ((valid >> i) & 1) ? silu_f(s) : 0.f;
-        win[0][v] = win[1][v];
-        win[1][v] = win[2][v];
-        win[2][v] = xf[v];
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const R xs = rows(run);
+      T* out = y + (int64_t)t0 * p.y.s1;
+      if (k.inside() && t0 + RUN <= s1) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          const f32x2 xf = xs.get(i, lane), pre = taps(win, xf, w);
+          if (on) put<T, VEC>(out, f2mul(pre, sigmoid2(pre)));
+          out += p.y.s1;
+          slide(win, xf);
+        }
+        continue;
       }
-      if (on && t0 + i < p.T) Vec<T, VEC>::store(y + (int64_t)(t0 + i) * p.y.s1, out);
-      if (((last >> i) & 1) && p.cache_out) {
-        const int n = __shfl_sync(0xffffffffu, mine.seq, i);
-        if (on)
+      #pragma unroll 1
+      for (int i = 0; i < RUN && t0 + i < s1; ++i) {
+        const int seq = __shfl_sync(0xffffffffu, k.seq, i);
+        const f32x2 xf = xs.get(i, lane);
+        if ((k.start >> i) & 1) window_before<T, VEC>(p, x + lane * VEC, seq, t0 + i, t0 + i, c0, on, win);
+        const f32x2 pre = taps(win, xf, w);
+        if (on) put<T, VEC>(out, (k.valid >> i) & 1 ? f2mul(pre, sigmoid2(pre)) : f2pk(0.f, 0.f));
+        out += p.y.s1;
+        slide(win, xf);
+        if (((k.last >> i) & 1) && p.cache_out && on)
+          #pragma unroll
+          for (int s = 0; s < HALO; ++s) put_f32<VEC>(p.cache_out + cache_at(p, seq, s, c0), win[s]);
+      }
+    }
+  }
+}
+
+// Adjoint.  Token s adds w[3-k] dpre_s to dx of token s - k, and to the
+// gradient of the three values before its sequence where s - k lies there;
+// the span that holds the sequence's first token collects those.
+template <typename T, int VEC, bool COOP, bool PACKED>
+__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p) {
+  typedef Rows<T, VEC, COOP> R;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int base = (int)blockIdx.x * 32 * VEC, c0 = base + lane * VEC;
+  const bool on = c0 < p.C;
+  const f32x2 zero = f2pk(0.f, 0.f), one = f2pk(1.f, 1.f), minus = f2pk(-1.f, -1.f);
+  if (PACKED && p.d_cache_in && blockIdx.y == 0) pass_empty<VEC>(p, p.d_cache_out, p.d_cache_in, c0, on);
+  f32x2 w[HALO + 1], dw[HALO + 1];
+  load_taps<VEC>(p, c0, on, w);
+  #pragma unroll
+  for (int j = 0; j <= HALO; ++j) dw[j] = zero;
+
+  const int64_t units = (int64_t)p.spans * (PACKED ? 1 : p.B);
+  for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < units; unit += (int64_t)gridDim.y * CONV_WARPS) {
+    const int b = PACKED ? 0 : (int)(unit / p.spans);
+    const int s0 = (int)(PACKED ? unit : unit % p.spans) * p.span, s1 = s0 + p.span < p.T ? s0 + p.span : p.T;
+    const int end = s1 + HALO;  // rows walked: a token's dx leaves three tokens later
+    const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
+    const T* dy = static_cast<const T*>(p.y.p) + b * p.y.s0 + base;
+    T* dx = static_cast<T*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + c0;
+    auto rows = [&](int run, int which) {
+      return R{smem + (((run % STAGES) * CONV_WARPS + warp) * 2 + which) * R::BYTES};
+    };
+    auto fetch = [&](int run) {
+      const int t0 = s0 + run * RUN;
+      if (t0 < end) {
+        rows(run, 0).fetch(x, p.x.s1, t0, p.T, p.C - base, lane);
+        rows(run, 1).fetch(dy, p.y.s1, t0, p.T, p.C - base, lane);
+      }
+      cp_async_commit();
+    };
+    __syncwarp();
+    fetch(0);
+    f32x2 win[HALO], pend[HALO] = {zero, zero, zero}, before[HALO] = {zero, zero, zero};
+    int pos = HALO;      // place of the next token in its sequence, as far as the first three count
+    bool owned = false;  // the sequence begins in this span
+    for (int run = 0, t0 = s0; t0 < end; ++run, t0 += RUN) {
+      __syncwarp();
+      fetch(run + 1);
+      const ConvRun k = conv_run<PACKED>(p, b, t0, lane);
+      if (t0 == s0) {
+        #pragma unroll
+        for (int i = 0; i < HALO; ++i) win[i] = zero;
+        const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
+        if ((k.valid & 1) && !(k.start & 1)) {
+          window_before<T, VEC>(p, x + lane * VEC, seq, first, t0, c0, on, win);
+          pos = t0 - first;
+        }
+      }
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const R xs = rows(run, 0), ds = rows(run, 1);
+      T* out = dx + (int64_t)(t0 - HALO) * p.dx.s1;
+      // dpre of a token, and its part of dw where the token is the span's own
+      auto adjoint = [&](f32x2 xf, f32x2 df, bool own) {
+        const f32x2 pre = taps(win, xf, w), sig = sigmoid2(pre);
+        const f32x2 dp = f2mul(df, f2mul(sig, f2fma(pre, f2fma(sig, minus, one), one)));
+        if (own) {
+          #pragma unroll
+          for (int j = 0; j < HALO; ++j) dw[j] = f2fma(dp, win[j], dw[j]);
+          dw[HALO] = f2fma(dp, xf, dw[HALO]);
+        }
+        return dp;
+      };
+      if (k.inside() && pos >= HALO) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          const f32x2 xf = xs.get(i, lane);
+          const f32x2 dp = adjoint(xf, ds.get(i, lane), i < RUN - HALO || t0 + i < s1);
+          const f32x2 done = f2fma(w[0], dp, pend[2]);
+          if (on && (i >= HALO || t0 > s0)) put<T, VEC>(out, done);
+          out += p.dx.s1;
+          pend[2] = f2fma(w[1], dp, pend[1]);
+          pend[1] = f2fma(w[2], dp, pend[0]);
+          pend[0] = f2mul(w[3], dp);
+          slide(win, xf);
+        }
+        continue;
+      }
+      #pragma unroll 1
+      for (int i = 0; i < RUN && t0 + i < end; ++i) {
+        const int seq = __shfl_sync(0xffffffffu, k.seq, i);
+        const bool opens = (k.start >> i) & 1, closes = (k.last >> i) & 1, in = (k.valid >> i) & 1;
+        const f32x2 xf = xs.get(i, lane);
+        if (opens) {
+          pos = 0;
+          owned = t0 + i < s1;
+          window_before<T, VEC>(p, x + lane * VEC, seq, t0 + i, t0 + i, c0, on, win);
+          before[0] = before[1] = before[2] = zero;
+        }
+        const f32x2 dp = in ? adjoint(xf, ds.get(i, lane), t0 + i < s1) : zero;
+        f32x2 part[HALO + 1] = {zero, pend[0], pend[1], pend[2]};  // dx of this token and the three before it
+        auto give = [&](int j, f32x2 v) {  // to token s - j, or to what lies before the sequence
+          if (pos >= j) part[j] = f2add(part[j], v);
           #pragma unroll
           for (int s = 0; s < HALO; ++s)
-            store_f32<VEC>(p.cache_out + ((int64_t)n * HALO + s) * p.C + c0, win[s]);
-      }
-    }
-  }
-}
-
-// Adjoint.  A run's tokens are walked with the three behind it; token s adds
-// w[3-k] dpre_s to dx of token s - k, and to the cache's (or the first
-// token's) gradient where s - k lies before its sequence, which the run that
-// holds the sequence's first token collects.
-template <typename T, int VEC, bool PACKED>
-__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(ConvParams p) {
-  __shared__ float red[CONV_WARPS][32 * VEC][HALO + 2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chain = blockIdx.x;  // set of channels (all sequences of a dense batch are walked by one grid column)
-  const int c0 = (int)chain * 32 * VEC + lane * VEC;
-  const bool on = c0 < p.C;
-  if (PACKED && p.d_cache_in && blockIdx.y == 0) pass_empty<VEC>(p, p.d_cache_out, p.d_cache_in, c0, on, warp, lane);
-
-  float w[VEC][HALO + 1], dw[VEC][HALO + 1];
-  #pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    #pragma unroll
-    for (int j = 0; j <= HALO; ++j) {
-      w[v][j] = on ? __ldg(p.w + (int64_t)(c0 + v) * (HALO + 1) + j) : 0.f;
-      dw[v][j] = 0.f;
-    }
-
-  const int64_t all = PACKED ? p.runs : (int64_t)p.runs * p.B;
-  for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < all; unit += (int64_t)gridDim.y * CONV_WARPS) {
-    const int b = PACKED ? 0 : (int)(unit / p.runs);
-    const int t0 = (int)(PACKED ? unit : unit % p.runs) * CONV_RUN;
-    const T* x = static_cast<const T*>(p.x.p) + (PACKED ? 0 : (int64_t)b * p.x.s0) + c0;
-    const T* dy = static_cast<const T*>(p.y.p) + (PACKED ? 0 : (int64_t)b * p.y.s0) + c0;
-    T* dx = static_cast<T*>(const_cast<void*>(p.dx.p)) + (PACKED ? 0 : (int64_t)b * p.dx.s0) + c0;
-    constexpr int N = CONV_RUN + HALO;
-    typename Vec<T, VEC>::Raw xr[N], dr[N];
-    #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      xr[i] = dr[i] = typename Vec<T, VEC>::Raw{};
-      if (on && t0 + i < p.T) {
-        xr[i] = Vec<T, VEC>::load(x + (int64_t)(t0 + i) * p.x.s1);
-        dr[i] = Vec<T, VEC>::load(dy + (int64_t)(t0 + i) * p.y.s1);
-      }
-    }
-    const Place mine = place_of<PACKED>(p, b, lane < N ? t0 + lane : p.T);
-    const unsigned valid = __ballot_sync(0xffffffffu, mine.seq >= 0);
-    const unsigned start = __ballot_sync(0xffffffffu, mine.seq >= 0 && mine.first == t0 + lane);
-    const unsigned last = __ballot_sync(0xffffffffu, mine.seq >= 0 && mine.end == t0 + lane + 1);
-    float win[HALO][VEC] = {};
-    if (valid & 1) {
-      const Place q{__shfl_sync(0xffffffffu, mine.seq, 0), __shfl_sync(0xffffffffu, mine.first, 0), 0};
-      if (on) window_before<T, VEC>(p, x, q, t0, c0, win);
-    }
-    int pos = HALO;  // place of the token in its sequence, as far as the first three count
-    if (valid & 1) pos = t0 - __shfl_sync(0xffffffffu, mine.first, 0);
-    bool owned = false;  // the sequence began in this run
-    float pend[HALO + 1][VEC] = {};  // dx of tokens s, s - 1, s - 2, s - 3 as far as it is summed
-    float before[HALO][VEC] = {};    // gradient of the three values before the sequence
-    #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float xf[VEC], df[VEC];
-      Vec<T, VEC>::unpack(xr[i], xf);
-      Vec<T, VEC>::unpack(dr[i], df);
-      const bool opens = (start >> i) & 1, closes = (last >> i) & 1, in = (valid >> i) & 1;
-      if (opens) {
-        pos = 0;
-        owned = i < CONV_RUN;
-        if (i) {
-          const Place q{__shfl_sync(0xffffffffu, mine.seq, i), t0 + i, 0};
-          if (on) window_before<T, VEC>(p, x, q, t0 + i, c0, win);
-        }
-        #pragma unroll
-        for (int s = 0; s < HALO; ++s)
+            if (pos < j && pos - j + HALO == s) before[s] = f2add(before[s], v);
+        };
+        if (in) {
           #pragma unroll
-          for (int v = 0; v < VEC; ++v) before[s][v] = 0.f;
-      }
-      #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float pre = win[0][v] * w[v][0];
-        pre = fmaf(win[1][v], w[v][1], pre);
-        pre = fmaf(win[2][v], w[v][2], pre);
-        pre = fmaf(xf[v], w[v][3], pre);
-        const float sig = __fdividef(1.f, 1.f + __expf(-pre));
-        const float dp = in ? df[v] * (sig * fmaf(pre, 1.f - sig, 1.f)) : 0.f;
-        if (i < CONV_RUN && in) {
-          dw[v][0] = fmaf(dp, win[0][v], dw[v][0]);
-          dw[v][1] = fmaf(dp, win[1][v], dw[v][1]);
-          dw[v][2] = fmaf(dp, win[2][v], dw[v][2]);
-          dw[v][3] = fmaf(dp, xf[v], dw[v][3]);
-        }
-        win[0][v] = win[1][v];
-        win[1][v] = win[2][v];
-        win[2][v] = xf[v];
-        pend[3][v] = pend[2][v];
-        pend[2][v] = pend[1][v];
-        pend[1][v] = pend[0][v];
-        pend[0][v] = 0.f;
-        #pragma unroll
-        for (int k = 0; k <= HALO; ++k) {
-          const float add = w[v][HALO - k] * dp;
-          if (pos >= k) pend[k][v] += add;
-          else
+          for (int j = 0; j <= HALO; ++j) give(j, f2mul(w[HALO - j], dp));
+          if (closes && p.d_cache_out && on) {  // the new cache holds the last three values
             #pragma unroll
-            for (int s = 0; s < HALO; ++s)  // value s of the three before: pos - k = s - 3
-              if (pos - k + HALO == s) before[s][v] += add;
-        }
-      }
-      if (closes && p.d_cache_out) {  // the new cache holds the last three values
-        const int n = __shfl_sync(0xffffffffu, mine.seq, i);
-        if (on)
-          #pragma unroll
-          for (int k = 0; k < HALO; ++k) {
-            float d[VEC];
-            load_f32<VEC>(cache_row<VEC>(p.d_cache_out, n, HALO - 1 - k, p.C, c0), d);
-            #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              if (pos >= k) pend[k][v] += d[v];
-              else
+            for (int j = 0; j < HALO; ++j)
+              give(j, get_f32<VEC>(p.d_cache_out + cache_at(p, seq, HALO - 1 - j, c0)));
+          }
+          // no later token reaches before the sequence: hand on what does
+          if (owned && (pos == HALO - 1 || (closes && pos < HALO - 1))) {
+            if (p.d_cache_in) {
+              if (on)
                 #pragma unroll
-                for (int s = 0; s < HALO; ++s)
-                  if (pos - k + HALO == s) before[s][v] += d[v];
+                for (int s = 0; s < HALO; ++s) put_f32<VEC>(p.d_cache_in + cache_at(p, seq, s, c0), before[s]);
+            } else if (!p.cache_in) {  // copies of the first token
+              #pragma unroll
+              for (int j = 0; j < HALO; ++j)
+                if (pos == j) part[j] = f2add(part[j], f2add(before[0], f2add(before[1], before[2])));
             }
           }
-      }
-      // the sequence's first tokens are past (no later token reaches before it): hand on what lies before it
-      if (owned && in && (pos == HALO - 1 || (closes && pos < HALO - 1))) {
-        const int n = __shfl_sync(0xffffffffu, mine.seq, i);
-        if (p.d_cache_in) {
-          if (on)
-            #pragma unroll
-            for (int s = 0; s < HALO; ++s)
-              store_f32<VEC>(p.d_cache_in + ((int64_t)n * HALO + s) * p.C + c0, before[s]);
-        } else if (!p.cache_in) {  // copies of the first token
-          #pragma unroll
-          for (int v = 0; v < VEC; ++v)
-            #pragma unroll
-            for (int k = 0; k < HALO; ++k)
-              if (pos == k) pend[k][v] += before[0][v] + before[1][v] + before[2][v];
         }
+        const int row = t0 + i - HALO;
+        if (on && row >= s0 && row < s1) put<T, VEC>(out, part[HALO]);
+        out += p.dx.s1;
+        pend[0] = part[0];
+        pend[1] = part[1];
+        pend[2] = part[2];
+        slide(win, xf);
+        pos = pos < HALO ? pos + 1 : pos;
       }
-      if (i >= HALO && on && t0 + i - HALO < p.T) Vec<T, VEC>::store(dx + (int64_t)(t0 + i - HALO) * p.dx.s1, pend[HALO]);
-      pos = pos < HALO ? pos + 1 : pos;
     }
   }
   if (!p.part) return;
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);  // [warp][channel][tap]
   #pragma unroll
-  for (int v = 0; v < VEC; ++v)
+  for (int j = 0; j <= HALO; ++j) {
+    float d[2];
+    f2un(dw[j], d[0], d[1]);
     #pragma unroll
-    for (int j = 0; j <= HALO; ++j) red[warp][lane * VEC + v][j] = dw[v][j];
+    for (int v = 0; v < VEC; ++v) red[((warp * 32 + lane) * VEC + v) * (HALO + 1) + j] = d[v];
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < 32 * VEC * (HALO + 1); e += 32 * CONV_WARPS) {
-    const int c = e / (HALO + 1), j = e % (HALO + 1);
-    const int at = (int)chain * 32 * VEC + c;
-    if (at >= p.C) continue;
+    if (base + e / (HALO + 1) >= p.C) continue;
     float s = 0.f;
     #pragma unroll
-    for (int k = 0; k < CONV_WARPS; ++k) s += red[k][c][j];
-    p.part[((int64_t)blockIdx.y * p.C + at) * (HALO + 1) + j] = s;
+    for (int k = 0; k < CONV_WARPS; ++k) s += red[k * 32 * VEC * (HALO + 1) + e];
+    p.part[((int64_t)blockIdx.y * p.C + base) * (HALO + 1) + e] = s;
   }
 }
 
 // ---- host ----
-
-static bool conv_rows_ok(const gdn2_view& v, int vec, int elem) {
-  return (uintptr_t)v.data % (vec * elem) == 0 && v.stride0 % vec == 0 && v.stride1 % vec == 0;
-}
 
 static int check_conv(const gdn2_conv_args* a, const char* fn) {
   if (!a) return set_error(GDN2_EINVAL, "%s: null args", fn);
@@ -340,27 +374,67 @@ static int check_conv(const gdn2_conv_args* a, const char* fn) {
   return GDN2_OK;
 }
 
-static void fill_conv(ConvParams& p, const gdn2_conv_args* a, int vec) {
+// How a call is cut up: channels per lane, 16-byte copies, spans of tokens and blocks along them.
+struct ConvPlan {
+  int vec;
+  bool coop;
+  int sets, span, spans, blocks;
+};
+
+// Spans of `runs` runs less `less` tokens, down to one run until the warps fill the GPU.  `blocks_per_sm`: blocks
+// along the spans (each leaves a partial row of dw), 0 for all of them.
+static ConvPlan plan_conv(const gdn2_conv_args* a, bool pairs, bool coop, int less, int blocks_per_sm) {
+  ConvPlan n;
+  n.vec = pairs ? 2 : 1;
+  n.coop = pairs && coop;
+  n.sets = (a->channels + 32 * n.vec - 1) / (32 * n.vec);
+  const int rows = a->cu_seqlens ? 1 : a->batch;
+  int runs = 8;
+  for (;; runs /= 2) {
+    n.span = runs * RUN - less;
+    n.spans = (a->seq_len + n.span - 1) / n.span;
+    if (runs == 1 || (int64_t)n.spans * rows * n.sets >= 148 * 4 * CONV_WARPS) break;
+  }
+  const int64_t most = ((int64_t)n.spans * rows + CONV_WARPS - 1) / CONV_WARPS;
+  int64_t want = blocks_per_sm ? (148 * blocks_per_sm + n.sets - 1) / n.sets : most;
+  want = want < most ? want : most;
+  n.blocks = (int)(want < 1 ? 1 : want > 65535 ? 65535 : want);
+  return n;
+}
+
+static void fill_conv(ConvParams& p, const gdn2_conv_args* a, const ConvPlan& n) {
   p = ConvParams{};
   p.B = a->batch; p.T = a->seq_len; p.C = a->channels;
-  p.runs = (p.T + CONV_RUN - 1) / CONV_RUN;
-  p.sets = (p.C + 32 * vec - 1) / (32 * vec);
+  p.sets = n.sets; p.span = n.span; p.spans = n.spans;
   p.cu = a->cu_seqlens;
   p.x = make_dview(a->x);
   p.w = a->weight;
   p.cache_in = a->cache_in;
 }
 
-template <typename T, int VEC>
-static int run_conv_fwd(const ConvParams& p, cudaStream_t st, const char* fn) {
-  const int64_t chains = p.cu ? p.sets : (int64_t)p.B * p.sets;
-  if (chains > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: too many channels", fn);
-  int gy = (p.runs + CONV_WARPS - 1) / CONV_WARPS;
-  gy = gy < 1 ? 1 : gy > 65535 ? 65535 : gy;
-  const dim3 grid((unsigned)chains, gy);
-  if (p.cu) k_conv_fwd<T, VEC, true><<<grid, 32 * CONV_WARPS, 0, st>>>(p);
-  else k_conv_fwd<T, VEC, false><<<grid, 32 * CONV_WARPS, 0, st>>>(p);
+template <typename K>
+static int launch_conv(K kernel, const ConvParams& p, const ConvPlan& n, int stage, cudaStream_t st, const char* fn) {
+  const int smem = STAGES * CONV_WARPS * stage;
+  int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
+  if (rc) return rc;
+  kernel<<<dim3(n.sets, n.blocks), 32 * CONV_WARPS, smem, st>>>(p);
   return check_cuda(cudaGetLastError(), fn);
+}
+
+template <typename T, int VEC, bool COOP>
+static int run_conv(const ConvParams& p, const ConvPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  const int bytes = Rows<T, VEC, COOP>::BYTES;
+  if (bwd)
+    return p.cu ? launch_conv(k_conv_bwd<T, VEC, COOP, true>, p, n, 2 * bytes, st, fn)
+                : launch_conv(k_conv_bwd<T, VEC, COOP, false>, p, n, 2 * bytes, st, fn);
+  return p.cu ? launch_conv(k_conv_fwd<T, VEC, COOP, true>, p, n, bytes, st, fn)
+              : launch_conv(k_conv_fwd<T, VEC, COOP, false>, p, n, bytes, st, fn);
+}
+
+template <typename T>
+static int dispatch_conv(const ConvParams& p, const ConvPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  if (n.coop) return run_conv<T, 2, true>(p, n, bwd, st, fn);
+  return n.vec == 2 ? run_conv<T, 2, false>(p, n, bwd, st, fn) : run_conv<T, 1, false>(p, n, bwd, st, fn);
 }
 
 int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_out, cudaStream_t st) {
@@ -368,47 +442,28 @@ int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_ou
   int rc = check_conv(a, fn);
   if (rc) return rc;
   if (a->seq_len && !y.data) return set_error(GDN2_EINVAL, "%s: null tensor pointer", fn);
-  const int elem = a->dtype == GDN2_DTYPE_BF16 ? 2 : 4;
-  const bool pairs = a->channels % 2 == 0 && conv_rows_ok(a->x, 2, elem) && conv_rows_ok(y, 2, elem);
+  const int e = elem_bytes(a->dtype);
+  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * e, e) && rows_ok(y, 2 * e, e);
+  const ConvPlan n = plan_conv(a, pairs, a->channels * e % 16 == 0 && rows_ok(a->x, 16, e), 0, 0);
   ConvParams p;
-  fill_conv(p, a, pairs ? 2 : 1);
+  fill_conv(p, a, n);
   p.y = make_dview(y);
   p.cache_out = cache_out;
-  if (a->dtype == GDN2_DTYPE_F32)
-    return pairs ? run_conv_fwd<float, 2>(p, st, fn) : run_conv_fwd<float, 1>(p, st, fn);
-  return pairs ? run_conv_fwd<__nv_bfloat16, 2>(p, st, fn) : run_conv_fwd<__nv_bfloat16, 1>(p, st, fn);
+  return a->dtype == GDN2_DTYPE_F32 ? dispatch_conv<float>(p, n, false, st, fn)
+                                    : dispatch_conv<__nv_bfloat16>(p, n, false, st, fn);
 }
 
-// Blocks along the runs of a channel set in the adjoint: each leaves one partial row of dw.
-static int conv_bwd_blocks(const gdn2_conv_args* a, int sets) {
-  const int64_t runs = (int64_t)((a->seq_len + CONV_RUN - 1) / CONV_RUN) * (a->cu_seqlens ? 1 : a->batch);
-  const int64_t most = (runs + CONV_WARPS - 1) / CONV_WARPS;
-  int64_t want = (148 * 4 + sets - 1) / sets;
-  want = want < most ? want : most;
-  return (int)(want < 1 ? 1 : want);
+static ConvPlan plan_conv_bwd(const gdn2_conv_bwd_args* q) {
+  const gdn2_conv_args* a = &q->fwd;
+  const int e = elem_bytes(a->dtype);
+  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * e, e) && rows_ok(q->d_y, 2 * e, e) && rows_ok(q->dx, 2 * e, e);
+  const bool coop = a->channels * e % 16 == 0 && rows_ok(a->x, 16, e) && rows_ok(q->d_y, 16, e);
+  return plan_conv(a, pairs, coop, HALO, 5);
 }
-
-static bool conv_bwd_pairs(const gdn2_conv_bwd_args* q) {
-  const int elem = q->fwd.dtype == GDN2_DTYPE_BF16 ? 2 : 4;
-  return q->fwd.channels % 2 == 0 && conv_rows_ok(q->fwd.x, 2, elem) && conv_rows_ok(q->d_y, 2, elem) &&
-         conv_rows_ok(q->dx, 2, elem);
-}
-
-static int conv_sets(int C, bool pairs) { return pairs ? (C + 63) / 64 : (C + 31) / 32; }
 
 size_t conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* q) {
-  if (!q || check_conv(&q->fwd, "gdn2_causal_conv_bwd_workspace_bytes")) return 0;
-  if (!q->d_weight) return 0;
-  const int sets = conv_sets(q->fwd.channels, conv_bwd_pairs(q));
-  return (size_t)conv_bwd_blocks(&q->fwd, sets) * q->fwd.channels * (HALO + 1) * sizeof(float);
-}
-
-template <typename T, int VEC>
-static int run_conv_bwd(const ConvParams& p, int gy, cudaStream_t st, const char* fn) {
-  const dim3 grid((unsigned)p.sets, gy);
-  if (p.cu) k_conv_bwd<T, VEC, true><<<grid, 32 * CONV_WARPS, 0, st>>>(p);
-  else k_conv_bwd<T, VEC, false><<<grid, 32 * CONV_WARPS, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), fn);
+  if (!q || check_conv(&q->fwd, "gdn2_causal_conv_bwd_workspace_bytes") || !q->d_weight) return 0;
+  return (size_t)plan_conv_bwd(q).blocks * q->fwd.channels * (HALO + 1) * sizeof(float);
 }
 
 int launch_column_sums(const float* part, int64_t rows, int cols, int arrays, float* out0, float* out1,
@@ -427,21 +482,18 @@ int launch_conv_bwd(const gdn2_conv_bwd_args* q, void* ws, size_t ws_bytes, cuda
   const size_t need = conv_bwd_workspace_bytes(q);
   if (need && (!ws || ws_bytes < need))
     return set_error(GDN2_EWORKSPACE, "%s: workspace %zu bytes < required %zu", fn, ws ? ws_bytes : 0, need);
-  const bool pairs = conv_bwd_pairs(q);
+  const ConvPlan n = plan_conv_bwd(q);
   ConvParams p;
-  fill_conv(p, a, pairs ? 2 : 1);
+  fill_conv(p, a, n);
   p.y = make_dview(q->d_y);
   p.dx = make_dview(q->dx);
   p.d_cache_out = q->d_cache_out;
   p.d_cache_in = q->d_cache_in;
   p.part = need ? static_cast<float*>(ws) : nullptr;
-  const int gy = conv_bwd_blocks(a, p.sets);
-  if (a->dtype == GDN2_DTYPE_F32)
-    rc = pairs ? run_conv_bwd<float, 2>(p, gy, st, fn) : run_conv_bwd<float, 1>(p, gy, st, fn);
-  else
-    rc = pairs ? run_conv_bwd<__nv_bfloat16, 2>(p, gy, st, fn) : run_conv_bwd<__nv_bfloat16, 1>(p, gy, st, fn);
+  rc = a->dtype == GDN2_DTYPE_F32 ? dispatch_conv<float>(p, n, true, st, fn)
+                                  : dispatch_conv<__nv_bfloat16>(p, n, true, st, fn);
   if (rc || !need) return rc;
-  return launch_column_sums(p.part, gy, p.C * (HALO + 1), 1, q->d_weight, nullptr, st, fn);
+  return launch_column_sums(p.part, n.blocks, p.C * (HALO + 1), 1, q->d_weight, nullptr, st, fn);
 }
 
 }  // namespace gdn2

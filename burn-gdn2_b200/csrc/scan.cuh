@@ -1,6 +1,6 @@
-// Pieces shared by the sequence operators (gated scan, short conv, group
-// norm): vector access to rows of channels, packed-sequence lookup and the
-// decay's exponential.
+// Pieces shared by the sequence operators (gated scan, causal convolution,
+// group norm): vector access to rows of channels, staged rows, packed-sequence
+// lookup and the decay's exponential.
 #pragma once
 
 #include "common.cuh"
@@ -97,5 +97,85 @@ __device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& k) {
   if constexpr (WITH_K) k = f2fma(f2mul(s, kMinus), p, f2fma(s, kMinus, kOne));
 }
 constexpr float kExpRange = 87.f;
+
+constexpr int RUN = 16;     // tokens of a warp's run
+constexpr int STAGES = 2;   // runs in flight or in use
+
+// One warp's staged rows, [RUN][32 * VEC] of T.  Copied 16 bytes a lane over
+// several rows where rows allow it (COOP: few instructions; lanes read what
+// others copied), else each lane its own values.
+template <typename T, int VEC, bool COOP>
+struct Rows {
+  static constexpr int ROW = 32 * VEC * (int)sizeof(T), BYTES = RUN * ROW;
+  unsigned char* base;
+  // rows t0 .. of p (its lane 0 channel), those below T, channels below `left`
+  __device__ __forceinline__ void fetch(const T* p, int64_t stride, int t0, int T_, int left, int lane) const {
+    if constexpr (COOP) {
+      constexpr int LANES = ROW / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
+      const int c = lane % LANES * (16 / (int)sizeof(T)), r = lane / LANES;
+      const T* q = p + (int64_t)(t0 + r) * stride + c;
+      #pragma unroll
+      for (int i = 0; i < RUN; i += AT_ONCE) {
+        const bool in = c < left && t0 + r + i < T_;
+        cp_async_zfill<16>(base + (i + r) * ROW + lane % LANES * 16, in ? q : p, in);
+        q += AT_ONCE * stride;
+      }
+    } else {
+      typedef typename Vec<T, VEC>::Raw Raw;
+      const T* q = p + (int64_t)t0 * stride + lane * VEC;
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        const bool in = lane * VEC < left && t0 + i < T_;
+        Raw* to = reinterpret_cast<Raw*>(base + i * ROW) + lane;
+        if constexpr (sizeof(Raw) >= 4) cp_async_zfill<(int)sizeof(Raw)>(to, in ? q : p, in);
+        else *to = in ? Vec<T, VEC>::load(q) : Raw{};
+        q += stride;
+      }
+    }
+  }
+  // a lane's channels of row i as a pair (the second zero for VEC = 1)
+  __device__ __forceinline__ f32x2 get(int i, int lane) const {
+    float f[2] = {0.f, 0.f};
+    const T* p = reinterpret_cast<const T*>(base + i * ROW) + lane * VEC;
+    if constexpr (VEC == 2) Vec<T, 2>::unpack(*reinterpret_cast<const typename Vec<T, 2>::Raw*>(p), f);
+    else f[0] = to_f32<T>(*p);
+    return f2pk(f[0], f[1]);
+  }
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* p, f32x2 v) {
+  float f[2];
+  f2un(v, f[0], f[1]);
+  if constexpr (VEC == 2) Vec<T, 2>::store(p, f);
+  else {
+    float one[1] = {f[0]};
+    Vec<T, 1>::store(p, one);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ f32x2 get_f32(const float* p) {
+  return f2pk(p[0], VEC == 2 ? p[VEC - 1] : 0.f);
+}
+template <int VEC>
+__device__ __forceinline__ void put_f32(float* p, f32x2 v) {
+  float f0, f1;
+  f2un(v, f0, f1);
+  p[0] = f0;
+  if (VEC == 2) p[VEC - 1] = f1;
+}
+
+// Whether packed sequence n has no row.  Offsets beyond the T rows count as T.
+__device__ __forceinline__ bool is_empty(const int* __restrict__ cu, int n, int T) {
+  const int from = __ldg(cu + n);
+  return __ldg(cu + n + 1) <= from || from >= T;
+}
+
+// Rows of v start on `bytes` boundaries.
+inline bool rows_ok(const gdn2_view& v, int bytes, int elem) {
+  return (uintptr_t)v.data % bytes == 0 && v.stride0 * elem % bytes == 0 && v.stride1 * elem % bytes == 0;
+}
+
+inline int elem_bytes(int dtype) { return dtype == GDN2_DTYPE_BF16 ? 2 : 4; }
 
 }  // namespace gdn2
