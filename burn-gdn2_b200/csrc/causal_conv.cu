@@ -124,13 +124,6 @@ __device__ __forceinline__ void slide(f32x2 (&win)[HALO], f32x2 x) {
   win[1] = win[2];
   win[2] = x;
 }
-// sigmoid of a pair
-__device__ __forceinline__ f32x2 sigmoid2(f32x2 t) {
-  float t0, t1;
-  f2un(t, t0, t1);
-  return f2pk(__fdividef(1.f, 1.f + __expf(-t0)), __fdividef(1.f, 1.f + __expf(-t1)));
-}
-
 template <int VEC>
 __device__ __forceinline__ void load_taps(const ConvParams& p, int c0, bool on, f32x2 (&w)[HALO + 1]) {
   #pragma unroll

@@ -43,6 +43,37 @@ struct Vec {
   }
 };
 
+// A vector as pairs of f32 (one pair with a zero for VEC = 1).
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack_pairs(typename Vec<T, VEC>::Raw r, f32x2 (&f)[VEC == 1 ? 1 : VEC / 2]) {
+  float v[VEC == 1 ? 2 : VEC];
+  v[VEC == 1 ? 1 : 0] = 0.f;
+  Vec<T, VEC>::unpack(r, *reinterpret_cast<float (*)[VEC]>(v));
+  #pragma unroll
+  for (int i = 0; i < (VEC == 1 ? 1 : VEC / 2); ++i) f[i] = f2pk(v[2 * i], v[2 * i + 1]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pairs(T* p, const f32x2 (&f)[VEC == 1 ? 1 : VEC / 2]) {
+  float v[VEC == 1 ? 2 : VEC];
+  #pragma unroll
+  for (int i = 0; i < (VEC == 1 ? 1 : VEC / 2); ++i) f2un(f[i], v[2 * i], v[2 * i + 1]);
+  Vec<T, VEC>::store(p, *reinterpret_cast<const float (*)[VEC]>(v));
+}
+
+// Sigmoid of a pair: 1 / (1 + 2^(-t log2 e)) by the approximate exponential
+// and reciprocal (2 ulp and 1 ulp), far below the rounding of a bf16 result
+// and near f32's own.
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 t) {
+  float e0, e1;
+  f2un(f2mul(t, f2pk(-1.44269504088896f, -1.44269504088896f)), e0, e1);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  f2un(f2add(f2pk(e0, e1), f2pk(1.f, 1.f)), e0, e1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  return f2pk(e0, e1);
+}
+
 template <int VEC>
 __device__ __forceinline__ void load_f32(const float* p, float (&f)[VEC]) {
   #pragma unroll
