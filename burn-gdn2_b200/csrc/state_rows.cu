@@ -4,25 +4,53 @@
 // row (zeros), a row's own number leaves it alone.
 //
 // Bound by HBM: every moved row is read and written once, no other row is
-// touched.  A block owns a span of byte columns across all rows.  It packs
-// the list of moved rows, reads that span of every source into shared memory
-// and writes it only after the last of them has been read, so no row has to
-// be staged elsewhere and no order of moves can go wrong.  The span is
+// touched.  Each block packs the list of moved rows.  Where no move's source
+// is overwritten by another one (a compaction, a fork, rows gathered into
+// another pool) the blocks copy pieces of rows in no particular order.
+// Otherwise a block owns a span of byte columns across all rows, reads that
+// span of every source into shared memory and writes it only after the last
+// of them has been read, so no order of moves can go wrong; the span is
 // narrowed until all moved rows fit.
 #include "scan.cuh"
 
 namespace gdn2 {
 
-constexpr int ROWS_THREADS = 256, ROWS_BLOCKS = 2;  // threads, blocks per SM
-constexpr int ROWS_SMEM = 96 * 1024;                // list of moved rows, then the staged spans
-constexpr int MAX_POOL = 16;                        // tensors a launch takes
+constexpr int ROWS_THREADS = 256;
+constexpr int ROWS_SMEM_MIN = 16 * 1024, ROWS_SMEM_MAX = 96 * 1024;  // list of moved rows, then the staged spans
+constexpr int MAX_POOL = 16;                                         // tensors a launch takes
+constexpr int PIECE_WORDS = 4;                                       // words of a piece per thread
 
 struct RowsParams {
-  int count, src_rows, dst_rows;
+  int count, src_rows, dst_rows, smem;
   bool inplace;
   const int* index;
-  struct { const unsigned char* src; unsigned char* dst; int64_t bytes; int width; } t[MAX_POOL];
+  int64_t pieces;  // of one row, over all tensors
+  struct {
+    const unsigned char* src;
+    unsigned char* dst;
+    int64_t bytes, first_piece;
+    int width;
+  } t[MAX_POOL];
 };
+
+// Piece `at` of a row: PIECE_WORDS words a thread.
+template <typename W>
+__device__ __forceinline__ void copy_piece(const unsigned char* src, unsigned char* dst, int64_t bytes, int64_t at, int2 move) {
+  const int64_t words = bytes / (int64_t)sizeof(W), w0 = at * (ROWS_THREADS * PIECE_WORDS) + threadIdx.x;
+  const W* from = reinterpret_cast<const W*>(src + (int64_t)(move.y < 0 ? 0 : move.y) * bytes);
+  W* to = reinterpret_cast<W*>(dst + (int64_t)move.x * bytes);
+  W v[PIECE_WORDS];
+  #pragma unroll
+  for (int i = 0; i < PIECE_WORDS; ++i) {
+    const int64_t w = w0 + i * ROWS_THREADS;
+    v[i] = move.y >= 0 && w < words ? __ldcs(from + w) : W{};
+  }
+  #pragma unroll
+  for (int i = 0; i < PIECE_WORDS; ++i) {
+    const int64_t w = w0 + i * ROWS_THREADS;
+    if (w < words) __stcs(to + w, v[i]);
+  }
+}
 
 template <typename W>
 __device__ __forceinline__ void move_spans(const unsigned char* src, unsigned char* dst, int64_t bytes,
@@ -55,7 +83,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) k_state_rows(RowsParams p) {
   int2* moves = reinterpret_cast<int2*>(smem);  // (row, source)
   __shared__ int counts[ROWS_THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int n = 0;
+  int n = 0, entangled = 0;
   for (int d0 = 0; d0 < p.dst_rows; d0 += ROWS_THREADS) {
     const int d = d0 + threadIdx.x;
     int s = 0;
@@ -66,6 +94,10 @@ __global__ void __launch_bounds__(ROWS_THREADS) k_state_rows(RowsParams p) {
       if (bad && blockIdx.x == 0) atomicOr(&g_device_errors, DEVERR_STATE_INDEX);
       moved = !p.inplace || (!bad && s != d);
       if (bad) s = -1;
+      if (p.inplace && moved && s >= 0) {
+        const int over = __ldg(p.index + s);  // is the source a moved row too?
+        entangled |= over != s && over >= -1 && over < p.src_rows;
+      }
     }
     const unsigned m = __ballot_sync(0xffffffffu, moved);
     if (lane == 0) counts[warp] = __popc(m);
@@ -80,15 +112,26 @@ __global__ void __launch_bounds__(ROWS_THREADS) k_state_rows(RowsParams p) {
     __syncthreads();
   }
   if (!n) return;
+  if (!__syncthreads_or(entangled)) {
+    for (int64_t unit = blockIdx.x; unit < n * p.pieces; unit += gridDim.x) {
+      const int64_t piece = unit % p.pieces;
+      int k = 0;
+      while (k + 1 < p.count && piece >= p.t[k + 1].first_piece) ++k;
+      const int64_t at = piece - p.t[k].first_piece;
+      const int2 move = moves[unit / p.pieces];
+      if (p.t[k].width == 16) copy_piece<uint4>(p.t[k].src, p.t[k].dst, p.t[k].bytes, at, move);
+      else if (p.t[k].width == 4) copy_piece<unsigned>(p.t[k].src, p.t[k].dst, p.t[k].bytes, at, move);
+      else copy_piece<unsigned char>(p.t[k].src, p.t[k].dst, p.t[k].bytes, at, move);
+    }
+    return;
+  }
   const int list = (n * (int)sizeof(int2) + 15) / 16 * 16;
   unsigned char* stage = smem + list;
+  const int room = p.smem - list;
   for (int k = 0; k < p.count; ++k) {
-    if (p.t[k].width == 16)
-      move_spans<uint4>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, ROWS_SMEM - list);
-    else if (p.t[k].width == 4)
-      move_spans<unsigned>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, ROWS_SMEM - list);
-    else
-      move_spans<unsigned char>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, ROWS_SMEM - list);
+    if (p.t[k].width == 16) move_spans<uint4>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, room);
+    else if (p.t[k].width == 4) move_spans<unsigned>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, room);
+    else move_spans<unsigned char>(p.t[k].src, p.t[k].dst, p.t[k].bytes, moves, n, stage, room);
   }
 }
 
@@ -101,7 +144,7 @@ int launch_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* in
     return set_error(GDN2_EINVAL, "%s: negative size (count=%d src_rows=%d dst_rows=%d)", fn, count, src_rows, dst_rows);
   if (!count || !dst_rows) return GDN2_OK;
   if (!t || !index) return set_error(GDN2_EINVAL, "%s: null pointer", fn);
-  static_assert(GDN2_MAX_STATE_ROWS * (16 + sizeof(int2)) <= ROWS_SMEM, "a word of every row and the list of moves");
+  static_assert(GDN2_MAX_STATE_ROWS * (16 + sizeof(int2)) <= ROWS_SMEM_MAX, "a word of every row and the list of moves");
   if (dst_rows > GDN2_MAX_STATE_ROWS)
     return set_error(GDN2_EUNSUPPORTED, "%s: %d rows, at most %d", fn, dst_rows, GDN2_MAX_STATE_ROWS);
   bool inplace = false;
@@ -118,25 +161,30 @@ int launch_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* in
   }
   if (inplace && src_rows != dst_rows)
     return set_error(GDN2_EINVAL, "%s: in place with %d and %d rows", fn, src_rows, dst_rows);
-  int rc = check_cuda(cudaFuncSetAttribute(k_state_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM), fn);
+  // room for 256 bytes of every row, so that the spans stay wide without crowding out a second and third block
+  const int want = dst_rows * (int)(sizeof(int2) + 256) + 16;
+  const int smem = want < ROWS_SMEM_MIN ? ROWS_SMEM_MIN : want > ROWS_SMEM_MAX ? ROWS_SMEM_MAX : want / 16 * 16;
+  int rc = check_cuda(cudaFuncSetAttribute(k_state_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
   for (int first = 0; !rc && first < count; first += MAX_POOL) {
     RowsParams p;
     p.count = count - first < MAX_POOL ? count - first : MAX_POOL;
     p.src_rows = src_rows; p.dst_rows = dst_rows;
+    p.smem = smem;
     p.inplace = inplace;
     p.index = index;
-    int64_t widest = 0;
+    p.pieces = 0;
     for (int k = 0; k < p.count; ++k) {
       const gdn2_state_rows& e = t[first + k];
       const uintptr_t all = (uintptr_t)e.src | (uintptr_t)e.dst | (uintptr_t)e.row_bytes;
-      p.t[k] = {static_cast<const unsigned char*>(e.src), static_cast<unsigned char*>(e.dst), e.row_bytes,
-                all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1};
-      const int64_t spans = e.row_bytes / p.t[k].width;
-      widest = spans > widest ? spans : widest;
+      const int width = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+      p.t[k] = {static_cast<const unsigned char*>(e.src), static_cast<unsigned char*>(e.dst), e.row_bytes, p.pieces, width};
+      const int64_t piece = (int64_t)width * ROWS_THREADS * PIECE_WORDS;
+      p.pieces += (e.row_bytes + piece - 1) / piece;
     }
-    const int64_t want = (widest + 3) / 4;  // a block has at least a few words of every row to do
-    const int blocks = (int)(want < 148 * ROWS_BLOCKS ? want : 148 * ROWS_BLOCKS);
-    k_state_rows<<<blocks, ROWS_THREADS, ROWS_SMEM, st>>>(p);
+    // every SM filled, or a piece of every row at most
+    const int64_t most = p.pieces * dst_rows, resident = 148 * (int64_t)(200 * 1024 / smem < 8 ? 200 * 1024 / smem : 8);
+    const int blocks = (int)(most < resident ? most : resident);
+    k_state_rows<<<blocks, ROWS_THREADS, smem, st>>>(p);
     rc = check_cuda(cudaGetLastError(), fn);
   }
   return rc;
