@@ -39,7 +39,7 @@ def _on(device: torch.device):
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream() builds an object: 2 us a call
 
 
 def _same_device(what: str, device: torch.device, *tensors):
@@ -95,8 +95,12 @@ def _f32(what: str, name: str, t: Optional[torch.Tensor], shape) -> Optional[tor
     return t.contiguous()
 
 
-def _workspace(size: int, device: torch.device):
-    return (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+def _workspace(size: int, near: torch.Tensor):
+    return (near.new_empty(size, dtype=torch.uint8) if size else None), size
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -113,11 +117,12 @@ def _scan_args(x, g, state, cu, complement, carry):
 
 def _scan_forward(x, g, state, cu, complement, state_out, keep):
     B, T, C = x.shape
-    h = torch.empty((B, T, C), dtype=x.dtype, device=x.device)
-    carry = torch.empty((B, -(-T // SCAN_CARRY), C), dtype=torch.float32, device=x.device) if keep else None
+    h = _like(x)
+    carry = x.new_empty((B, -(-T // SCAN_CARRY), C), dtype=torch.float32) if keep else None
     a, out = _scan_args(x, g, state, cu, complement, carry), _view3(h)
     with _on(x.device):
-        ws, size = _workspace(LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(a), out), x.device)
+        # up to 64 tokens are one block's and never cut into segments
+        ws, size = _workspace(LIB.gdn2_gated_scan_workspace_bytes(ctypes.byref(a), out) if T > 64 else 0, x)
         check(LIB.gdn2_gated_scan(ctypes.byref(a), out, _ptr(state_out), _ptr(ws), size, _stream(x.device)))
     return h, carry
 
@@ -126,7 +131,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, g, state, cu, complement):
         n = x.shape[0] if cu is None else cu.numel() - 1
-        last = torch.empty((n, x.shape[2]), dtype=torch.float32, device=x.device)
+        last = x.new_empty((n, x.shape[2]), dtype=torch.float32)
         h, carry = _scan_forward(x, g, state, cu, complement, last, True)
         ctx.save_for_backward(x, g, state, cu, carry)
         ctx.complement = complement
@@ -139,13 +144,12 @@ class _GatedScan(torch.autograd.Function):
         x, g, state, cu, carry = ctx.saved_tensors
         d_h = torch.zeros_like(x) if d_h is None else _rows(d_h)
         d_last = None if d_last is None else d_last.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dg = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        dx, dg = _like(x), _like(g)
         d_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[2] else None
         a = _lib.ScanBwdArgs(_scan_args(x, g, state, cu, ctx.complement, carry), _view3(d_h), _ptr(d_last),
                              _view3(dx), _view3(dg), _ptr(d_state))
         with _on(x.device):
-            ws, size = _workspace(LIB.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(a)), x.device)
+            ws, size = _workspace(LIB.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(a)), x)
             check(LIB.gdn2_gated_scan_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
         return dx, dg, d_state, None, None
 
@@ -190,7 +194,7 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
         return x + g.to(x.dtype), last if inplace else last.clone()
     if grads:
         return _GatedScan.apply(x, g, state, cu, bool(complement))
-    last = state if inplace else torch.empty((n, C), dtype=torch.float32, device=x.device)
+    last = state if inplace else x.new_empty((n, C), dtype=torch.float32)
     h, _ = _scan_forward(x, g, state, cu, complement, last, False)
     return h, last
 
@@ -205,8 +209,8 @@ def _conv_args(x, weight, cache, cu):
 
 def _conv_forward(x, weight, cache, cu):
     n = x.shape[0] if cu is None else cu.numel() - 1
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    new = torch.empty((n, SHORT_CONV_CACHE, x.shape[2]), dtype=torch.float32, device=x.device)
+    y = _like(x)
+    new = x.new_empty((n, SHORT_CONV_CACHE, x.shape[2]), dtype=torch.float32)
     a = _conv_args(x, weight, cache, cu)
     with _on(x.device):
         check(LIB.gdn2_causal_conv(ctypes.byref(a), _view3(y), new.data_ptr(), _stream(x.device)))
@@ -226,13 +230,13 @@ class _CausalConv(torch.autograd.Function):
         x, weight, cache, cu = ctx.saved_tensors
         d_y = torch.zeros_like(x) if d_y is None else _rows(d_y)
         d_new = None if d_new is None else d_new.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _like(x)
         d_weight = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         d_cache = torch.empty_like(cache) if cache is not None and ctx.needs_input_grad[2] else None
         a = _lib.ConvBwdArgs(_conv_args(x, weight, cache, cu), _view3(d_y), _ptr(d_new), _view3(dx), _ptr(d_weight),
                              _ptr(d_cache))
         with _on(x.device):
-            ws, size = _workspace(LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(a)), x.device)
+            ws, size = _workspace(LIB.gdn2_causal_conv_bwd_workspace_bytes(ctypes.byref(a)), x)
             check(LIB.gdn2_causal_conv_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
         return dx, d_weight, d_cache, None
 
@@ -277,8 +281,15 @@ def _norm_args(x, gate, weight, bias, groups, eps, center):
                               x.stride(0), _ptr(gate), 0 if gate is None else gate.stride(0), _ptr(weight), _ptr(bias))
 
 
+def _norm_rows(t: Optional[torch.Tensor], chan: int) -> Optional[torch.Tensor]:
+    """[..., C] as rows; a copy where the rows are not evenly spaced or their channels not contiguous."""
+    if t is None:
+        return None
+    return _rows(t if t.dim() == 2 else t.reshape(-1, chan))
+
+
 def _norm_forward(x, gate, weight, bias, groups, eps, center):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _like(x)
     if x.shape[0]:
         a = _norm_args(x, gate, weight, bias, groups, eps, center)
         with _on(x.device):
@@ -289,24 +300,30 @@ def _norm_forward(x, gate, weight, bias, groups, eps, center):
 class _GroupNormGate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, weight, bias, groups, eps, center):
-        ctx.save_for_backward(x, gate, weight, bias)
+        rows, gate_rows = _norm_rows(x, x.shape[-1]), _norm_rows(gate, x.shape[-1])
+        ctx.save_for_backward(rows, gate_rows, weight, bias)
         ctx.rest = (groups, eps, center)
-        return _norm_forward(x, gate, weight, bias, groups, eps, center)
+        ctx.shape = x.shape
+        y = _norm_forward(rows, gate_rows, weight, bias, groups, eps, center)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_y):
         x, gate, weight, bias = ctx.saved_tensors
-        d_y = _rows(d_y)
-        new = lambda k, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if ctx.needs_input_grad[k] else None
-        dx, d_gate, d_weight, d_bias = (new(k, t) for k, t in enumerate((x, gate, weight, bias)))
-        if not x.shape[0]:
-            return (dx, d_gate, *(None if t is None else t.zero_() for t in (d_weight, d_bias)), None, None, None)
-        a = _lib.GroupNormBwdArgs(_norm_args(x, gate, weight, bias, *ctx.rest), d_y.data_ptr(), d_y.stride(0),
-                                  _ptr(dx), _ptr(d_gate), _ptr(d_weight), _ptr(d_bias))
-        with _on(x.device):
-            ws, size = _workspace(LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(a)), x.device)
-            check(LIB.gdn2_group_norm_gate_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
+        d_y = _norm_rows(d_y, x.shape[1])
+        need = ctx.needs_input_grad
+        dx, d_gate, d_weight, d_bias = (_like(t) if need[k] else None for k, t in enumerate((x, gate, weight, bias)))
+        if x.shape[0]:
+            a = _lib.GroupNormBwdArgs(_norm_args(x, gate, weight, bias, *ctx.rest), d_y.data_ptr(), d_y.stride(0),
+                                      _ptr(dx), _ptr(d_gate), _ptr(d_weight), _ptr(d_bias))
+            with _on(x.device):
+                ws, size = _workspace(LIB.gdn2_group_norm_gate_bwd_workspace_bytes(ctypes.byref(a)), x)
+                check(LIB.gdn2_group_norm_gate_bwd(ctypes.byref(a), _ptr(ws), size, _stream(x.device)))
+        else:
+            d_weight, d_bias = (None if t is None else t.zero_() for t in (d_weight, d_bias))
+        if len(ctx.shape) != 2:
+            dx, d_gate = (None if t is None else t.view(ctx.shape) for t in (dx, d_gate))
         return dx, d_gate, d_weight, d_bias, None, None, None
 
 
@@ -342,11 +359,11 @@ def group_norm_gate(x, gate=None, weight=None, bias=None, *, num_groups: int, ep
         raise ValueError(f"{what}: a bias goes with a weight of its shape")
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    flat = lambda t: None if t is None else _rows(t.reshape(-1, chan))
-    args = (flat(x), flat(gate), weight, bias, int(num_groups), float(eps), bool(center))
+    rest = (weight, bias, int(num_groups), float(eps), bool(center))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias)):
-        return _GroupNormGate.apply(*args).reshape(shape)
-    return _norm_forward(*args).reshape(shape)
+        return _GroupNormGate.apply(x, gate, *rest)
+    y = _norm_forward(_norm_rows(x, chan), _norm_rows(gate, chan), *rest)
+    return y if x.dim() == 2 else y.view(shape)
 
 
 # -- state pools ---------------------------------------------------------------
@@ -374,17 +391,18 @@ def _pool_like(states, new):
 
 def _checked_pool(what: str, states):
     tensors = _pool_tensors(what, states)
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} runs on the B200 CUDA kernels only; got a CPU tensor")
-        if t.dim() < 1 or t.shape[0] != tensors[0].shape[0]:
-            raise ValueError(f"{what}: every tensor of a pool has its rows first and as many, got {[list(t.shape) for t in tensors]}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: the tensors of a pool must be contiguous")
-        if t.requires_grad:
-            raise ValueError(f"{what}: the rows of a pool move without gradients; detach its tensors")
-        _same_device(what, tensors[0].device, t)
-    if tensors and tensors[0].shape[0] > _lib.GDN2_MAX_STATE_ROWS:
+    if not tensors:
+        return tensors
+    if not all(t.is_cuda for t in tensors):
+        raise RuntimeError(f"{what} runs on the B200 CUDA kernels only; got a CPU tensor")
+    if not all(t.dim() for t in tensors) or len({t.shape[0] for t in tensors}) > 1:
+        raise ValueError(f"{what}: every tensor of a pool has its rows first and as many, got {[list(t.shape) for t in tensors]}")
+    if not all(t.is_contiguous() for t in tensors):
+        raise ValueError(f"{what}: the tensors of a pool must be contiguous")
+    if any(t.requires_grad for t in tensors):
+        raise ValueError(f"{what}: the rows of a pool move without gradients; detach its tensors")
+    _same_device(what, tensors[0].device, *tensors)
+    if tensors[0].shape[0] > _lib.GDN2_MAX_STATE_ROWS:
         raise ValueError(f"{what}: {tensors[0].shape[0]} rows, at most {_lib.GDN2_MAX_STATE_ROWS}")
     return tensors
 
@@ -407,15 +425,13 @@ def _pool_index(what: str, index, rows: int, device) -> torch.Tensor:
     return index.contiguous()
 
 
-def _move_rows(pairs, index, src_rows):
-    pairs = [(s, d) for s, d in pairs if s.numel() or d.numel()]
-    if not pairs or not index.numel():
-        return
-    device = index.device
-    rows = (_lib.StateRows * len(pairs))(*((s.data_ptr(), d.data_ptr(), d.numel() // d.shape[0] * d.element_size())
-                                           for s, d in pairs))
-    with _on(device):
-        check(LIB.gdn2_move_state_rows(rows, len(pairs), index.data_ptr(), src_rows, index.shape[0], _stream(device)))
+def _move_rows(sources, targets, index, src_rows):
+    device, n = index.device, index.shape[0]
+    rows = [(s.data_ptr(), t.data_ptr(), t.nbytes // n) for s, t in zip(sources, targets) if t.nbytes]
+    if rows:
+        with _on(device):
+            check(LIB.gdn2_move_state_rows((_lib.StateRows * len(rows))(*rows), len(rows), index.data_ptr(), src_rows, n,
+                                           _stream(device)))
 
 
 def reorder_states(states, index) -> None:
@@ -437,13 +453,13 @@ def reorder_states(states, index) -> None:
     if not tensors:
         return
     rows = tensors[0].shape[0]
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+    spans = sorted([(t.data_ptr(), t.nbytes) for t in tensors])
+    if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
         raise ValueError(f"{what}: a tensor (or a part of one) comes twice")
     index = _pool_index(what, index, rows, tensors[0].device)
     if index.shape[0] != rows:
         raise ValueError(f"{what}: {index.shape[0]} row numbers for {rows} rows")
-    _move_rows([(t, t) for t in tensors], index, rows)
+    _move_rows(tensors, tensors, index, rows)
 
 
 def select_states(states, index):
@@ -457,6 +473,6 @@ def select_states(states, index):
         return _pool_like(states, iter(()))
     rows = tensors[0].shape[0]
     index = _pool_index(what, index, rows, tensors[0].device)
-    new = [torch.empty((index.shape[0], *t.shape[1:]), dtype=t.dtype, device=t.device) for t in tensors]
-    _move_rows([(t, n) for t, n in zip(tensors, new)], index, rows)
+    new = [t.new_empty((index.shape[0], *t.shape[1:])) for t in tensors]
+    _move_rows(tensors, new, index, rows)
     return _pool_like(states, iter(new))

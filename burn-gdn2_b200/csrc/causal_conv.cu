@@ -6,7 +6,7 @@
 //
 // The three tokens before a sequence are its cache, or copies of its first
 // token (src/short_conv.rs:42-54).  Bound by HBM: x in and y out, or x and dy
-// in and dx out.  A warp walks a span of tokens of 32 * VEC channels in runs
+// in and dx out.  A warp walks a span of tokens of 64 channels in runs
 // that are copied to shared memory a run ahead; the three values before a
 // token stay in registers, so a span reads nothing twice but the three rows
 // in front of it.  In the adjoint the dx of the last three tokens stay in
@@ -16,7 +16,7 @@
 // ends sort out caches and copies token by token.  Each lane sums dw over its
 // spans, the block adds its warps' sums and a second kernel the blocks', in a
 // fixed order.
-#include "scan.cuh"
+#include "sequence.cuh"
 
 namespace gdn2 {
 
@@ -25,7 +25,7 @@ constexpr int CONV_WARPS = 4;
 
 struct ConvParams {
   int B, T, C;
-  int sets;   // sets of 32 * VEC channels
+  int sets;   // sets of 64 channels
   int span;   // tokens of a warp's span
   int spans;  // spans of a sequence (of the packed buffer)
   const int* cu;
@@ -70,14 +70,14 @@ __device__ __forceinline__ ConvRun conv_run(const ConvParams& p, int b, int t0, 
 }
 
 // Row `slot` of a sequence's cache.
-__device__ __forceinline__ int64_t cache_at(const ConvParams& p, int seq, int slot, int c0) {
-  return ((int64_t)seq * HALO + slot) * p.C + c0;
+__device__ __forceinline__ int64_t cache_at(const ConvParams& p, int seq, int slot, int base) {
+  return ((int64_t)seq * HALO + slot) * p.C + base;
 }
 
 // Empty sequences: the cache (its gradient) goes through; without one a new
 // cache is zero.
-template <int VEC>
-__device__ __forceinline__ void pass_empty(const ConvParams& p, const float* from, float* to, int c0, bool on) {
+template <RowMode MODE>
+__device__ __forceinline__ void pass_empty(const ConvParams& p, const float* from, float* to, const Pair<MODE>& ch, int base) {
   const int lane = threadIdx.x & 31;
   for (int n0 = (int)threadIdx.x - lane; n0 < p.B; n0 += blockDim.x) {
     const int n = n0 + lane;
@@ -85,34 +85,24 @@ __device__ __forceinline__ void pass_empty(const ConvParams& p, const float* fro
     while (empty) {
       const int j = n0 + __ffs(empty) - 1;
       empty &= empty - 1;
-      if (!on) continue;
+      if (!ch.on0) continue;
       #pragma unroll
       for (int s = 0; s < HALO; ++s)
-        put_f32<VEC>(to + cache_at(p, j, s, c0), from ? get_f32<VEC>(from + cache_at(p, j, s, c0)) : f2pk(0.f, 0.f));
+        ch.store_state(to + cache_at(p, j, s, base), from ? ch.load(from + cache_at(p, j, s, base)) : f2pk(0.f, 0.f));
     }
   }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ f32x2 get(const T* p) {
-  float f[2] = {0.f, 0.f};
-  if constexpr (VEC == 2) Vec<T, 2>::unpack(Vec<T, 2>::load(p), f);
-  else f[0] = to_f32<T>(*p);
-  return f2pk(f[0], f[1]);
-}
-
-// The three values before row t of sequence seq that begins at row first, oldest first; x at this lane's channels.
-template <typename T, int VEC>
-__device__ __forceinline__ void window_before(const ConvParams& p, const T* x, int seq, int first, int t, int c0,
-                                              bool on, f32x2 (&win)[HALO]) {
+// The three values before row t of sequence seq that begins at row first, oldest first; x at the set's first channel.
+template <typename T, RowMode MODE>
+__device__ __forceinline__ void window_before(const ConvParams& p, const T* x, int seq, int first, int t, int base,
+                                              const Pair<MODE>& ch, f32x2 (&win)[HALO]) {
   #pragma unroll
   for (int i = 0; i < HALO; ++i) {
     const int row = t - HALO + i;
-    win[i] = f2pk(0.f, 0.f);
-    if (!on) continue;
-    if (row >= first) win[i] = get<T, VEC>(x + (int64_t)row * p.x.s1);
-    else if (p.cache_in) win[i] = get_f32<VEC>(p.cache_in + cache_at(p, seq, row - first + HALO, c0));
-    else win[i] = get<T, VEC>(x + (int64_t)first * p.x.s1);
+    if (row >= first) win[i] = ch.load(x + (int64_t)row * p.x.s1);
+    else if (p.cache_in) win[i] = ch.load(p.cache_in + cache_at(p, seq, row - first + HALO, base));
+    else win[i] = ch.load(x + (int64_t)first * p.x.s1);
   }
 }
 
@@ -124,31 +114,31 @@ __device__ __forceinline__ void slide(f32x2 (&win)[HALO], f32x2 x) {
   win[1] = win[2];
   win[2] = x;
 }
-template <int VEC>
-__device__ __forceinline__ void load_taps(const ConvParams& p, int c0, bool on, f32x2 (&w)[HALO + 1]) {
+template <RowMode MODE>
+__device__ __forceinline__ void load_taps(const ConvParams& p, int base, const Pair<MODE>& ch, f32x2 (&w)[HALO + 1]) {
   #pragma unroll
   for (int j = 0; j <= HALO; ++j)
-    w[j] = on ? f2pk(__ldg(p.w + (int64_t)c0 * 4 + j), VEC == 2 ? __ldg(p.w + (int64_t)(c0 + VEC - 1) * 4 + j) : 0.f)
-              : f2pk(0.f, 0.f);
+    w[j] = f2pk(ch.on0 ? __ldg(p.w + (int64_t)(base + ch.c0) * (HALO + 1) + j) : 0.f,
+                ch.on1 ? __ldg(p.w + (int64_t)(base + ch.c1) * (HALO + 1) + j) : 0.f);
 }
 
-template <typename T, int VEC, bool COOP, bool PACKED>
+template <typename T, RowMode MODE, bool PACKED>
 __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p) {
-  typedef Rows<T, VEC, COOP> R;
+  typedef Rows<T, MODE> R;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int base = (int)blockIdx.x * 32 * VEC, c0 = base + lane * VEC;
-  const bool on = c0 < p.C;
-  if (PACKED && p.cache_out && blockIdx.y == 0) pass_empty<VEC>(p, p.cache_in, p.cache_out, c0, on);
+  const int base = (int)blockIdx.x * SET;
+  const Pair<MODE> ch(lane, p.C - base);
+  if (PACKED && p.cache_out && blockIdx.y == 0) pass_empty(p, p.cache_in, p.cache_out, ch, base);
   f32x2 w[HALO + 1];
-  load_taps<VEC>(p, c0, on, w);
+  load_taps(p, base, ch, w);
 
   const int64_t units = (int64_t)p.spans * (PACKED ? 1 : p.B);
   for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < units; unit += (int64_t)gridDim.y * CONV_WARPS) {
     const int b = PACKED ? 0 : (int)(unit / p.spans);
     const int s0 = (int)(PACKED ? unit : unit % p.spans) * p.span, s1 = s0 + p.span < p.T ? s0 + p.span : p.T;
     const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
-    T* y = static_cast<T*>(const_cast<void*>(p.y.p)) + b * p.y.s0 + c0;
+    T* y = static_cast<T*>(const_cast<void*>(p.y.p)) + b * p.y.s0 + base;
     auto rows = [&](int run) { return R{smem + ((run % STAGES) * CONV_WARPS + warp) * R::BYTES}; };
     auto fetch = [&](int run) {
       if (s0 + run * RUN < s1) rows(run).fetch(x, p.x.s1, s0 + run * RUN, p.T, p.C - base, lane);
@@ -165,17 +155,17 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p
         #pragma unroll
         for (int i = 0; i < HALO; ++i) win[i] = f2pk(0.f, 0.f);
         const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
-        if ((k.valid & 1) && !(k.start & 1)) window_before<T, VEC>(p, x + lane * VEC, seq, first, t0, c0, on, win);
+        if ((k.valid & 1) && !(k.start & 1)) window_before(p, x, seq, first, t0, base, ch, win);
       }
       cp_async_wait<STAGES - 1>();
       __syncwarp();
-      const R xs = rows(run);
+      const auto xs = rows(run).view(x, p.x.s1, t0, lane);
       T* out = y + (int64_t)t0 * p.y.s1;
       if (k.inside() && t0 + RUN <= s1) {
         #pragma unroll
         for (int i = 0; i < RUN; ++i) {
-          const f32x2 xf = xs.get(i, lane), pre = taps(win, xf, w);
-          if (on) put<T, VEC>(out, f2mul(pre, sigmoid2(pre)));
+          const f32x2 xf = xs.get(i), pre = taps(win, xf, w);
+          if (ch.on0) ch.store(out, f2mul(pre, sigmoid2(pre)));
           out += p.y.s1;
           slide(win, xf);
         }
@@ -184,15 +174,15 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p
       #pragma unroll 1
       for (int i = 0; i < RUN && t0 + i < s1; ++i) {
         const int seq = __shfl_sync(0xffffffffu, k.seq, i);
-        const f32x2 xf = xs.get(i, lane);
-        if ((k.start >> i) & 1) window_before<T, VEC>(p, x + lane * VEC, seq, t0 + i, t0 + i, c0, on, win);
+        const f32x2 xf = xs.get(i);
+        if ((k.start >> i) & 1) window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
         const f32x2 pre = taps(win, xf, w);
-        if (on) put<T, VEC>(out, (k.valid >> i) & 1 ? f2mul(pre, sigmoid2(pre)) : f2pk(0.f, 0.f));
+        if (ch.on0) ch.store(out, (k.valid >> i) & 1 ? f2mul(pre, sigmoid2(pre)) : f2pk(0.f, 0.f));
         out += p.y.s1;
         slide(win, xf);
-        if (((k.last >> i) & 1) && p.cache_out && on)
+        if (((k.last >> i) & 1) && p.cache_out && ch.on0)
           #pragma unroll
-          for (int s = 0; s < HALO; ++s) put_f32<VEC>(p.cache_out + cache_at(p, seq, s, c0), win[s]);
+          for (int s = 0; s < HALO; ++s) ch.store_state(p.cache_out + cache_at(p, seq, s, base), win[s]);
       }
     }
   }
@@ -201,17 +191,17 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p
 // Adjoint.  Token s adds w[3-k] dpre_s to dx of token s - k, and to the
 // gradient of the three values before its sequence where s - k lies there;
 // the span that holds the sequence's first token collects those.
-template <typename T, int VEC, bool COOP, bool PACKED>
+template <typename T, RowMode MODE, bool PACKED>
 __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p) {
-  typedef Rows<T, VEC, COOP> R;
+  typedef Rows<T, MODE> R;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int base = (int)blockIdx.x * 32 * VEC, c0 = base + lane * VEC;
-  const bool on = c0 < p.C;
+  const int base = (int)blockIdx.x * SET;
+  const Pair<MODE> ch(lane, p.C - base);
   const f32x2 zero = f2pk(0.f, 0.f), one = f2pk(1.f, 1.f), minus = f2pk(-1.f, -1.f);
-  if (PACKED && p.d_cache_in && blockIdx.y == 0) pass_empty<VEC>(p, p.d_cache_out, p.d_cache_in, c0, on);
+  if (PACKED && p.d_cache_in && blockIdx.y == 0) pass_empty(p, p.d_cache_out, p.d_cache_in, ch, base);
   f32x2 w[HALO + 1], dw[HALO + 1];
-  load_taps<VEC>(p, c0, on, w);
+  load_taps(p, base, ch, w);
   #pragma unroll
   for (int j = 0; j <= HALO; ++j) dw[j] = zero;
 
@@ -222,7 +212,7 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
     const int end = s1 + HALO;  // rows walked: a token's dx leaves three tokens later
     const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
     const T* dy = static_cast<const T*>(p.y.p) + b * p.y.s0 + base;
-    T* dx = static_cast<T*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + c0;
+    T* dx = static_cast<T*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + base;
     auto rows = [&](int run, int which) {
       return R{smem + (((run % STAGES) * CONV_WARPS + warp) * 2 + which) * R::BYTES};
     };
@@ -248,13 +238,14 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
         for (int i = 0; i < HALO; ++i) win[i] = zero;
         const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
         if ((k.valid & 1) && !(k.start & 1)) {
-          window_before<T, VEC>(p, x + lane * VEC, seq, first, t0, c0, on, win);
+          window_before(p, x, seq, first, t0, base, ch, win);
           pos = t0 - first;
         }
       }
       cp_async_wait<STAGES - 1>();
       __syncwarp();
-      const R xs = rows(run, 0), ds = rows(run, 1);
+      const auto xs = rows(run, 0).view(x, p.x.s1, t0, lane);
+      const auto ds = rows(run, 1).view(dy, p.y.s1, t0, lane);
       T* out = dx + (int64_t)(t0 - HALO) * p.dx.s1;
       // dpre of a token, and its part of dw where the token is the span's own
       auto adjoint = [&](f32x2 xf, f32x2 df, bool own) {
@@ -270,10 +261,10 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
       if (k.inside() && pos >= HALO) {
         #pragma unroll
         for (int i = 0; i < RUN; ++i) {
-          const f32x2 xf = xs.get(i, lane);
-          const f32x2 dp = adjoint(xf, ds.get(i, lane), i < RUN - HALO || t0 + i < s1);
+          const f32x2 xf = xs.get(i);
+          const f32x2 dp = adjoint(xf, ds.get(i), i < RUN - HALO || t0 + i < s1);
           const f32x2 done = f2fma(w[0], dp, pend[2]);
-          if (on && (i >= HALO || t0 > s0)) put<T, VEC>(out, done);
+          if (ch.on0 && (i >= HALO || t0 > s0)) ch.store(out, done);
           out += p.dx.s1;
           pend[2] = f2fma(w[1], dp, pend[1]);
           pend[1] = f2fma(w[2], dp, pend[0]);
@@ -286,14 +277,14 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
       for (int i = 0; i < RUN && t0 + i < end; ++i) {
         const int seq = __shfl_sync(0xffffffffu, k.seq, i);
         const bool opens = (k.start >> i) & 1, closes = (k.last >> i) & 1, in = (k.valid >> i) & 1;
-        const f32x2 xf = xs.get(i, lane);
+        const f32x2 xf = xs.get(i);
         if (opens) {
           pos = 0;
           owned = t0 + i < s1;
-          window_before<T, VEC>(p, x + lane * VEC, seq, t0 + i, t0 + i, c0, on, win);
+          window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
           before[0] = before[1] = before[2] = zero;
         }
-        const f32x2 dp = in ? adjoint(xf, ds.get(i, lane), t0 + i < s1) : zero;
+        const f32x2 dp = in ? adjoint(xf, ds.get(i), t0 + i < s1) : zero;
         f32x2 part[HALO + 1] = {zero, pend[0], pend[1], pend[2]};  // dx of this token and the three before it
         auto give = [&](int j, f32x2 v) {  // to token s - j, or to what lies before the sequence
           if (pos >= j) part[j] = f2add(part[j], v);
@@ -304,17 +295,17 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
         if (in) {
           #pragma unroll
           for (int j = 0; j <= HALO; ++j) give(j, f2mul(w[HALO - j], dp));
-          if (closes && p.d_cache_out && on) {  // the new cache holds the last three values
+          if (closes && p.d_cache_out) {  // the new cache holds the last three values
             #pragma unroll
             for (int j = 0; j < HALO; ++j)
-              give(j, get_f32<VEC>(p.d_cache_out + cache_at(p, seq, HALO - 1 - j, c0)));
+              give(j, ch.load(p.d_cache_out + cache_at(p, seq, HALO - 1 - j, base)));
           }
           // no later token reaches before the sequence: hand on what does
           if (owned && (pos == HALO - 1 || (closes && pos < HALO - 1))) {
             if (p.d_cache_in) {
-              if (on)
+              if (ch.on0)
                 #pragma unroll
-                for (int s = 0; s < HALO; ++s) put_f32<VEC>(p.d_cache_in + cache_at(p, seq, s, c0), before[s]);
+                for (int s = 0; s < HALO; ++s) ch.store_state(p.d_cache_in + cache_at(p, seq, s, base), before[s]);
             } else if (!p.cache_in) {  // copies of the first token
               #pragma unroll
               for (int j = 0; j < HALO; ++j)
@@ -323,7 +314,7 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
           }
         }
         const int row = t0 + i - HALO;
-        if (on && row >= s0 && row < s1) put<T, VEC>(out, part[HALO]);
+        if (ch.on0 && row >= s0 && row < s1) ch.store(out, part[HALO]);
         out += p.dx.s1;
         pend[0] = part[0];
         pend[1] = part[1];
@@ -338,17 +329,17 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
   float* red = reinterpret_cast<float*>(smem);  // [warp][channel][tap]
   #pragma unroll
   for (int j = 0; j <= HALO; ++j) {
-    float d[2];
-    f2un(dw[j], d[0], d[1]);
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) red[((warp * 32 + lane) * VEC + v) * (HALO + 1) + j] = d[v];
+    float d0, d1;
+    f2un(dw[j], d0, d1);
+    red[(warp * SET + ch.c0) * (HALO + 1) + j] = d0;
+    red[(warp * SET + ch.c1) * (HALO + 1) + j] = d1;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 32 * VEC * (HALO + 1); e += 32 * CONV_WARPS) {
+  for (int e = threadIdx.x; e < SET * (HALO + 1); e += 32 * CONV_WARPS) {
     if (base + e / (HALO + 1) >= p.C) continue;
     float s = 0.f;
     #pragma unroll
-    for (int k = 0; k < CONV_WARPS; ++k) s += red[k * 32 * VEC * (HALO + 1) + e];
+    for (int k = 0; k < CONV_WARPS; ++k) s += red[k * SET * (HALO + 1) + e];
     p.part[((int64_t)blockIdx.y * p.C + base) * (HALO + 1) + e] = s;
   }
 }
@@ -367,20 +358,18 @@ static int check_conv(const gdn2_conv_args* a, const char* fn) {
   return GDN2_OK;
 }
 
-// How a call is cut up: channels per lane, 16-byte copies, spans of tokens and blocks along them.
+// How a call is cut up: how rows are held, spans of tokens and blocks along them.
 struct ConvPlan {
-  int vec;
-  bool coop;
+  RowMode mode;
   int sets, span, spans, blocks;
 };
 
 // Spans of `runs` runs less `less` tokens, down to one run until the warps fill the GPU.  `blocks_per_sm`: blocks
 // along the spans (each leaves a partial row of dw), 0 for all of them.
-static ConvPlan plan_conv(const gdn2_conv_args* a, bool pairs, bool coop, int less, int blocks_per_sm) {
+static ConvPlan plan_conv(const gdn2_conv_args* a, RowMode mode, int less, int blocks_per_sm) {
   ConvPlan n;
-  n.vec = pairs ? 2 : 1;
-  n.coop = pairs && coop;
-  n.sets = (a->channels + 32 * n.vec - 1) / (32 * n.vec);
+  n.mode = mode;
+  n.sets = (a->channels + SET - 1) / SET;
   const int rows = a->cu_seqlens ? 1 : a->batch;
   int runs = 8;
   for (;; runs /= 2) {
@@ -414,20 +403,22 @@ static int launch_conv(K kernel, const ConvParams& p, const ConvPlan& n, int sta
   return check_cuda(cudaGetLastError(), fn);
 }
 
-template <typename T, int VEC, bool COOP>
+template <typename T, RowMode MODE>
 static int run_conv(const ConvParams& p, const ConvPlan& n, bool bwd, cudaStream_t st, const char* fn) {
-  const int bytes = Rows<T, VEC, COOP>::BYTES;
+  const int bytes = Rows<T, MODE>::BYTES;
   if (bwd)
-    return p.cu ? launch_conv(k_conv_bwd<T, VEC, COOP, true>, p, n, 2 * bytes, st, fn)
-                : launch_conv(k_conv_bwd<T, VEC, COOP, false>, p, n, 2 * bytes, st, fn);
-  return p.cu ? launch_conv(k_conv_fwd<T, VEC, COOP, true>, p, n, bytes, st, fn)
-              : launch_conv(k_conv_fwd<T, VEC, COOP, false>, p, n, bytes, st, fn);
+    return p.cu ? launch_conv(k_conv_bwd<T, MODE, true>, p, n, 2 * bytes, st, fn)
+                : launch_conv(k_conv_bwd<T, MODE, false>, p, n, 2 * bytes, st, fn);
+  return p.cu ? launch_conv(k_conv_fwd<T, MODE, true>, p, n, bytes, st, fn)
+              : launch_conv(k_conv_fwd<T, MODE, false>, p, n, bytes, st, fn);
 }
 
 template <typename T>
 static int dispatch_conv(const ConvParams& p, const ConvPlan& n, bool bwd, cudaStream_t st, const char* fn) {
-  if (n.coop) return run_conv<T, 2, true>(p, n, bwd, st, fn);
-  return n.vec == 2 ? run_conv<T, 2, false>(p, n, bwd, st, fn) : run_conv<T, 1, false>(p, n, bwd, st, fn);
+  return n.mode == ROWS16      ? run_conv<T, ROWS16>(p, n, bwd, st, fn)
+         : n.mode == ROWS_PAIR ? run_conv<T, ROWS_PAIR>(p, n, bwd, st, fn)
+         : n.mode == ROWS_ODD  ? run_conv<T, ROWS_ODD>(p, n, bwd, st, fn)
+                               : run_conv<T, ROWS_ANY>(p, n, bwd, st, fn);
 }
 
 int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_out, cudaStream_t st) {
@@ -436,8 +427,8 @@ int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_ou
   if (rc) return rc;
   if (a->seq_len && !y.data) return set_error(GDN2_EINVAL, "%s: null tensor pointer", fn);
   const int e = elem_bytes(a->dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * e, e) && rows_ok(y, 2 * e, e);
-  const ConvPlan n = plan_conv(a, pairs, a->channels * e % 16 == 0 && rows_ok(a->x, 16, e), 0, 0);
+  const RowTensor t[] = {{&a->x, e, true}, {&y, e, false}};
+  const ConvPlan n = plan_conv(a, row_mode(a->channels, t, 2), 0, 0);
   ConvParams p;
   fill_conv(p, a, n);
   p.y = make_dview(y);
@@ -449,9 +440,8 @@ int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_ou
 static ConvPlan plan_conv_bwd(const gdn2_conv_bwd_args* q) {
   const gdn2_conv_args* a = &q->fwd;
   const int e = elem_bytes(a->dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * e, e) && rows_ok(q->d_y, 2 * e, e) && rows_ok(q->dx, 2 * e, e);
-  const bool coop = a->channels * e % 16 == 0 && rows_ok(a->x, 16, e) && rows_ok(q->d_y, 16, e);
-  return plan_conv(a, pairs, coop, HALO, 5);
+  const RowTensor t[] = {{&a->x, e, true}, {&q->d_y, e, true}, {&q->dx, e, false}};
+  return plan_conv(a, row_mode(a->channels, t, 3), HALO, 5);
 }
 
 size_t conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* q) {

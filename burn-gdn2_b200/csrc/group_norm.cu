@@ -17,7 +17,7 @@
 // of their gradients stay in registers too.  Those sums leave through one
 // partial row per slot of lanes, added up by a second kernel in a fixed
 // order: no atomics.
-#include "scan.cuh"
+#include "sequence.cuh"
 
 namespace gdn2 {
 

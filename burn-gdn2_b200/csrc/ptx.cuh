@@ -200,14 +200,13 @@ __device__ __forceinline__ void cp_async16(void* sdst, const void* gsrc) {
 __device__ __forceinline__ void cp_async8(void* sdst, const void* gsrc) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(sdst)), "l"(gsrc) : "memory");
 }
-// 4, 8 or 16 bytes, or zeros in their place without a read of gsrc
+// The same of `read` bytes (0 to BYTES; none: gsrc is not read), zeros behind them; BYTES 4, 8 or 16, both aligned to it.
 template <int BYTES>
-__device__ __forceinline__ void cp_async_zfill(void* sdst, const void* gsrc, bool read) {
-  const int n = read ? BYTES : 0;
+__device__ __forceinline__ void cp_async_zfill(void* sdst, const void* gsrc, int read) {
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sdst)), "l"(gsrc), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sdst)), "l"(gsrc), "r"(read) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(sdst)), "l"(gsrc), "r"(n), "n"(BYTES)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem_u32(sdst)), "l"(gsrc), "r"(read), "n"(BYTES)
                  : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -1,444 +1,31 @@
-// Gated scan: the diagonal gated linear recurrence
-//
-//   h_t = e^{g_t} h_{t-1} + s_t x_t        s_t = 1, or 1 - e^{g_t} (complement)
-//
-// per channel of [B][T][C] (or of packed sequences), and its adjoint
-//
-//   l_t = dh_t + e^{g_{t+1}} l_{t+1},  dx_t = s_t l_t,
-//   dg_t = e^{g_t} (h_{t-1} [- x_t]) l_t,  dstate = e^{g_0} l_0.
-//
-// Both are bound by HBM with the issue rate close behind (some twenty
-// instructions for 8 to 14 bytes a value): a forward reads x and g and writes
-// h, a backward reads x, g and dh and writes dx and dg.  So each value is
-// read once and its decay computed once, between the load and the store, in
-// packed pairs of channels: a warp holds RUN tokens of 32 * VEC channels in
-// registers, reduces them to the affine map c -> A c + H of the run, the maps of
-// a block's runs are joined through shared memory, and the block walks its
-// channels' time axis, the loads of the next step in flight meanwhile.
-//
-// With few chains (sequences times sets of channels) the time axis is cut
-// into segments as well: a first launch reduces every segment to its map, the
-// second starts each segment from the maps before it.  That reads the inputs
-// twice, and pays below about 100 chains, where one block each would leave
-// the memory system idle.  The joining order is fixed by the sizes: results
-// do not depend on timing.
+// Gated scan, host side: argument checks, how a call is cut up, and its
+// launches (kernels: scan.cuh).
 #include "scan.cuh"
 
 namespace gdn2 {
 
-static_assert(RUN == 16, "the spacing of the states a backward starts from is part of the interface");
-constexpr int MAX_SEGMENTS = 128;
-
-struct ScanParams {
-  int B, T, C;      // dense: B sequences of T; packed: N sequences in T rows
-  int sets;         // sets of 32 * VEC channels
-  int steps;        // tiles of a segment
-  int segments;
-  const int* cu;
-  DView x, g, h;    // forward: h out.  backward: h = dh
-  DView dx, dg;
-  const float* state_in;
-  float* state_out;
-  const float* d_state_out;
-  float* d_state_in;
-  float* carry;     // [B or 1][ceil(T / RUN)][C]: state before every RUN-th token
-  float2* maps;     // [chain][segment][CH] maps of the segments, or null (one segment)
-  int* map_cuts;    // [chain][segment]: a sequence begins (adjoint: ends) in the segment
-};
-
-// The maps of a step's runs, twice for alternating steps.  cut: a sequence
-// begins (adjoint: ends) in the run, so that nothing from before it comes
-// through, not even an infinity or NaN times zero.
-template <int NW>
-struct ScanMaps {
-  ulonglong2 run[2][NW][32];  // (A, H) pairs
-  int cut[2][NW];
-};
-
-// From the state `c` before the step's first token (after its last, in the
-// adjoint), the state before this warp's run; c becomes the state after the
-// step, and the maps join to `A` of the whole (with SUM).
-template <int NW, bool PACKED, bool SUM>
-__device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int lane, f32x2 A, f32x2 H, bool cut,
-                                      f32x2& c, f32x2& all, bool& any_cut) {
-  sh.run[buf][warp][lane] = make_ulonglong2(A, H);
-  if (PACKED && lane == 0) sh.cut[buf][warp] = cut;
-  __syncthreads();
-  f32x2 cin = c;
-  #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w == warp) cin = c;
-    const ulonglong2 m = sh.run[buf][w][lane];
-    const bool cuts = PACKED && sh.cut[buf][w];
-    c = cuts ? m.y : f2fma(m.x, c, m.y);
-    if (SUM) {
-      all = f2mul(all, m.x);
-      any_cut |= cuts;
-    }
-  }
-  return cin;
-}
-
-// Decays of a run: a = e^g, and k = 1 - e^g where it is wanted.
-template <typename G, bool COMP>
-__device__ __forceinline__ void decays(const G& rows, int lane, f32x2 (&a)[RUN], f32x2 (&k)[RUN]) {
-  float far = 0.f;
-  #pragma unroll
-  for (int i = 0; i < RUN; ++i) {
-    const f32x2 g = rows.get(i, lane);
-    float g0, g1;
-    f2un(g, g0, g1);
-    far = fmaxf(far, fmaxf(fabsf(g0), fabsf(g1)));
-    exp_pair<COMP>(g, a[i], k[i]);
-  }
-  if (far > kExpRange) {  // a reset (-inf), a decay below every f32, or growth
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      float g[2], e[2], m[2];
-      f2un(rows.get(i, lane), g[0], g[1]);
-      f2un(a[i], e[0], e[1]);
-      if (COMP) f2un(k[i], m[0], m[1]);
-      #pragma unroll
-      for (int v = 0; v < 2; ++v)
-        if (fabsf(g[v]) > kExpRange) {
-          e[v] = expf(g[v]);
-          m[v] = -expm1f(g[v]);
-        }
-      a[i] = f2pk(e[0], e[1]);
-      if (COMP) k[i] = f2pk(m[0], m[1]);
-    }
-  }
-}
-
-// Which of a run's tokens open or close a sequence or lie in one, one bit a
-// token; seq: the sequence of token `lane`.
-struct RunMasks {
-  unsigned start, last, valid;
-  int seq;
-  __device__ __forceinline__ int sequence(int i) const { return __shfl_sync(0xffffffffu, seq, i); }
-};
-__device__ __forceinline__ RunMasks run_masks(const int* __restrict__ cu, int N, int T, int t0, int lane) {
-  RunMasks k;
-  const int t = t0 + lane;
-  k.seq = -1;
-  bool s = false, l = false;
-  if (lane < RUN && t < T) {
-    k.seq = find_sequence(cu, N, t);
-    if (k.seq >= 0) {
-      s = __ldg(cu + k.seq) == t;
-      l = t + 1 == T || __ldg(cu + k.seq + 1) == t + 1;
-    }
-  }
-  k.start = __ballot_sync(0xffffffffu, s);
-  k.last = __ballot_sync(0xffffffffu, l);
-  k.valid = __ballot_sync(0xffffffffu, k.seq >= 0);
-  return k;
-}
-
-// Empty sequences hand their state (its gradient) through.
-template <int VEC>
-__device__ __forceinline__ void pass_empty(const ScanParams& p, const float* from, float* to, int c0, bool on) {
-  const int lane = threadIdx.x & 31;
-  for (int n0 = (int)threadIdx.x - lane; n0 < p.B; n0 += blockDim.x) {
-    const int n = n0 + lane;
-    unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
-    while (empty) {
-      const int64_t at = (int64_t)(n0 + __ffs(empty) - 1) * p.C + c0;
-      empty &= empty - 1;
-      if (on) put_f32<VEC>(to + at, from ? get_f32<VEC>(from + at) : f2pk(0.f, 0.f));
-    }
-  }
-}
-
-// The state before segment `seg` (adjoint: after it): `c` through the maps of
-// the segments before (after) it.
-template <bool PACKED>
-__device__ __forceinline__ f32x2 through_segments(const ScanParams& p, int64_t chain, int seg, int lane, f32x2 c) {
-  const ulonglong2* m = reinterpret_cast<const ulonglong2*>(p.maps) + chain * p.segments * 32 + lane;
-  const int* cut = p.map_cuts + chain * p.segments;
-  #pragma unroll 8
-  for (int s = 0; s < seg; ++s) {
-    const ulonglong2 v = m[s * 32];
-    c = PACKED && cut[s] ? v.y : f2fma(v.x, c, v.y);
-  }
-  return c;
-}
-template <bool PACKED>
-__device__ __forceinline__ void write_map(const ScanParams& p, int64_t chain, int seg, f32x2 A, f32x2 H, bool cut) {
-  if (threadIdx.x < 32) reinterpret_cast<ulonglong2*>(p.maps)[(chain * p.segments + seg) * 32 + threadIdx.x] = make_ulonglong2(A, H);
-  if (PACKED && threadIdx.x == 0) p.map_cuts[chain * p.segments + seg] = cut;
-}
-
-// MAPS: only the segment's map, for the first of two launches.
-template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED, bool MAPS>
-__global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
-  typedef Rows<TX, VEC, COOP> RX;
-  typedef Rows<TG, VEC, COOP> RG;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ ScanMaps<NW> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int seg = (int)(blockIdx.x % p.segments);
-  const int64_t chain = blockIdx.x / p.segments;
-  const int b = PACKED ? 0 : (int)(chain / p.sets);
-  const int base = (int)(chain % p.sets) * 32 * VEC, c0 = base + lane * VEC;
-  const bool on = c0 < p.C;
-  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
-  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
-  TX* h = static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + c0;
-  const int runs = (p.T + RUN - 1) / RUN;
-
-  if (PACKED && !MAPS && p.state_out && seg == 0) pass_empty<VEC>(p, p.state_in, p.state_out, c0, on);
-  if (!p.steps) return;
-  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
-  bool any_cut = false;
-  if (!MAPS) {
-    if (!PACKED && p.state_in && on) c = get_f32<VEC>(p.state_in + (int64_t)b * p.C + c0);
-    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
-  }
-
-  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * (RX::BYTES + RG::BYTES); };
-  auto run_at = [&](int step) { return ((seg * p.steps + step) * NW + warp) * RUN; };
-  auto fetch = [&](int step) {
-    if (step < p.steps) {
-      RX{stage(step)}.fetch(x, p.x.s1, run_at(step), p.T, p.C - base, lane);
-      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, run_at(step), p.T, p.C - base, lane);
-    }
-    cp_async_commit();
-  };
-  for (int step = 0; step < STAGES - 1; ++step) fetch(step);
-  for (int step = 0; step < p.steps; ++step) {
-    __syncwarp();
-    fetch(step + STAGES - 1);
-    const int t0 = run_at(step);
-    RunMasks k;
-    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const RX xs{stage(step)};
-
-    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run (after the
-    // run's last cut, a[i] has no meaning)
-    f32x2 a[RUN], u[RUN], A = f2pk(1.f, 1.f), H = f2pk(0.f, 0.f);
-    decays<RG, COMP>(RG{stage(step) + RX::BYTES}, lane, a, u);
-    const unsigned cuts = PACKED ? (k.start | ~k.valid) & ((1u << RUN) - 1) : 0;
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      const f32x2 in = COMP ? f2mul(u[i], xs.get(i, lane)) : xs.get(i, lane);
-      if (PACKED && ((cuts >> i) & 1)) {
-        const int n = k.sequence(i);
-        f32x2 st = f2pk(0.f, 0.f);
-        if ((k.start >> i) & 1) {
-          if (p.state_in && on) st = get_f32<VEC>(p.state_in + (int64_t)n * p.C + c0);
-          H = f2fma(a[i], st, in);
-        } else {
-          H = st;
-        }
-      } else {
-        H = f2fma(a[i], H, in);
-        A = f2mul(A, a[i]);
-      }
-      a[i] = A;
-      u[i] = H;
-    }
-    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cuts != 0, c, all, any_cut);
-    if (MAPS) continue;
-
-    const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
-    if (on && t0 < p.T) {
-      if (p.carry) put_f32<VEC>(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + c0, cin);
-      TX* out = h + (int64_t)t0 * p.h.s1;
-      #pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        if (!PACKED || i < first_cut) u[i] = f2fma(a[i], cin, u[i]);
-        if (t0 + i < p.T) put<TX, VEC>(out, u[i]);
-        out += p.h.s1;
-      }
-    }
-    if (PACKED && p.state_out && k.last) {
-      #pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        if (!((k.last >> i) & 1)) continue;
-        const int n = k.sequence(i);
-        if (on) put_f32<VEC>(p.state_out + (int64_t)n * p.C + c0, u[i]);
-      }
-    }
-  }
-  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
-  else if (!PACKED && p.state_out && seg == p.segments - 1 && warp == 0 && on)
-    put_f32<VEC>(p.state_out + (int64_t)b * p.C + c0, c);
-}
-
-// The adjoint, walked from the last tile to the first; warp 0 takes a step's
-// latest run, segment 0 the latest segment.  States inside a run are rebuilt
-// from the state that the forward kept before it.
-template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED, bool MAPS>
-__global__ void __launch_bounds__(32 * NW) k_scan_bwd(const ScanParams p) {
-  typedef Rows<TX, VEC, COOP> RX;
-  typedef Rows<TG, VEC, COOP> RG;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ ScanMaps<NW> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int seg = (int)(blockIdx.x % p.segments);
-  const int64_t chain = blockIdx.x / p.segments;
-  const int b = PACKED ? 0 : (int)(chain / p.sets);
-  const int base = (int)(chain % p.sets) * 32 * VEC, c0 = base + lane * VEC;
-  const bool on = c0 < p.C;
-  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
-  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
-  const TX* dh = static_cast<const TX*>(p.h.p) + b * p.h.s0 + base;
-  TX* dx = static_cast<TX*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + c0;
-  TG* dg = static_cast<TG*>(const_cast<void*>(p.dg.p)) + b * p.dg.s0 + c0;
-  const int runs = (p.T + RUN - 1) / RUN;
-
-  if (PACKED && !MAPS && p.d_state_in && seg == 0) pass_empty<VEC>(p, p.d_state_out, p.d_state_in, c0, on);
-  if (!p.steps) return;
-  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
-  bool any_cut = false;
-  if (!MAPS) {
-    if (!PACKED && p.d_state_out && on) c = get_f32<VEC>(p.d_state_out + (int64_t)b * p.C + c0);
-    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
-  }
-
-  constexpr int STAGE = 2 * RX::BYTES + RG::BYTES;
-  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
-  auto run_at = [&](int step) { return ((p.segments * p.steps - 1 - (seg * p.steps + step)) * NW + NW - 1 - warp) * RUN; };
-  f32x2 next_state = f2pk(0.f, 0.f);  // state before the next step's run
-  auto fetch = [&](int step) {
-    if (step < p.steps) {
-      const int t0 = run_at(step);
-      RX{stage(step)}.fetch(dh, p.h.s1, t0, p.T, p.C - base, lane);
-      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, t0, p.T, p.C - base, lane);
-      if (!MAPS) RX{stage(step) + RX::BYTES + RG::BYTES}.fetch(x, p.x.s1, t0, p.T, p.C - base, lane);
-      if (!MAPS && on && t0 < p.T) next_state = get_f32<VEC>(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + c0);
-    }
-    cp_async_commit();
-  };
-  static_assert(STAGES == 2, "next_state is one step ahead");
-  fetch(0);
-  for (int step = 0; step < p.steps; ++step) {
-    __syncwarp();
-    f32x2 hp = next_state;
-    fetch(step + 1);
-    const int t0 = run_at(step);
-    RunMasks k;
-    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const RX ds{stage(step)}, xs{stage(step) + RX::BYTES + RG::BYTES};
-
-    // a[i]: decay of token i; w[i]: what dg multiplies, h_{i-1} or h_{i-1} - x_i
-    f32x2 a[RUN], m[RUN], w[RUN];
-    decays<RG, COMP && !MAPS>(RG{stage(step) + RX::BYTES}, lane, a, m);
-    if (!MAPS) {
-      #pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        const f32x2 xf = xs.get(i, lane);
-        if (PACKED && ((k.start >> i) & 1)) {
-          const int n = k.sequence(i);
-          hp = p.state_in && on ? get_f32<VEC>(p.state_in + (int64_t)n * p.C + c0) : f2pk(0.f, 0.f);
-        }
-        w[i] = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
-        hp = f2fma(a[i], hp, COMP ? f2mul(m[i], xf) : xf);
-      }
-    }
-    // the run's map from the adjoint after it to the adjoint before it
-    const unsigned cuts = PACKED ? (k.last | ~k.valid) & ((1u << RUN) - 1) : 0;
-    f32x2 A = f2pk(1.f, 1.f), M = f2pk(0.f, 0.f);
-    #pragma unroll
-    for (int i = RUN - 1; i >= 0; --i) {
-      if (PACKED && ((cuts >> i) & 1)) {
-        const int n = k.sequence(i);
-        M = f2pk(0.f, 0.f);
-        if ((k.last >> i) & 1) {
-          if (p.d_state_out && on) M = get_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0);
-          M = f2mul(a[i], f2add(ds.get(i, lane), M));
-        }
-      } else {
-        M = f2mul(a[i], f2add(ds.get(i, lane), M));
-        A = f2mul(A, a[i]);
-      }
-    }
-    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cuts != 0, c, all, any_cut);
-    if (MAPS) continue;
-
-    TX* ox = dx + (int64_t)(t0 + RUN - 1) * p.dx.s1;
-    TG* og = dg + (int64_t)(t0 + RUN - 1) * p.dg.s1;
-    #pragma unroll
-    for (int i = RUN - 1; i >= 0; --i) {
-      const bool out = PACKED && !((k.valid >> i) & 1);
-      if (PACKED && ((k.last >> i) & 1)) {
-        const int n = k.sequence(i);
-        mu = p.d_state_out && on ? get_f32<VEC>(p.d_state_out + (int64_t)n * p.C + c0) : f2pk(0.f, 0.f);
-      }
-      const f32x2 l = f2add(ds.get(i, lane), mu);
-      f32x2 vx = COMP ? f2mul(m[i], l) : l;
-      mu = f2mul(a[i], l);
-      f32x2 vg = f2mul(mu, w[i]);
-      if (out) vx = vg = mu = f2pk(0.f, 0.f);
-      if (on && t0 + i < p.T) {
-        put<TX, VEC>(ox, vx);
-        put<TG, VEC>(og, vg);
-      }
-      ox -= p.dx.s1;
-      og -= p.dg.s1;
-      if (PACKED && p.d_state_in && ((k.start >> i) & 1)) {
-        const int n = k.sequence(i);
-        if (on) put_f32<VEC>(p.d_state_in + (int64_t)n * p.C + c0, mu);
-      }
-    }
-  }
-  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
-  else if (!PACKED && p.d_state_in && seg == p.segments - 1 && warp == 0 && on)
-    put_f32<VEC>(p.d_state_in + (int64_t)b * p.C + c0, c);
-}
-
-// One token per sequence, the decode step: elementwise, state read and
-// written once.  One thread per VEC channels of a sequence.
-template <typename TX, typename TG, int VEC, bool COMP>
-__global__ void __launch_bounds__(256) k_scan_step(const ScanParams p) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = p.C / VEC;
-  if (e >= (int64_t)p.B * per) return;
-  const int64_t b = e / per;
-  const int c0 = (int)(e % per) * VEC;
-  float g[VEC], x[VEC], s[VEC] = {};
-  Vec<TG, VEC>::unpack(Vec<TG, VEC>::load(static_cast<const TG*>(p.g.p) + b * p.g.s0 + c0), g);
-  Vec<TX, VEC>::unpack(Vec<TX, VEC>::load(static_cast<const TX*>(p.x.p) + b * p.x.s0 + c0), x);
-  if (p.state_in) load_f32<VEC>(p.state_in + b * p.C + c0, s);
-  #pragma unroll
-  for (int v = 0; v < VEC; ++v) s[v] = fmaf(expf(g[v]), s[v], COMP ? -expm1f(g[v]) * x[v] : x[v]);
-  if (p.state_out) store_f32<VEC>(p.state_out + b * p.C + c0, s);
-  Vec<TX, VEC>::store(static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + c0, s);
-}
-
-// ---- host ----
-
-// How a call is cut up: channels per lane, 16-byte copies, warps (runs) of a block, segments of the time axis.
-struct ScanPlan {
-  int vec;
-  bool coop;
-  int warps, sets, steps, segments;
-  int64_t chains;
-};
-
-static ScanPlan plan_scan(const gdn2_scan_args* a, bool pairs, bool coop) {
+static ScanPlan plan_scan(const gdn2_scan_args* a, RowMode mode) {
   ScanPlan n;
-  n.vec = pairs ? 2 : 1;
-  n.coop = pairs && coop;
-  n.sets = (a->channels + 32 * n.vec - 1) / (32 * n.vec);
+  n.mode = mode;
+  n.sets = (a->channels + SET - 1) / SET;
   n.chains = (int64_t)n.sets * (a->cu_seqlens ? 1 : a->batch);
   const int runs = (a->seq_len + RUN - 1) / RUN;
-  n.warps = runs <= 1 && !a->cu_seqlens ? 1 : 4;
-  int tiles = (runs + n.warps - 1) / n.warps;
+  // 4096 tokens of 32 n chains, bf16 x and f32 g, forward: n = 2: segments 53 us, eight warps 62; n = 3: 71 and 63;
+  // n = 8: eight warps 102, four 98.
+  const bool cut = n.chains < 80;
+  n.warps = cut || n.chains >= 220 ? 4 : 8;
+  const int tiles = (runs + n.warps - 1) / n.warps;
   n.segments = 1;
-  if (n.warps == 4 && n.chains < 100 && tiles > 1) {
+  n.steps = tiles;
+  if (cut) {
     int64_t want = 148 * 4 / n.chains;
-    if (want > MAX_SEGMENTS) want = MAX_SEGMENTS;
-    if (want > tiles) want = tiles;
-    n.steps = (int)((tiles + want - 1) / want);
-    n.segments = (tiles + n.steps - 1) / n.steps;
+    want = want < MAX_SEGMENTS ? want : MAX_SEGMENTS;
+    want = want < tiles ? want : tiles;
+    if (want > 1) {
+      n.steps = (int)((tiles + want - 1) / want);
+      n.segments = (tiles + n.steps - 1) / n.steps;
+    }
   }
-  if (n.segments == 1) n.steps = tiles;
   return n;
 }
 
@@ -456,56 +43,6 @@ static ScanSpace scan_workspace(const ScanPlan& n, const gdn2_scan_args* a) {
   return w;
 }
 
-template <typename K>
-static int launch(K kernel, const ScanParams& p, const ScanPlan& n, int stage, cudaStream_t st, const char* fn) {
-  const int64_t grid = n.chains * n.segments;
-  if (grid > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: %lld blocks", fn, (long long)grid);
-  const int smem = STAGES * n.warps * stage;
-  int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
-  if (rc) return rc;
-  kernel<<<(unsigned)grid, 32 * n.warps, smem, st>>>(p);
-  return check_cuda(cudaGetLastError(), fn);
-}
-
-template <typename TX, typename TG, int VEC, bool COOP, int NW, bool COMP, bool PACKED>
-static int run_scan(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
-  const int rx = Rows<TX, VEC, COOP>::BYTES, rg = Rows<TG, VEC, COOP>::BYTES;
-  int rc = GDN2_OK;
-  if (bwd) {
-    if (NW > 1 && n.segments > 1)
-      rc = launch(k_scan_bwd<TX, TG, VEC, COOP, NW, COMP, PACKED, NW != 1>, p, n, 2 * rx + rg, st, fn);
-    return rc ? rc : launch(k_scan_bwd<TX, TG, VEC, COOP, NW, COMP, PACKED, false>, p, n, 2 * rx + rg, st, fn);
-  }
-  if (NW > 1 && n.segments > 1)
-    rc = launch(k_scan_fwd<TX, TG, VEC, COOP, NW, COMP, PACKED, NW != 1>, p, n, rx + rg, st, fn);
-  return rc ? rc : launch(k_scan_fwd<TX, TG, VEC, COOP, NW, COMP, PACKED, false>, p, n, rx + rg, st, fn);
-}
-
-template <typename TX, typename TG, int VEC, bool COOP, bool COMP>
-static int run_shape(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
-  if (p.cu) return run_scan<TX, TG, VEC, COOP, 4, COMP, true>(p, n, bwd, st, fn);
-  if (p.T == 1 && !p.carry && !bwd) {
-    const int64_t count = ((int64_t)p.B * (p.C / VEC) + 255) / 256;
-    if (count > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: too many channels", fn);
-    k_scan_step<TX, TG, VEC, COMP><<<(unsigned)count, 256, 0, st>>>(p);
-    return check_cuda(cudaGetLastError(), fn);
-  }
-  if (n.warps == 1) return run_scan<TX, TG, VEC, COOP, 1, COMP, false>(p, n, bwd, st, fn);
-  return run_scan<TX, TG, VEC, COOP, 4, COMP, false>(p, n, bwd, st, fn);
-}
-
-template <typename TX, typename TG>
-static int run_vec(const ScanParams& p, const ScanPlan& n, bool comp, bool bwd, cudaStream_t st, const char* fn) {
-  if (n.coop)
-    return comp ? run_shape<TX, TG, 2, true, true>(p, n, bwd, st, fn)
-                : run_shape<TX, TG, 2, true, false>(p, n, bwd, st, fn);
-  if (n.vec == 2)
-    return comp ? run_shape<TX, TG, 2, false, true>(p, n, bwd, st, fn)
-                : run_shape<TX, TG, 2, false, false>(p, n, bwd, st, fn);
-  return comp ? run_shape<TX, TG, 1, false, true>(p, n, bwd, st, fn)
-              : run_shape<TX, TG, 1, false, false>(p, n, bwd, st, fn);
-}
-
 static int dispatch(ScanParams& p, const gdn2_scan_args* a, const ScanPlan& n, bool bwd, void* ws, size_t ws_bytes,
                     cudaStream_t st, const char* fn) {
   const ScanSpace w = scan_workspace(n, a);
@@ -515,7 +52,7 @@ static int dispatch(ScanParams& p, const gdn2_scan_args* a, const ScanPlan& n, b
   p.sets = n.sets; p.steps = n.steps; p.segments = n.segments;
   if (w.bytes) {
     char* at = static_cast<char*>(ws);
-    p.maps = reinterpret_cast<float2*>(at);
+    p.maps = reinterpret_cast<ulonglong2*>(at);
     p.map_cuts = reinterpret_cast<int*>(at + w.cuts);
     if (!bwd && p.state_in && p.state_in == p.state_out) {
       int rc = check_cuda(cudaMemcpyAsync(at + w.states, p.state_in, (size_t)p.B * p.C * sizeof(float),
@@ -525,9 +62,9 @@ static int dispatch(ScanParams& p, const gdn2_scan_args* a, const ScanPlan& n, b
     }
   }
   const bool comp = a->complement != 0;
-  if (a->dtype == GDN2_DTYPE_F32) return run_vec<float, float>(p, n, comp, bwd, st, fn);
-  if (a->g_dtype == GDN2_DTYPE_F32) return run_vec<__nv_bfloat16, float>(p, n, comp, bwd, st, fn);
-  return run_vec<__nv_bfloat16, __nv_bfloat16>(p, n, comp, bwd, st, fn);
+  if (a->dtype == GDN2_DTYPE_F32) return run_types<float, float>(p, n, comp, bwd, st, fn);
+  if (a->g_dtype == GDN2_DTYPE_F32) return run_types<__nv_bfloat16, float>(p, n, comp, bwd, st, fn);
+  return run_types<__nv_bfloat16, __nv_bfloat16>(p, n, comp, bwd, st, fn);
 }
 
 static int check_scan(const gdn2_scan_args* a, const char* fn) {
@@ -554,20 +91,17 @@ static void fill(ScanParams& p, const gdn2_scan_args* a) {
   p.carry = a->carry;
 }
 
-// The plan by the rows' alignment; outputs need pairs, inputs 16 bytes for the copies.
 static ScanPlan plan_fwd(const gdn2_scan_args* a, const gdn2_view& h) {
   const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * ex, ex) && rows_ok(a->g, 2 * eg, eg) && rows_ok(h, 2 * ex, ex);
-  return plan_scan(a, pairs, a->channels * ex % 16 == 0 && rows_ok(a->x, 16, ex) && rows_ok(a->g, 16, eg));
+  const RowTensor t[] = {{&a->x, ex, true}, {&a->g, eg, true}, {&h, ex, false}};
+  return plan_scan(a, row_mode(a->channels, t, 3));
 }
 
 static ScanPlan plan_bwd(const gdn2_scan_bwd_args* q) {
   const gdn2_scan_args* a = &q->fwd;
   const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
-  const bool pairs = a->channels % 2 == 0 && rows_ok(a->x, 2 * ex, ex) && rows_ok(a->g, 2 * eg, eg) &&
-                     rows_ok(q->d_h, 2 * ex, ex) && rows_ok(q->dx, 2 * ex, ex) && rows_ok(q->dg, 2 * eg, eg);
-  return plan_scan(a, pairs, a->channels * ex % 16 == 0 && rows_ok(a->x, 16, ex) && rows_ok(a->g, 16, eg) &&
-                                 rows_ok(q->d_h, 16, ex));
+  const RowTensor t[] = {{&a->x, ex, true}, {&a->g, eg, true}, {&q->d_h, ex, true}, {&q->dx, ex, false}, {&q->dg, eg, false}};
+  return plan_scan(a, row_mode(a->channels, t, 5));
 }
 
 size_t scan_workspace_bytes(const gdn2_scan_args* a, const gdn2_view& h) {

@@ -1,212 +1,494 @@
-// Pieces shared by the sequence operators (gated scan, causal convolution,
-// group norm): vector access to rows of channels, staged rows, packed-sequence
-// lookup and the decay's exponential.
+// Gated scan: the diagonal gated linear recurrence
+//
+//   h_t = e^{g_t} h_{t-1} + s_t x_t        s_t = 1, or 1 - e^{g_t} (complement)
+//
+// per channel of [B][T][C] (or of packed sequences), and its adjoint
+//
+//   l_t = dh_t + e^{g_{t+1}} l_{t+1},  dx_t = s_t l_t,
+//   dg_t = e^{g_t} (h_{t-1} [- x_t]) l_t,  dstate = e^{g_0} l_0.
+//
+// Both are bound by HBM with the issue rate close behind (some twenty
+// instructions for 8 to 14 bytes a value): a forward reads x and g and writes
+// h, a backward reads x, g and dh and writes dx and dg.  So each value is
+// read once and its decay computed once, between the load and the store, in
+// packed pairs of channels: a warp holds RUN tokens of 64 channels in
+// registers, reduces them to the affine map c -> A c + H of the run, the maps of
+// a block's runs are joined through shared memory, and the block walks its
+// channels' time axis, the loads of the next step in flight meanwhile.
+//
+// With few chains (sequences times sets of channels) the time axis is cut
+// into segments as well: a first launch reduces every segment to its map, the
+// second starts each segment from the maps before it.  That reads the inputs
+// twice, and pays below about 100 chains, where one block each would leave
+// the memory system idle.  The joining order is fixed by the sizes: results
+// do not depend on timing.
 #pragma once
 
-#include "common.cuh"
-#include "ptx.cuh"
+#include "sequence.cuh"
 
 namespace gdn2 {
 
-// VEC consecutive elements of T as one memory access of sizeof(T) * VEC bytes.
-template <int BYTES>
-struct RawOf;
-template <>
-struct RawOf<2> { typedef unsigned short type; };
-template <>
-struct RawOf<4> { typedef unsigned type; };
-template <>
-struct RawOf<8> { typedef uint2 type; };
-template <>
-struct RawOf<16> { typedef uint4 type; };
+static_assert(RUN == 16, "the spacing of the states a backward starts from is part of the interface");
+constexpr int MAX_SEGMENTS = 128;
 
-template <typename T, int VEC>
-struct Vec {
-  typedef typename RawOf<(int)sizeof(T) * VEC>::type Raw;
-  static __device__ __forceinline__ Raw load(const T* p) { return __ldcs(reinterpret_cast<const Raw*>(p)); }
-  static __device__ __forceinline__ void unpack(Raw r, float (&f)[VEC]) {
-    T e[VEC];
-    memcpy(e, &r, sizeof(r));
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = to_f32<T>(e[v]);
-  }
-  static __device__ __forceinline__ Raw pack(const float (&f)[VEC]) {
-    T e[VEC];
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) e[v] = from_f32<T>(f[v]);
-    Raw r;
-    memcpy(&r, e, sizeof(r));
-    return r;
-  }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
-    __stcs(reinterpret_cast<Raw*>(p), pack(f));
-  }
+struct ScanParams {
+  int B, T, C;      // dense: B sequences of T; packed: N sequences in T rows
+  int sets;         // sets of 64 channels
+  int steps;        // tiles of a segment
+  int segments;
+  const int* cu;
+  DView x, g, h;    // forward: h out.  backward: h = dh
+  DView dx, dg;
+  const float* state_in;
+  float* state_out;
+  const float* d_state_out;
+  float* d_state_in;
+  float* carry;     // [B or 1][ceil(T / RUN)][C]: state before every RUN-th token
+  ulonglong2* maps; // [chain][segment][32 lanes] maps of the segments, or null (one segment)
+  int* map_cuts;    // [chain][segment]: a sequence begins (adjoint: ends) in the segment
 };
 
-// A vector as pairs of f32 (one pair with a zero for VEC = 1).
-template <typename T, int VEC>
-__device__ __forceinline__ void unpack_pairs(typename Vec<T, VEC>::Raw r, f32x2 (&f)[VEC == 1 ? 1 : VEC / 2]) {
-  float v[VEC == 1 ? 2 : VEC];
-  v[VEC == 1 ? 1 : 0] = 0.f;
-  Vec<T, VEC>::unpack(r, *reinterpret_cast<float (*)[VEC]>(v));
-  #pragma unroll
-  for (int i = 0; i < (VEC == 1 ? 1 : VEC / 2); ++i) f[i] = f2pk(v[2 * i], v[2 * i + 1]);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_pairs(T* p, const f32x2 (&f)[VEC == 1 ? 1 : VEC / 2]) {
-  float v[VEC == 1 ? 2 : VEC];
-  #pragma unroll
-  for (int i = 0; i < (VEC == 1 ? 1 : VEC / 2); ++i) f2un(f[i], v[2 * i], v[2 * i + 1]);
-  Vec<T, VEC>::store(p, *reinterpret_cast<const float (*)[VEC]>(v));
-}
+// The maps of a step's runs, twice for alternating steps.  cut: a sequence
+// begins (adjoint: ends) in the run, so that nothing from before it comes
+// through, not even an infinity or NaN times zero.
+template <int NW>
+struct ScanMaps {
+  ulonglong2 run[2][NW][32];  // (A, H) pairs
+  int cut[2][NW];
+};
 
-// Sigmoid of a pair: 1 / (1 + 2^(-t log2 e)) by the approximate exponential
-// and reciprocal (2 ulp and 1 ulp), far below the rounding of a bf16 result
-// and near f32's own.
-__device__ __forceinline__ f32x2 sigmoid2(f32x2 t) {
-  float e0, e1;
-  f2un(f2mul(t, f2pk(-1.44269504088896f, -1.44269504088896f)), e0, e1);
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e0));
-  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e1));
-  f2un(f2add(f2pk(e0, e1), f2pk(1.f, 1.f)), e0, e1);
-  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
-  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
-  return f2pk(e0, e1);
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_f32(const float* p, float (&f)[VEC]) {
+// From the state `c` before the step's first token (after its last, in the
+// adjoint), the state before this warp's run; c becomes the state after the
+// step, and the maps join to `A` of the whole (with SUM).
+template <int NW, bool PACKED, bool SUM>
+__device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int lane, f32x2 A, f32x2 H, bool cut,
+                                      f32x2& c, f32x2& all, bool& any_cut) {
+  sh.run[buf][warp][lane] = make_ulonglong2(A, H);
+  if (PACKED && lane == 0) sh.cut[buf][warp] = cut;
+  __syncthreads();
+  f32x2 cin = c;
   #pragma unroll
-  for (int v = 0; v < VEC; ++v) f[v] = p[v];
-}
-template <int VEC>
-__device__ __forceinline__ void store_f32(float* p, const float (&f)[VEC]) {
-  #pragma unroll
-  for (int v = 0; v < VEC; ++v) p[v] = f[v];
-}
-
-// Sequence of packed row t: the n with cu[n] <= t < cu[n + 1], or -1 for a
-// row outside every sequence.  Reads cu[0..N] only, whatever it holds, and
-// takes at most 32 halvings.
-__device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int N, int t) {
-  int lo = 0, hi = N + 1;  // first index whose entry is above t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid + 1;
-    else hi = mid;
+  for (int w = 0; w < NW; ++w) {
+    if (w == warp) cin = c;
+    const ulonglong2 m = sh.run[buf][w][lane];
+    const bool stop = PACKED && sh.cut[buf][w];
+    c = stop ? m.y : f2fma(m.x, c, m.y);
+    if (SUM) {
+      all = f2mul(all, m.x);
+      any_cut |= stop;
+    }
   }
-  return lo >= 1 && lo <= N ? lo - 1 : -1;
+  return cin;
 }
 
-// a = e^g and k = 1 - e^g of two log decays.  Argument reduction by powers of
-// two (Cody and Waite): g = n ln 2 + r with |r| <= ln 2 / 2, p = e^r - 1 by its
-// Taylor polynomial to r^7 (its first dropped term is below 2^-25 of p), then
-// a = 2^n (1 + p), k = (1 - 2^n) - 2^n p.  For n = 0 (the slow channels, whose
-// decay is applied thousands of times) a is 1 + p rounded once and k is -p
-// itself, without the cancellation of 1 - a: an ulp of bias in a would grow
-// by the length of the channel's memory.  Valid for |g| <= 87; NaN stays NaN.
-template <bool WITH_K>
-__device__ __forceinline__ void exp_pair(f32x2 g, f32x2& a, f32x2& k) {
-  const f32x2 kLog2e = f2pk(1.44269504088896f, 1.44269504088896f);
-  const f32x2 kMagic = f2pk(12582912.f, 12582912.f);  // 1.5 * 2^23: its sum rounds to a whole number
-  const f32x2 kOne = f2pk(1.f, 1.f), kMinus = f2pk(-1.f, -1.f);
-  const f32x2 t = f2fma(g, kLog2e, kMagic);
-  const f32x2 n = f2fma(kMagic, kMinus, t);
-  f32x2 r = f2fma(n, f2pk(-0.693145751953125f, -0.693145751953125f), g);
-  r = f2fma(n, f2pk(-1.42860677e-6f, -1.42860677e-6f), r);
-  f32x2 q = f2fma(r, f2pk(1.f / 5040, 1.f / 5040), f2pk(1.f / 720, 1.f / 720));
-  q = f2fma(q, r, f2pk(1.f / 120, 1.f / 120));
-  q = f2fma(q, r, f2pk(1.f / 24, 1.f / 24));
-  q = f2fma(q, r, f2pk(1.f / 6, 1.f / 6));
-  q = f2fma(q, r, f2pk(0.5f, 0.5f));
-  const f32x2 p = f2fma(f2mul(r, r), q, r);
-  float t0, t1;
-  f2un(t, t0, t1);
-  const f32x2 s = f2pk(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u),
-                       __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
-  a = f2fma(s, p, s);
-  if constexpr (WITH_K) k = f2fma(f2mul(s, kMinus), p, f2fma(s, kMinus, kOne));
-}
-constexpr float kExpRange = 87.f;
-
-constexpr int RUN = 16;     // tokens of a warp's run
-constexpr int STAGES = 2;   // runs in flight or in use
-
-// One warp's staged rows, [RUN][32 * VEC] of T.  Copied 16 bytes a lane over
-// several rows where rows allow it (COOP: few instructions; lanes read what
-// others copied), else each lane its own values.
-template <typename T, int VEC, bool COOP>
-struct Rows {
-  static constexpr int ROW = 32 * VEC * (int)sizeof(T), BYTES = RUN * ROW;
-  unsigned char* base;
-  // rows t0 .. of p (its lane 0 channel), those below T, channels below `left`
-  __device__ __forceinline__ void fetch(const T* p, int64_t stride, int t0, int T_, int left, int lane) const {
-    if constexpr (COOP) {
-      constexpr int LANES = ROW / 16, AT_ONCE = 32 / LANES;  // lanes of a row, rows at once
-      const int c = lane % LANES * (16 / (int)sizeof(T)), r = lane / LANES;
-      const T* q = p + (int64_t)(t0 + r) * stride + c;
+// Decays of a run: a = e^g, and k = 1 - e^g where it is wanted.
+template <bool COMP, typename View>
+__device__ __forceinline__ void decays(const View& rows, f32x2 (&a)[RUN], f32x2 (&k)[RUN]) {
+  float far = 0.f;
+  #pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const f32x2 g = rows.get(i);
+    float g0, g1;
+    f2un(g, g0, g1);
+    far = fmaxf(far, fmaxf(fabsf(g0), fabsf(g1)));
+    exp_pair<COMP>(g, a[i], k[i]);
+  }
+  if (far > kExpRange) {  // a reset (-inf), a decay below every f32, or growth
+    #pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      float g[2], e[2], m[2];
+      f2un(rows.get(i), g[0], g[1]);
+      f2un(a[i], e[0], e[1]);
+      if (COMP) f2un(k[i], m[0], m[1]);
       #pragma unroll
-      for (int i = 0; i < RUN; i += AT_ONCE) {
-        const bool in = c < left && t0 + r + i < T_;
-        cp_async_zfill<16>(base + (i + r) * ROW + lane % LANES * 16, in ? q : p, in);
-        q += AT_ONCE * stride;
+      for (int v = 0; v < 2; ++v)
+        if (fabsf(g[v]) > kExpRange) {
+          e[v] = expf(g[v]);
+          m[v] = -expm1f(g[v]);
+        }
+      a[i] = f2pk(e[0], e[1]);
+      if (COMP) k[i] = f2pk(m[0], m[1]);
+    }
+  }
+}
+
+// Which of a run's tokens open or close a sequence or lie in one, one bit a
+// token; seq: the sequence of token `lane`.
+struct RunMasks {
+  unsigned start, last, valid;
+  int seq;
+  __device__ __forceinline__ int sequence(int i) const { return __shfl_sync(0xffffffffu, seq, i); }
+};
+__device__ __forceinline__ RunMasks run_masks(const int* __restrict__ cu, int N, int T, int t0, int lane) {
+  RunMasks k;
+  const int t = t0 + lane;
+  k.seq = -1;
+  bool s = false, l = false;
+  if (lane < RUN && t < T) {
+    k.seq = find_sequence(cu, N, t);
+    if (k.seq >= 0) {
+      s = __ldg(cu + k.seq) == t;
+      l = t + 1 == T || __ldg(cu + k.seq + 1) == t + 1;
+    }
+  }
+  k.start = __ballot_sync(0xffffffffu, s);
+  k.last = __ballot_sync(0xffffffffu, l);
+  k.valid = __ballot_sync(0xffffffffu, k.seq >= 0);
+  return k;
+}
+
+// Empty sequences hand their state (its gradient) through.
+template <RowMode MODE>
+__device__ __forceinline__ void pass_empty(const ScanParams& p, const float* from, float* to, const Pair<MODE>& ch, int base) {
+  const int lane = threadIdx.x & 31;
+  for (int n0 = (int)threadIdx.x - lane; n0 < p.B; n0 += blockDim.x) {
+    const int n = n0 + lane;
+    unsigned empty = __ballot_sync(0xffffffffu, n < p.B && is_empty(p.cu, n, p.T));
+    while (empty) {
+      const int64_t at = (int64_t)(n0 + __ffs(empty) - 1) * p.C + base;
+      empty &= empty - 1;
+      if (ch.on0) ch.store_state(to + at, from ? ch.load(from + at) : f2pk(0.f, 0.f));
+    }
+  }
+}
+
+// The state before segment `seg` (adjoint: after it): `c` through the maps of
+// the segments before (after) it.
+template <bool PACKED>
+__device__ __forceinline__ f32x2 through_segments(const ScanParams& p, int64_t chain, int seg, int lane, f32x2 c) {
+  const ulonglong2* m = p.maps + chain * p.segments * 32 + lane;
+  const int* cut = p.map_cuts + chain * p.segments;
+  #pragma unroll 8
+  for (int s = 0; s < seg; ++s) {
+    const ulonglong2 v = m[s * 32];
+    c = PACKED && cut[s] ? v.y : f2fma(v.x, c, v.y);
+  }
+  return c;
+}
+template <bool PACKED>
+__device__ __forceinline__ void write_map(const ScanParams& p, int64_t chain, int seg, f32x2 A, f32x2 H, bool cut) {
+  if (threadIdx.x < 32) p.maps[(chain * p.segments + seg) * 32 + threadIdx.x] = make_ulonglong2(A, H);
+  if (PACKED && threadIdx.x == 0) p.map_cuts[chain * p.segments + seg] = cut;
+}
+
+// MAPS: only the segment's map, for the first of two launches.
+template <typename TX, typename TG, RowMode MODE, int NW, bool COMP, bool PACKED, bool MAPS>
+__global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
+  typedef Rows<TX, MODE> RX;
+  typedef Rows<TG, MODE> RG;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ ScanMaps<NW> sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int seg = (int)(blockIdx.x % p.segments);
+  const int64_t chain = blockIdx.x / p.segments;
+  const int b = PACKED ? 0 : (int)(chain / p.sets);
+  const int base = (int)(chain % p.sets) * SET;
+  const Pair<MODE> ch(lane, p.C - base);
+  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
+  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
+  TX* h = static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + base;
+  const int runs = (p.T + RUN - 1) / RUN;
+
+  if (PACKED && !MAPS && p.state_out && seg == 0) pass_empty(p, p.state_in, p.state_out, ch, base);
+  if (!p.steps) return;
+  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
+  bool any_cut = false;
+  if (!MAPS) {
+    if (!PACKED && p.state_in) c = ch.load(p.state_in + (int64_t)b * p.C + base);
+    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
+  }
+
+  constexpr int STAGE = RX::BYTES + RG::BYTES;
+  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
+  auto run_at = [&](int step) { return ((seg * p.steps + step) * NW + warp) * RUN; };
+  auto fetch = [&](int step) {
+    if (step < p.steps) {
+      RX{stage(step)}.fetch(x, p.x.s1, run_at(step), p.T, p.C - base, lane);
+      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, run_at(step), p.T, p.C - base, lane);
+    }
+    cp_async_commit();
+  };
+  for (int step = 0; step < STAGES - 1; ++step) fetch(step);
+  for (int step = 0; step < p.steps; ++step) {
+    __syncwarp();
+    fetch(step + STAGES - 1);
+    const int t0 = run_at(step);
+    RunMasks k;
+    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const auto xs = RX{stage(step)}.view(x, p.x.s1, t0, lane);
+    const auto gs = RG{stage(step) + RX::BYTES}.view(g, p.g.s1, t0, lane);
+
+    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run (after the
+    // run's last cut, a[i] has no meaning)
+    f32x2 a[RUN], u[RUN], A = f2pk(1.f, 1.f), H = f2pk(0.f, 0.f);
+    decays<COMP>(gs, a, u);
+    const unsigned cuts = PACKED ? (k.start | ~k.valid) & ((1u << RUN) - 1) : 0;
+    #pragma unroll
+    for (int i = 0; i < RUN; ++i) {
+      const f32x2 in = COMP ? f2mul(u[i], xs.get(i)) : xs.get(i);
+      if (PACKED && ((cuts >> i) & 1)) {
+        const int n = k.sequence(i);
+        f32x2 st = f2pk(0.f, 0.f);
+        if ((k.start >> i) & 1) {
+          if (p.state_in) st = ch.load(p.state_in + (int64_t)n * p.C + base);
+          H = f2fma(a[i], st, in);
+        } else {
+          H = st;
+        }
+      } else {
+        H = f2fma(a[i], H, in);
+        A = f2mul(A, a[i]);
       }
-    } else {
-      typedef typename Vec<T, VEC>::Raw Raw;
-      const T* q = p + (int64_t)t0 * stride + lane * VEC;
+      a[i] = A;
+      u[i] = H;
+    }
+    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cuts != 0, c, all, any_cut);
+    if (MAPS) continue;
+
+    const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
+    if (ch.on0 && t0 < p.T) {
+      if (p.carry) ch.store_state(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + base, cin);
+      TX* out = h + (int64_t)t0 * p.h.s1;
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        if (!PACKED || i < first_cut) u[i] = f2fma(a[i], cin, u[i]);
+      if (t0 + RUN <= p.T) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i, out += p.h.s1) ch.store(out, u[i]);
+      } else {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i, out += p.h.s1)
+          if (t0 + i < p.T) ch.store(out, u[i]);
+      }
+    }
+    if (PACKED && p.state_out && k.last) {
       #pragma unroll
       for (int i = 0; i < RUN; ++i) {
-        const bool in = lane * VEC < left && t0 + i < T_;
-        Raw* to = reinterpret_cast<Raw*>(base + i * ROW) + lane;
-        if constexpr (sizeof(Raw) >= 4) cp_async_zfill<(int)sizeof(Raw)>(to, in ? q : p, in);
-        else *to = in ? Vec<T, VEC>::load(q) : Raw{};
-        q += stride;
+        if (!((k.last >> i) & 1)) continue;
+        const int n = k.sequence(i);
+        if (ch.on0) ch.store_state(p.state_out + (int64_t)n * p.C + base, u[i]);
       }
     }
   }
-  // a lane's channels of row i as a pair (the second zero for VEC = 1)
-  __device__ __forceinline__ f32x2 get(int i, int lane) const {
-    float f[2] = {0.f, 0.f};
-    const T* p = reinterpret_cast<const T*>(base + i * ROW) + lane * VEC;
-    if constexpr (VEC == 2) Vec<T, 2>::unpack(*reinterpret_cast<const typename Vec<T, 2>::Raw*>(p), f);
-    else f[0] = to_f32<T>(*p);
-    return f2pk(f[0], f[1]);
+  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
+  else if (!PACKED && p.state_out && seg == p.segments - 1 && warp == 0 && ch.on0)
+    ch.store_state(p.state_out + (int64_t)b * p.C + base, c);
+}
+
+// The adjoint, walked from the last tile to the first; warp 0 takes a step's
+// latest run, segment 0 the latest segment.  States inside a run are rebuilt
+// from the state that the forward kept before it.
+template <typename TX, typename TG, RowMode MODE, int NW, bool COMP, bool PACKED, bool MAPS>
+__global__ void __launch_bounds__(32 * NW) k_scan_bwd(const ScanParams p) {
+  typedef Rows<TX, MODE> RX;
+  typedef Rows<TG, MODE> RG;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ ScanMaps<NW> sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int seg = (int)(blockIdx.x % p.segments);
+  const int64_t chain = blockIdx.x / p.segments;
+  const int b = PACKED ? 0 : (int)(chain / p.sets);
+  const int base = (int)(chain % p.sets) * SET;
+  const Pair<MODE> ch(lane, p.C - base);
+  const TX* x = static_cast<const TX*>(p.x.p) + b * p.x.s0 + base;
+  const TG* g = static_cast<const TG*>(p.g.p) + b * p.g.s0 + base;
+  const TX* dh = static_cast<const TX*>(p.h.p) + b * p.h.s0 + base;
+  TX* dx = static_cast<TX*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + base;
+  TG* dg = static_cast<TG*>(const_cast<void*>(p.dg.p)) + b * p.dg.s0 + base;
+  const int runs = (p.T + RUN - 1) / RUN;
+
+  if (PACKED && !MAPS && p.d_state_in && seg == 0) pass_empty(p, p.d_state_out, p.d_state_in, ch, base);
+  if (!p.steps) return;
+  f32x2 c = f2pk(0.f, 0.f), all = f2pk(1.f, 1.f);
+  bool any_cut = false;
+  if (!MAPS) {
+    if (!PACKED && p.d_state_out) c = ch.load(p.d_state_out + (int64_t)b * p.C + base);
+    if (p.maps) c = through_segments<PACKED>(p, chain, seg, lane, c);
   }
+
+  constexpr int STAGE = 2 * RX::BYTES + RG::BYTES;
+  auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
+  auto run_at = [&](int step) { return ((p.segments * p.steps - 1 - (seg * p.steps + step)) * NW + NW - 1 - warp) * RUN; };
+  f32x2 next_state = f2pk(0.f, 0.f);  // state before the next step's run
+  auto fetch = [&](int step) {
+    if (step < p.steps) {
+      const int t0 = run_at(step);
+      RX{stage(step)}.fetch(dh, p.h.s1, t0, p.T, p.C - base, lane);
+      RG{stage(step) + RX::BYTES}.fetch(g, p.g.s1, t0, p.T, p.C - base, lane);
+      if (!MAPS) RX{stage(step) + RX::BYTES + RG::BYTES}.fetch(x, p.x.s1, t0, p.T, p.C - base, lane);
+      if (!MAPS && t0 < p.T) next_state = ch.load(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + base);
+    }
+    cp_async_commit();
+  };
+  static_assert(STAGES == 2, "next_state is one step ahead");
+  fetch(0);
+  for (int step = 0; step < p.steps; ++step) {
+    __syncwarp();
+    f32x2 hp = next_state;
+    fetch(step + 1);
+    const int t0 = run_at(step);
+    RunMasks k;
+    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const auto ds = RX{stage(step)}.view(dh, p.h.s1, t0, lane);
+    const auto gs = RG{stage(step) + RX::BYTES}.view(g, p.g.s1, t0, lane);
+    const auto xs = RX{stage(step) + RX::BYTES + RG::BYTES}.view(x, p.x.s1, t0, lane);
+
+    // a[i]: decay of token i; w[i]: what dg multiplies, h_{i-1} or h_{i-1} - x_i
+    f32x2 a[RUN], m[RUN], w[RUN];
+    decays<COMP && !MAPS>(gs, a, m);
+    if (!MAPS) {
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        const f32x2 xf = xs.get(i);
+        if (PACKED && ((k.start >> i) & 1)) {
+          const int n = k.sequence(i);
+          hp = p.state_in ? ch.load(p.state_in + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
+        }
+        w[i] = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
+        hp = f2fma(a[i], hp, COMP ? f2mul(m[i], xf) : xf);
+      }
+    }
+    // the run's map from the adjoint after it to the adjoint before it
+    const unsigned cuts = PACKED ? (k.last | ~k.valid) & ((1u << RUN) - 1) : 0;
+    f32x2 A = f2pk(1.f, 1.f), M = f2pk(0.f, 0.f);
+    #pragma unroll
+    for (int i = RUN - 1; i >= 0; --i) {
+      if (PACKED && ((cuts >> i) & 1)) {
+        const int n = k.sequence(i);
+        M = f2pk(0.f, 0.f);
+        if ((k.last >> i) & 1) {
+          if (p.d_state_out) M = ch.load(p.d_state_out + (int64_t)n * p.C + base);
+          M = f2mul(a[i], f2add(ds.get(i), M));
+        }
+      } else {
+        M = f2mul(a[i], f2add(ds.get(i), M));
+        A = f2mul(A, a[i]);
+      }
+    }
+    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cuts != 0, c, all, any_cut);
+    if (MAPS) continue;
+
+    TX* ox = dx + (int64_t)(t0 + RUN - 1) * p.dx.s1;
+    TG* og = dg + (int64_t)(t0 + RUN - 1) * p.dg.s1;
+    #pragma unroll
+    for (int i = RUN - 1; i >= 0; --i) {
+      const bool out = PACKED && !((k.valid >> i) & 1);
+      if (PACKED && ((k.last >> i) & 1)) {
+        const int n = k.sequence(i);
+        mu = p.d_state_out ? ch.load(p.d_state_out + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
+      }
+      const f32x2 l = f2add(ds.get(i), mu);
+      f32x2 vx = COMP ? f2mul(m[i], l) : l;
+      mu = f2mul(a[i], l);
+      f32x2 vg = f2mul(mu, w[i]);
+      if (out) vx = vg = mu = f2pk(0.f, 0.f);
+      if (ch.on0 && t0 + i < p.T) {
+        ch.store(ox, vx);
+        ch.store(og, vg);
+      }
+      ox -= p.dx.s1;
+      og -= p.dg.s1;
+      if (PACKED && p.d_state_in && ((k.start >> i) & 1)) {
+        const int n = k.sequence(i);
+        if (ch.on0) ch.store_state(p.d_state_in + (int64_t)n * p.C + base, mu);
+      }
+    }
+  }
+  if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
+  else if (!PACKED && p.d_state_in && seg == p.segments - 1 && warp == 0 && ch.on0)
+    ch.store_state(p.d_state_in + (int64_t)b * p.C + base, c);
+}
+
+// One token per sequence, the decode step: elementwise, state read and
+// written once.  One thread per VEC channels of a sequence.
+template <typename TX, typename TG, int VEC, bool COMP>
+__global__ void __launch_bounds__(256) k_scan_step(const ScanParams p) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = p.C / VEC;
+  if (e >= (int64_t)p.B * per) return;
+  const int64_t b = e / per;
+  const int c0 = (int)(e % per) * VEC;
+  float g[VEC], x[VEC], s[VEC] = {};
+  Vec<TG, VEC>::unpack(Vec<TG, VEC>::load(static_cast<const TG*>(p.g.p) + b * p.g.s0 + c0), g);
+  Vec<TX, VEC>::unpack(Vec<TX, VEC>::load(static_cast<const TX*>(p.x.p) + b * p.x.s0 + c0), x);
+  if (p.state_in) load_f32<VEC>(p.state_in + b * p.C + c0, s);
+  #pragma unroll
+  for (int v = 0; v < VEC; ++v) s[v] = fmaf(expf(g[v]), s[v], COMP ? -expm1f(g[v]) * x[v] : x[v]);
+  if (p.state_out) store_f32<VEC>(p.state_out + b * p.C + c0, s);
+  Vec<TX, VEC>::store(static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + c0, s);
+}
+
+// ---- host: the kernels of one pair of types (one source file each, compiled side by side) ----
+
+// How a call is cut up: how rows are held, warps (runs) of a block, segments of the time axis.
+struct ScanPlan {
+  RowMode mode;
+  int warps, sets, steps, segments;
+  int64_t chains;
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void put(T* p, f32x2 v) {
-  float f[2];
-  f2un(v, f[0], f[1]);
-  if constexpr (VEC == 2) Vec<T, 2>::store(p, f);
-  else {
-    float one[1] = {f[0]};
-    Vec<T, 1>::store(p, one);
+template <typename K>
+static int launch(K kernel, const ScanParams& p, const ScanPlan& n, int stage, cudaStream_t st, const char* fn) {
+  const int64_t grid = n.chains * n.segments;
+  if (grid > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: %lld blocks", fn, (long long)grid);
+  const int smem = STAGES * n.warps * stage;
+  int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
+  if (rc) return rc;
+  kernel<<<(unsigned)grid, 32 * n.warps, smem, st>>>(p);
+  return check_cuda(cudaGetLastError(), fn);
+}
+
+template <typename TX, typename TG, RowMode MODE, bool COMP, bool PACKED>
+static int run_scan(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  const int rx = Rows<TX, MODE>::BYTES, rg = Rows<TG, MODE>::BYTES, stage = bwd ? 2 * rx + rg : rx + rg;
+  if (n.warps == 8)
+    return bwd ? launch(k_scan_bwd<TX, TG, MODE, 8, COMP, PACKED, false>, p, n, stage, st, fn)
+               : launch(k_scan_fwd<TX, TG, MODE, 8, COMP, PACKED, false>, p, n, stage, st, fn);
+  if (n.segments > 1) {
+    int rc = bwd ? launch(k_scan_bwd<TX, TG, MODE, 4, COMP, PACKED, true>, p, n, stage, st, fn)
+                 : launch(k_scan_fwd<TX, TG, MODE, 4, COMP, PACKED, true>, p, n, stage, st, fn);
+    if (rc) return rc;
   }
-}
-template <int VEC>
-__device__ __forceinline__ f32x2 get_f32(const float* p) {
-  return f2pk(p[0], VEC == 2 ? p[VEC - 1] : 0.f);
-}
-template <int VEC>
-__device__ __forceinline__ void put_f32(float* p, f32x2 v) {
-  float f0, f1;
-  f2un(v, f0, f1);
-  p[0] = f0;
-  if (VEC == 2) p[VEC - 1] = f1;
+  return bwd ? launch(k_scan_bwd<TX, TG, MODE, 4, COMP, PACKED, false>, p, n, stage, st, fn)
+             : launch(k_scan_fwd<TX, TG, MODE, 4, COMP, PACKED, false>, p, n, stage, st, fn);
 }
 
-// Whether packed sequence n has no row.  Offsets beyond the T rows count as T.
-__device__ __forceinline__ bool is_empty(const int* __restrict__ cu, int n, int T) {
-  const int from = __ldg(cu + n);
-  return __ldg(cu + n + 1) <= from || from >= T;
+template <typename TX, typename TG, bool COMP>
+static int run_step(const ScanParams& p, bool pairs, cudaStream_t st, const char* fn) {
+  const int64_t count = ((int64_t)p.B * (p.C / (pairs ? 2 : 1)) + 255) / 256;
+  if (count > 0x7fffffffll) return set_error(GDN2_EUNSUPPORTED, "%s: too many channels", fn);
+  if (pairs) k_scan_step<TX, TG, 2, COMP><<<(unsigned)count, 256, 0, st>>>(p);
+  else k_scan_step<TX, TG, 1, COMP><<<(unsigned)count, 256, 0, st>>>(p);
+  return check_cuda(cudaGetLastError(), fn);
 }
 
-// Rows of v start on `bytes` boundaries.
-inline bool rows_ok(const gdn2_view& v, int bytes, int elem) {
-  return (uintptr_t)v.data % bytes == 0 && v.stride0 * elem % bytes == 0 && v.stride1 * elem % bytes == 0;
+template <typename TX, typename TG, bool COMP>
+static int run_mode(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
+  if (p.T == 1 && !p.cu && !p.carry && !bwd)
+    return run_step<TX, TG, COMP>(p, n.mode == ROWS16 || n.mode == ROWS_PAIR, st, fn);
+  if (p.cu)
+    return n.mode == ROWS16      ? run_scan<TX, TG, ROWS16, COMP, true>(p, n, bwd, st, fn)
+           : n.mode == ROWS_PAIR ? run_scan<TX, TG, ROWS_PAIR, COMP, true>(p, n, bwd, st, fn)
+           : n.mode == ROWS_ODD  ? run_scan<TX, TG, ROWS_ODD, COMP, true>(p, n, bwd, st, fn)
+                                 : run_scan<TX, TG, ROWS_ANY, COMP, true>(p, n, bwd, st, fn);
+  return n.mode == ROWS16      ? run_scan<TX, TG, ROWS16, COMP, false>(p, n, bwd, st, fn)
+         : n.mode == ROWS_PAIR ? run_scan<TX, TG, ROWS_PAIR, COMP, false>(p, n, bwd, st, fn)
+         : n.mode == ROWS_ODD  ? run_scan<TX, TG, ROWS_ODD, COMP, false>(p, n, bwd, st, fn)
+                               : run_scan<TX, TG, ROWS_ANY, COMP, false>(p, n, bwd, st, fn);
 }
 
-inline int elem_bytes(int dtype) { return dtype == GDN2_DTYPE_BF16 ? 2 : 4; }
+// The scan (its adjoint with bwd) of x in TX and g in TG.
+template <typename TX, typename TG>
+int run_types(const ScanParams& p, const ScanPlan& n, bool comp, bool bwd, cudaStream_t st, const char* fn) {
+  return comp ? run_mode<TX, TG, true>(p, n, bwd, st, fn) : run_mode<TX, TG, false>(p, n, bwd, st, fn);
+}
+extern template int run_types<float, float>(const ScanParams&, const ScanPlan&, bool, bool, cudaStream_t, const char*);
+extern template int run_types<__nv_bfloat16, float>(const ScanParams&, const ScanPlan&, bool, bool, cudaStream_t, const char*);
+extern template int run_types<__nv_bfloat16, __nv_bfloat16>(const ScanParams&, const ScanPlan&, bool, bool, cudaStream_t,
+                                                            const char*);
 
 }  // namespace gdn2

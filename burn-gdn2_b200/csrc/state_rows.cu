@@ -11,7 +11,7 @@
 // span of every source into shared memory and writes it only after the last
 // of them has been read, so no order of moves can go wrong; the span is
 // narrowed until all moved rows fit.
-#include "scan.cuh"
+#include "sequence.cuh"
 
 namespace gdn2 {
 
