@@ -4,7 +4,15 @@
 
 namespace gdn2 {
 
-static ScanPlan plan_scan(const gdn2_scan_args* a, RowMode mode) {
+template <typename TX, typename TG>
+static int resident(RowMode mode, bool bwd) {
+  return mode == ROWS16      ? resident_blocks<TX, TG, ROWS16>(4, bwd)
+         : mode == ROWS_PAIR ? resident_blocks<TX, TG, ROWS_PAIR>(4, bwd)
+         : mode == ROWS_ODD  ? resident_blocks<TX, TG, ROWS_ODD>(4, bwd)
+                             : resident_blocks<TX, TG, ROWS_ANY>(4, bwd);
+}
+
+static ScanPlan plan_scan(const gdn2_scan_args* a, RowMode mode, bool bwd) {
   ScanPlan n;
   n.mode = mode;
   n.sets = (a->channels + SET - 1) / SET;
@@ -18,7 +26,12 @@ static ScanPlan plan_scan(const gdn2_scan_args* a, RowMode mode) {
   n.segments = 1;
   n.steps = tiles;
   if (cut) {
-    int64_t want = 148 * 4 / n.chains;
+    // one wave of resident blocks: a second one would walk as long again
+    typedef __nv_bfloat16 bf;
+    const int per_sm = a->dtype == GDN2_DTYPE_F32     ? resident<float, float>(mode, bwd)
+                       : a->g_dtype == GDN2_DTYPE_F32 ? resident<bf, float>(mode, bwd)
+                                                      : resident<bf, bf>(mode, bwd);
+    int64_t want = 148 * per_sm / n.chains;
     want = want < MAX_SEGMENTS ? want : MAX_SEGMENTS;
     want = want < tiles ? want : tiles;
     if (want > 1) {
@@ -94,14 +107,14 @@ static void fill(ScanParams& p, const gdn2_scan_args* a) {
 static ScanPlan plan_fwd(const gdn2_scan_args* a, const gdn2_view& h) {
   const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
   const RowTensor t[] = {{&a->x, ex, true}, {&a->g, eg, true}, {&h, ex, false}};
-  return plan_scan(a, row_mode(a->channels, t, 3));
+  return plan_scan(a, row_mode(a->channels, t, 3), false);
 }
 
 static ScanPlan plan_bwd(const gdn2_scan_bwd_args* q) {
   const gdn2_scan_args* a = &q->fwd;
   const int ex = elem_bytes(a->dtype), eg = elem_bytes(a->g_dtype);
   const RowTensor t[] = {{&a->x, ex, true}, {&a->g, eg, true}, {&q->d_h, ex, true}, {&q->dx, ex, false}, {&q->dg, eg, false}};
-  return plan_scan(a, row_mode(a->channels, t, 5));
+  return plan_scan(a, row_mode(a->channels, t, 5), true);
 }
 
 size_t scan_workspace_bytes(const gdn2_scan_args* a, const gdn2_view& h) {

@@ -48,6 +48,20 @@ struct ScanParams {
   int* map_cuts;    // [chain][segment]: a sequence begins (adjoint: ends) in the segment
 };
 
+// Bytes of a run's staged rows, and blocks that an SM holds: by their shared
+// memory, and by registers 16 warps of a forward (128 a thread) and 12 of a
+// backward (168).
+template <typename TX, typename TG, RowMode MODE>
+constexpr int stage_bytes(bool bwd) {
+  return (bwd ? 2 : 1) * Rows<TX, MODE>::BYTES + Rows<TG, MODE>::BYTES;
+}
+template <typename TX, typename TG, RowMode MODE>
+constexpr int resident_blocks(int warps, bool bwd) {
+  const int smem = warps * (STAGES * stage_bytes<TX, TG, MODE>(bwd) + 1040) + 1024;
+  const int by_smem = 227 * 1024 / smem, by_regs = (bwd ? 12 : 16) / warps;
+  return by_smem < by_regs ? by_smem : by_regs;
+}
+
 // The maps of a step's runs, twice for alternating steps.  cut: a sequence
 // begins (adjoint: ends) in the run, so that nothing from before it comes
 // through, not even an infinity or NaN times zero.
@@ -81,9 +95,11 @@ __device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int l
   return cin;
 }
 
-// Decays of a run: a = e^g, and k = 1 - e^g where it is wanted.
+// Decays of a run: a = e^g, and k = 1 - e^g where it is wanted.  False where
+// some |g| is beyond the range of exp_pair: a reset (-inf), a decay below
+// every f32, or growth.
 template <bool COMP, typename View>
-__device__ __forceinline__ void decays(const View& rows, f32x2 (&a)[RUN], f32x2 (&k)[RUN]) {
+__device__ __forceinline__ bool decays(const View& rows, f32x2 (&a)[RUN], f32x2 (&k)[RUN]) {
   float far = 0.f;
   #pragma unroll
   for (int i = 0; i < RUN; ++i) {
@@ -93,49 +109,68 @@ __device__ __forceinline__ void decays(const View& rows, f32x2 (&a)[RUN], f32x2 
     far = fmaxf(far, fmaxf(fabsf(g0), fabsf(g1)));
     exp_pair<COMP>(g, a[i], k[i]);
   }
-  if (far > kExpRange) {  // a reset (-inf), a decay below every f32, or growth
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      float g[2], e[2], m[2];
-      f2un(rows.get(i), g[0], g[1]);
-      f2un(a[i], e[0], e[1]);
-      if (COMP) f2un(k[i], m[0], m[1]);
-      #pragma unroll
-      for (int v = 0; v < 2; ++v)
-        if (fabsf(g[v]) > kExpRange) {
-          e[v] = expf(g[v]);
-          m[v] = -expm1f(g[v]);
-        }
-      a[i] = f2pk(e[0], e[1]);
-      if (COMP) k[i] = f2pk(m[0], m[1]);
+  return __all_sync(0xffffffffu, far <= kExpRange);
+}
+// One token's, any g.
+template <bool COMP>
+__device__ __forceinline__ void decay_any(f32x2 g, f32x2& a, f32x2& k) {
+  float v[2], e[2], m[2];
+  f2un(g, v[0], v[1]);
+  exp_pair<COMP>(g, a, k);
+  f2un(a, e[0], e[1]);
+  if (COMP) f2un(k, m[0], m[1]);
+  #pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (fabsf(v[i]) > kExpRange) {
+      e[i] = expf(v[i]);
+      m[i] = -expm1f(v[i]);
     }
-  }
+  a = f2pk(e[0], e[1]);
+  if (COMP) k = f2pk(m[0], m[1]);
 }
 
 // Which of a run's tokens open or close a sequence or lie in one, one bit a
-// token; seq: the sequence of token `lane`.
+// token; seq: in lane i the sequence of token i, -1 outside (sequence(i): for all lanes).
+constexpr unsigned ALL = (1u << RUN) - 1;
 struct RunMasks {
   unsigned start, last, valid;
   int seq;
   __device__ __forceinline__ int sequence(int i) const { return __shfl_sync(0xffffffffu, seq, i); }
 };
-__device__ __forceinline__ RunMasks run_masks(const int* __restrict__ cu, int N, int T, int t0, int lane) {
-  RunMasks k;
-  const int t = t0 + lane;
-  k.seq = -1;
-  bool s = false, l = false;
-  if (lane < RUN && t < T) {
-    k.seq = find_sequence(cu, N, t);
-    if (k.seq >= 0) {
-      s = __ldg(cu + k.seq) == t;
-      l = t + 1 == T || __ldg(cu + k.seq + 1) == t + 1;
+// The packed sequence on the far side (token SIDE) of a warp's latest run;
+// most runs lie in that of the run before, and need no search.
+template <int SIDE>
+struct SequenceCursor {
+  int n = -1, from = 0, to = 0;
+  __device__ __forceinline__ RunMasks masks(const int* __restrict__ cu, int N, int T, int t0, int lane) {
+    RunMasks k;
+    if (n >= 0 && t0 >= from && t0 + RUN <= to) {
+      k.start = t0 == from;
+      k.last = t0 + RUN == to ? 1u << (RUN - 1) : 0u;
+      k.valid = ALL;
+      k.seq = n;
+      return k;
     }
+    const int t = t0 + lane;
+    int first = 0, end = 0;
+    k.seq = -1;
+    if (lane < RUN && t < T) {
+      k.seq = find_sequence(cu, N, t);
+      if (k.seq >= 0) {
+        first = __ldg(cu + k.seq);
+        end = __ldg(cu + k.seq + 1);
+        if (end > T) end = T;
+      }
+    }
+    k.start = __ballot_sync(0xffffffffu, k.seq >= 0 && first == t);
+    k.last = __ballot_sync(0xffffffffu, k.seq >= 0 && end == t + 1);
+    k.valid = __ballot_sync(0xffffffffu, k.seq >= 0);
+    n = __shfl_sync(0xffffffffu, k.seq, SIDE);
+    from = __shfl_sync(0xffffffffu, first, SIDE);
+    to = __shfl_sync(0xffffffffu, end, SIDE);
+    return k;
   }
-  k.start = __ballot_sync(0xffffffffu, s);
-  k.last = __ballot_sync(0xffffffffu, l);
-  k.valid = __ballot_sync(0xffffffffu, k.seq >= 0);
-  return k;
-}
+};
 
 // Empty sequences hand their state (its gradient) through.
 template <RowMode MODE>
@@ -173,7 +208,7 @@ __device__ __forceinline__ void write_map(const ScanParams& p, int64_t chain, in
 
 // MAPS: only the segment's map, for the first of two launches.
 template <typename TX, typename TG, RowMode MODE, int NW, bool COMP, bool PACKED, bool MAPS>
-__global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
+__global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, false)) k_scan_fwd(const ScanParams p) {
   typedef Rows<TX, MODE> RX;
   typedef Rows<TG, MODE> RG;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -208,68 +243,106 @@ __global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
     }
     cp_async_commit();
   };
+  SequenceCursor<RUN - 1> cursor;
   for (int step = 0; step < STAGES - 1; ++step) fetch(step);
   for (int step = 0; step < p.steps; ++step) {
     __syncwarp();
     fetch(step + STAGES - 1);
     const int t0 = run_at(step);
-    RunMasks k;
-    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    RunMasks k{0, 0, ALL, 0};
+    if (PACKED) k = cursor.masks(p.cu, p.B, p.T, t0, lane);
     cp_async_wait<STAGES - 1>();
     __syncwarp();
     const auto xs = RX{stage(step)}.view(x, p.x.s1, t0, lane);
     const auto gs = RG{stage(step) + RX::BYTES}.view(g, p.g.s1, t0, lane);
+    const unsigned cuts = PACKED ? (k.start | ~k.valid) & ALL : 0;
+    TX* out = h + (int64_t)t0 * p.h.s1;
+    float* carry = p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + base;
 
-    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run (after the
-    // run's last cut, a[i] has no meaning)
+    // a[i]: product of the decays up to token i, u[i]: the state there from a zero one before the run
     f32x2 a[RUN], u[RUN], A = f2pk(1.f, 1.f), H = f2pk(0.f, 0.f);
-    decays<COMP>(gs, a, u);
-    const unsigned cuts = PACKED ? (k.start | ~k.valid) & ((1u << RUN) - 1) : 0;
-    #pragma unroll
-    for (int i = 0; i < RUN; ++i) {
-      const f32x2 in = COMP ? f2mul(u[i], xs.get(i)) : xs.get(i);
-      if (PACKED && ((cuts >> i) & 1)) {
-        const int n = k.sequence(i);
-        f32x2 st = f2pk(0.f, 0.f);
-        if ((k.start >> i) & 1) {
-          if (p.state_in) st = ch.load(p.state_in + (int64_t)n * p.C + base);
-          H = f2fma(a[i], st, in);
-        } else {
-          H = st;
-        }
-      } else {
-        H = f2fma(a[i], H, in);
-        A = f2mul(A, a[i]);
-      }
-      a[i] = A;
-      u[i] = H;
-    }
-    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cuts != 0, c, all, any_cut);
-    if (MAPS) continue;
-
-    const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
-    if (ch.on0 && t0 < p.T) {
-      if (p.carry) ch.store_state(p.carry + (b * (int64_t)runs + t0 / RUN) * p.C + base, cin);
-      TX* out = h + (int64_t)t0 * p.h.s1;
-      #pragma unroll
-      for (int i = 0; i < RUN; ++i)
-        if (!PACKED || i < first_cut) u[i] = f2fma(a[i], cin, u[i]);
-      if (t0 + RUN <= p.T) {
-        #pragma unroll
-        for (int i = 0; i < RUN; ++i, out += p.h.s1) ch.store(out, u[i]);
-      } else {
-        #pragma unroll
-        for (int i = 0; i < RUN; ++i, out += p.h.s1)
-          if (t0 + i < p.T) ch.store(out, u[i]);
-      }
-    }
-    if (PACKED && p.state_out && k.last) {
+    f32x2 la[RUN], lu[RUN];  // the same token by token, where a decay is out of range
+    bool cut = false;
+    const bool plain = decays<COMP>(gs, a, u);
+    if (plain && !cuts) {
       #pragma unroll
       for (int i = 0; i < RUN; ++i) {
-        if (!((k.last >> i) & 1)) continue;
-        const int n = k.sequence(i);
-        if (ch.on0) ch.store_state(p.state_out + (int64_t)n * p.C + base, u[i]);
+        const f32x2 in = COMP ? f2mul(u[i], xs.get(i)) : xs.get(i);
+        H = f2fma(a[i], H, in);
+        A = f2mul(A, a[i]);
+        a[i] = A;
+        u[i] = H;
       }
+    } else {
+      auto token = [&](int i, f32x2 e, f32x2 r, f32x2& product, f32x2& state) {
+        const f32x2 in = COMP ? f2mul(r, xs.get(i)) : xs.get(i);
+        if (PACKED && ((cuts >> i) & 1)) {
+          const int n = k.sequence(i);
+          cut = true;
+          H = f2pk(0.f, 0.f);
+          if ((k.start >> i) & 1) {
+            if (p.state_in) H = ch.load(p.state_in + (int64_t)n * p.C + base);
+            H = f2fma(e, H, in);
+          }
+        } else {
+          H = f2fma(e, H, in);
+          if (!cut) A = f2mul(A, e);
+        }
+        product = A;
+        state = H;
+      };
+      if (PACKED && plain) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) token(i, a[i], u[i], a[i], u[i]);
+      } else {
+        #pragma unroll 1
+        for (int i = 0; i < RUN; ++i) {
+          f32x2 e, r;
+          decay_any<COMP>(gs.get(i), e, r);
+          token(i, e, r, la[i], lu[i]);
+        }
+      }
+    }
+    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, c, all, any_cut);
+    if (MAPS) continue;
+    if (p.carry && ch.on0 && t0 < p.T) ch.store_state(carry, cin);
+    const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
+    if (plain) {
+      if (!cuts) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) u[i] = f2fma(a[i], cin, u[i]);
+      } else {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i)
+          if (i < first_cut) u[i] = f2fma(a[i], cin, u[i]);
+      }
+      if (ch.on0) {
+        if (t0 + RUN <= p.T) {
+          #pragma unroll
+          for (int i = 0; i < RUN; ++i, out += p.h.s1) ch.store(out, u[i]);
+        } else {
+          #pragma unroll
+          for (int i = 0; i < RUN; ++i, out += p.h.s1)
+            if (t0 + i < p.T) ch.store(out, u[i]);
+        }
+      }
+      if (PACKED && p.state_out && k.last) {
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          if (!((k.last >> i) & 1)) continue;
+          const int n = k.sequence(i);
+          if (ch.on0) ch.store_state(p.state_out + (int64_t)n * p.C + base, u[i]);
+        }
+      }
+      continue;
+    }
+    #pragma unroll 1
+    for (int i = 0; i < RUN && t0 + i < p.T; ++i, out += p.h.s1) {
+      const f32x2 v = i < first_cut ? f2fma(la[i], cin, lu[i]) : lu[i];
+      const int n = k.sequence(i);
+      if (!ch.on0) continue;
+      ch.store(out, v);
+      if (PACKED && p.state_out && ((k.last >> i) & 1)) ch.store_state(p.state_out + (int64_t)n * p.C + base, v);
     }
   }
   if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
@@ -281,7 +354,7 @@ __global__ void __launch_bounds__(32 * NW) k_scan_fwd(const ScanParams p) {
 // latest run, segment 0 the latest segment.  States inside a run are rebuilt
 // from the state that the forward kept before it.
 template <typename TX, typename TG, RowMode MODE, int NW, bool COMP, bool PACKED, bool MAPS>
-__global__ void __launch_bounds__(32 * NW) k_scan_bwd(const ScanParams p) {
+__global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, true)) k_scan_bwd(const ScanParams p) {
   typedef Rows<TX, MODE> RX;
   typedef Rows<TG, MODE> RG;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -323,79 +396,126 @@ __global__ void __launch_bounds__(32 * NW) k_scan_bwd(const ScanParams p) {
     cp_async_commit();
   };
   static_assert(STAGES == 2, "next_state is one step ahead");
+  SequenceCursor<0> cursor;
   fetch(0);
   for (int step = 0; step < p.steps; ++step) {
     __syncwarp();
     f32x2 hp = next_state;
     fetch(step + 1);
     const int t0 = run_at(step);
-    RunMasks k;
-    if (PACKED) k = run_masks(p.cu, p.B, p.T, t0, lane);
+    RunMasks k{0, 0, ALL, 0};
+    if (PACKED) k = cursor.masks(p.cu, p.B, p.T, t0, lane);
     cp_async_wait<STAGES - 1>();
     __syncwarp();
     const auto ds = RX{stage(step)}.view(dh, p.h.s1, t0, lane);
     const auto gs = RG{stage(step) + RX::BYTES}.view(g, p.g.s1, t0, lane);
     const auto xs = RX{stage(step) + RX::BYTES + RG::BYTES}.view(x, p.x.s1, t0, lane);
+    const unsigned cuts = PACKED ? (k.last | ~k.valid) & ALL : 0;
+    const int n0 = PACKED ? k.sequence(0) : 0;
+    TX* ox = dx + (int64_t)(t0 + RUN - 1) * p.dx.s1;
+    TG* og = dg + (int64_t)(t0 + RUN - 1) * p.dg.s1;
 
     // a[i]: decay of token i; w[i]: what dg multiplies, h_{i-1} or h_{i-1} - x_i
-    f32x2 a[RUN], m[RUN], w[RUN];
-    decays<COMP && !MAPS>(gs, a, m);
-    if (!MAPS) {
-      #pragma unroll
-      for (int i = 0; i < RUN; ++i) {
-        const f32x2 xf = xs.get(i);
-        if (PACKED && ((k.start >> i) & 1)) {
-          const int n = k.sequence(i);
-          hp = p.state_in ? ch.load(p.state_in + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
-        }
-        w[i] = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
-        hp = f2fma(a[i], hp, COMP ? f2mul(m[i], xf) : xf);
+    f32x2 a[RUN], m[RUN], w[RUN], A = f2pk(1.f, 1.f), M = f2pk(0.f, 0.f);
+    f32x2 la[RUN], lm[RUN], lw[RUN];  // the same token by token, where a decay is out of range
+    bool cut = false;
+    const bool plain = decays<COMP && !MAPS>(gs, a, m);
+    // state after token i, from the one before it; its weight in dg
+    auto forward = [&](int i, f32x2 e, f32x2 r) {
+      const f32x2 xf = xs.get(i);
+      if (PACKED && ((k.start >> i) & 1)) {
+        const int n = k.sequence(i);
+        hp = p.state_in ? ch.load(p.state_in + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
       }
-    }
-    // the run's map from the adjoint after it to the adjoint before it
-    const unsigned cuts = PACKED ? (k.last | ~k.valid) & ((1u << RUN) - 1) : 0;
-    f32x2 A = f2pk(1.f, 1.f), M = f2pk(0.f, 0.f);
-    #pragma unroll
-    for (int i = RUN - 1; i >= 0; --i) {
+      const f32x2 weight = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
+      hp = f2fma(e, hp, COMP ? f2mul(r, xf) : xf);
+      return weight;
+    };
+    // the run's map, extended to the front by token i
+    auto adjoint = [&](int i, f32x2 e) {
       if (PACKED && ((cuts >> i) & 1)) {
         const int n = k.sequence(i);
+        cut = true;
         M = f2pk(0.f, 0.f);
         if ((k.last >> i) & 1) {
           if (p.d_state_out) M = ch.load(p.d_state_out + (int64_t)n * p.C + base);
-          M = f2mul(a[i], f2add(ds.get(i), M));
+          M = f2mul(e, f2add(ds.get(i), M));
         }
       } else {
+        M = f2mul(e, f2add(ds.get(i), M));
+        if (!cut) A = f2mul(A, e);
+      }
+    };
+    if (plain && !cuts) {
+      if (!MAPS) {
+        if (PACKED && k.start)  // at the run's first token, if anywhere
+          hp = p.state_in ? ch.load(p.state_in + (int64_t)n0 * p.C + base) : f2pk(0.f, 0.f);
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          const f32x2 xf = xs.get(i);
+          w[i] = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
+          hp = f2fma(a[i], hp, COMP ? f2mul(m[i], xf) : xf);
+        }
+      }
+      // the run's map from the adjoint after it to the adjoint before it
+      #pragma unroll
+      for (int i = RUN - 1; i >= 0; --i) {
         M = f2mul(a[i], f2add(ds.get(i), M));
         A = f2mul(A, a[i]);
       }
-    }
-    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cuts != 0, c, all, any_cut);
-    if (MAPS) continue;
-
-    TX* ox = dx + (int64_t)(t0 + RUN - 1) * p.dx.s1;
-    TG* og = dg + (int64_t)(t0 + RUN - 1) * p.dg.s1;
-    #pragma unroll
-    for (int i = RUN - 1; i >= 0; --i) {
-      const bool out = PACKED && !((k.valid >> i) & 1);
-      if (PACKED && ((k.last >> i) & 1)) {
-        const int n = k.sequence(i);
-        mu = p.d_state_out ? ch.load(p.d_state_out + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
+    } else if (PACKED && plain) {
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i)
+        if (!MAPS) w[i] = forward(i, a[i], m[i]);
+      #pragma unroll
+      for (int i = RUN - 1; i >= 0; --i) adjoint(i, a[i]);
+    } else {
+      #pragma unroll 1
+      for (int i = 0; i < RUN; ++i) {
+        decay_any<COMP && !MAPS>(gs.get(i), la[i], lm[i]);
+        if (!MAPS) lw[i] = forward(i, la[i], lm[i]);
       }
+      #pragma unroll 1
+      for (int i = RUN - 1; i >= 0; --i) adjoint(i, la[i]);
+    }
+    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, c, all, any_cut);
+    if (MAPS) continue;
+    if (plain && !cuts && t0 + RUN <= p.T) {
+      if (!ch.on0) continue;
+      #pragma unroll
+      for (int i = RUN - 1; i >= 0; --i, ox -= p.dx.s1, og -= p.dg.s1) {
+        const f32x2 l = f2add(ds.get(i), mu);
+        ch.store(ox, COMP ? f2mul(m[i], l) : l);
+        mu = f2mul(a[i], l);
+        ch.store(og, f2mul(mu, w[i]));
+      }
+      if (PACKED && p.d_state_in && k.start) ch.store_state(p.d_state_in + (int64_t)n0 * p.C + base, mu);
+      continue;
+    }
+    auto write = [&](int i, f32x2 e, f32x2 r, f32x2 weight) {
+      const int n = PACKED ? k.sequence(i) : 0;
+      if (PACKED && ((k.last >> i) & 1))
+        mu = p.d_state_out ? ch.load(p.d_state_out + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
       const f32x2 l = f2add(ds.get(i), mu);
-      f32x2 vx = COMP ? f2mul(m[i], l) : l;
-      mu = f2mul(a[i], l);
-      f32x2 vg = f2mul(mu, w[i]);
-      if (out) vx = vg = mu = f2pk(0.f, 0.f);
+      f32x2 vx = COMP ? f2mul(r, l) : l;
+      mu = f2mul(e, l);
+      f32x2 vg = f2mul(mu, weight);
+      if (PACKED && !((k.valid >> i) & 1)) vx = vg = mu = f2pk(0.f, 0.f);
       if (ch.on0 && t0 + i < p.T) {
         ch.store(ox, vx);
         ch.store(og, vg);
+        if (PACKED && p.d_state_in && ((k.start >> i) & 1)) ch.store_state(p.d_state_in + (int64_t)n * p.C + base, mu);
       }
       ox -= p.dx.s1;
       og -= p.dg.s1;
-      if (PACKED && p.d_state_in && ((k.start >> i) & 1)) {
-        const int n = k.sequence(i);
-        if (ch.on0) ch.store_state(p.d_state_in + (int64_t)n * p.C + base, mu);
-      }
+    };
+    if (plain) {
+      if (!PACKED && t0 >= p.T) continue;  // nothing to write
+      #pragma unroll
+      for (int i = RUN - 1; i >= 0; --i) write(i, a[i], m[i], w[i]);
+    } else {
+      #pragma unroll 1
+      for (int i = RUN - 1; i >= 0; --i) write(i, la[i], lm[i], lw[i]);
     }
   }
   if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
@@ -444,7 +564,7 @@ static int launch(K kernel, const ScanParams& p, const ScanPlan& n, int stage, c
 
 template <typename TX, typename TG, RowMode MODE, bool COMP, bool PACKED>
 static int run_scan(const ScanParams& p, const ScanPlan& n, bool bwd, cudaStream_t st, const char* fn) {
-  const int rx = Rows<TX, MODE>::BYTES, rg = Rows<TG, MODE>::BYTES, stage = bwd ? 2 * rx + rg : rx + rg;
+  const int stage = stage_bytes<TX, TG, MODE>(bwd);
   if (n.warps == 8)
     return bwd ? launch(k_scan_bwd<TX, TG, MODE, 8, COMP, PACKED, false>, p, n, stage, st, fn)
                : launch(k_scan_fwd<TX, TG, MODE, 8, COMP, PACKED, false>, p, n, stage, st, fn);
