@@ -19,9 +19,12 @@
 // With few chains (sequences times sets of channels) the time axis is cut
 // into segments as well: a first launch reduces every segment to its map, the
 // second starts each segment from the maps before it.  That reads the inputs
-// twice, and pays below about 100 chains, where one block each would leave
-// the memory system idle.  The joining order is fixed by the sizes: results
-// do not depend on timing.
+// twice, and pays below about 80 chains, where one block each would leave the
+// memory system idle.  The first launch walks its segments against the
+// direction of the scan: it ends where the second begins, so L2 still holds
+// that part of the inputs, and it stops at a packed sequence's boundary, since
+// nothing passes it.  The joining order is fixed by the sizes: results do not
+// depend on timing.
 #pragma once
 
 #include "sequence.cuh"
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
 
   constexpr int STAGE = RX::BYTES + RG::BYTES;
   auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
-  auto run_at = [&](int step) { return ((seg * p.steps + step) * NW + warp) * RUN; };
+  auto run_at = [&](int step) { return ((seg * p.steps + (MAPS ? p.steps - 1 - step : step)) * NW + warp) * RUN; };
   auto fetch = [&](int step) {
     if (step < p.steps) {
       RX{stage(step)}.fetch(x, p.x.s1, run_at(step), p.T, p.C - base, lane);
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
     }
     cp_async_commit();
   };
-  SequenceCursor<RUN - 1> cursor;
+  SequenceCursor<MAPS ? 0 : RUN - 1> cursor;
   for (int step = 0; step < STAGES - 1; ++step) fetch(step);
   for (int step = 0; step < p.steps; ++step) {
     __syncwarp();
@@ -303,8 +306,14 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
         }
       }
     }
-    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, c, all, any_cut);
-    if (MAPS) continue;
+    f32x2 tile = f2pk(1.f, 1.f), before = f2pk(0.f, 0.f);
+    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, MAPS ? before : c, tile, any_cut);
+    if (MAPS) {  // this tile, then those behind it
+      c = f2fma(all, before, c);
+      all = f2mul(all, tile);
+      if (PACKED && any_cut) break;
+      continue;
+    }
     if (p.carry && ch.on0 && t0 < p.T) ch.store_state(carry, cin);
     const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
     if (plain) {
@@ -345,6 +354,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
       if (PACKED && p.state_out && ((k.last >> i) & 1)) ch.store_state(p.state_out + (int64_t)n * p.C + base, v);
     }
   }
+  cp_async_wait<0>();
   if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
   else if (!PACKED && p.state_out && seg == p.segments - 1 && warp == 0 && ch.on0)
     ch.store_state(p.state_out + (int64_t)b * p.C + base, c);
@@ -383,7 +393,9 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
 
   constexpr int STAGE = 2 * RX::BYTES + RG::BYTES;
   auto stage = [&](int step) { return smem + ((step % STAGES) * NW + warp) * STAGE; };
-  auto run_at = [&](int step) { return ((p.segments * p.steps - 1 - (seg * p.steps + step)) * NW + NW - 1 - warp) * RUN; };
+  auto run_at = [&](int step) {
+    return ((p.segments * p.steps - 1 - (seg * p.steps + (MAPS ? p.steps - 1 - step : step))) * NW + NW - 1 - warp) * RUN;
+  };
   f32x2 next_state = f2pk(0.f, 0.f);  // state before the next step's run
   auto fetch = [&](int step) {
     if (step < p.steps) {
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
     cp_async_commit();
   };
   static_assert(STAGES == 2, "next_state is one step ahead");
-  SequenceCursor<0> cursor;
+  SequenceCursor<MAPS ? RUN - 1 : 0> cursor;
   fetch(0);
   for (int step = 0; step < p.steps; ++step) {
     __syncwarp();
@@ -478,8 +490,14 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
       #pragma unroll 1
       for (int i = RUN - 1; i >= 0; --i) adjoint(i, la[i]);
     }
-    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, c, all, any_cut);
-    if (MAPS) continue;
+    f32x2 tile = f2pk(1.f, 1.f), behind = f2pk(0.f, 0.f);
+    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, MAPS ? behind : c, tile, any_cut);
+    if (MAPS) {  // this tile, then those before it
+      c = f2fma(all, behind, c);
+      all = f2mul(all, tile);
+      if (PACKED && any_cut) break;
+      continue;
+    }
     if (plain && !cuts && t0 + RUN <= p.T) {
       if (!ch.on0) continue;
       #pragma unroll
@@ -518,6 +536,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
       for (int i = RUN - 1; i >= 0; --i) write(i, la[i], lm[i], lw[i]);
     }
   }
+  cp_async_wait<0>();
   if (MAPS) write_map<PACKED>(p, chain, seg, all, c, any_cut);
   else if (!PACKED && p.d_state_in && seg == p.segments - 1 && warp == 0 && ch.on0)
     ch.store_state(p.d_state_in + (int64_t)b * p.C + base, c);
