@@ -30,6 +30,7 @@ from ._lib import LIB, check
 from .config import Gdn2Config, Gdn2Mode
 from .ops import (SHORT_CONV_CACHE, chunk_args, chunk_workspace, precision_code, project_activations,
                   recurrent_args, rms_norm_gate_per_head, stream_handle)
+from .sequence import reorder_states, select_states
 
 FUSED_RECURRENT_MAX_SEQ = 64  # src/module.rs:17
 
@@ -64,6 +65,16 @@ class Gdn2State:
         z = lambda *s: torch.zeros(*s, dtype=torch.float32, device=device)
         return Gdn2State(z(batch, hv, hk, v_head), z(batch, SHORT_CONV_CACHE, kd), z(batch, SHORT_CONV_CACHE, kd),
                          z(batch, SHORT_CONV_CACHE, vd))
+
+    def reorder(self, index) -> None:
+        """Fork, compact and free the batch's sequences in place: row d
+        becomes what row index[d] was, -1 a fresh sequence (reorder_states)."""
+        reorder_states(self, index)
+
+    def select(self, index) -> "Gdn2State":
+        """A new state of len(index) sequences, copies of rows index
+        (-1: a fresh one) of this one (select_states)."""
+        return select_states(self, index)
 
 
 @dataclasses.dataclass

@@ -4,9 +4,10 @@ The crate trains by burn autodiff of its tensor path: ``forward_train``
 (src/module.rs:326-375) over ``project`` (src/module.rs:381-498), the chunked
 core (src/forward.rs:44-278) and the gated RMS norm + o_proj
 (src/module.rs:501-517).  ``layer_forward`` is the same graph for torch
-autograd: the projections and every elementwise step are torch ops, the
-recurrence is ``GatedDeltaCore`` (chunked tensor-core forward, exact-f32
-backward kernel), so ``loss.backward()`` gives the gradient of every weight
+autograd: the projections are torch ops, the recurrence is ``GatedDeltaCore``
+(chunked tensor-core forward, exact-f32 backward kernel), the short conv and
+the gated norm are ``causal_conv_silu`` and ``group_norm_gate`` (torch ops off
+the GPU and in float64), every other elementwise step is a torch op, so ``loss.backward()`` gives the gradient of every weight
 and of the input.  The fused inference path (``GatedDeltaNet2.forward_train``)
 stays the fast forward; this one keeps the intermediates autograd needs.
 
@@ -23,6 +24,7 @@ import torch.nn.functional as F
 
 from .config import Gdn2Config
 from .ops import GatedDeltaCore
+from .sequence import causal_conv_silu, group_norm_gate
 
 SHORT_CONV_KERNEL = 4  # src/short_conv.rs:5
 SHORT_CONV_CACHE = 3  # src/short_conv.rs:7
@@ -32,13 +34,20 @@ PARAM_NAMES = ("q_proj", "k_proj", "v_proj", "f_proj_0", "f_proj_1", "b_proj", "
                "g_proj_1_b", "A_log", "dt_bias", "o_norm_w", "o_proj", "q_conv_w", "k_conv_w", "v_conv_w")
 
 
+def _on_kernels(*tensors: torch.Tensor) -> bool:
+    """Whether the sequence operators take these tensors."""
+    return all(t.is_cuda and t.dtype == torch.float32 for t in tensors)
+
+
 def short_conv_silu(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """Causal depthwise conv (kernel 4) + SiLU from a zero state: the sequence
     start padded by replicating token 0 three times (src/short_conv.rs:22-65).
-    x [B,T,C]; weight [C,4].  One depthwise conv1d over the replicate-padded
+    x [B,T,C]; weight [C,4].  On the GPU causal_conv_silu; elsewhere one depthwise conv1d over the replicate-padded
     [B,C,T+3] sequence (cross-correlation: out[t] = sum_i w[c,i] x_pad[t+i])
     instead of four shifted products, so forward and backward are a few
     kernels, not a few dozen."""
+    if _on_kernels(x, weight):
+        return causal_conv_silu(x, weight)[0]
     C = x.shape[2]
     xp = F.pad(x.transpose(1, 2), (SHORT_CONV_CACHE, 0), mode="replicate")
     out = F.conv1d(xp, weight.reshape(C, 1, SHORT_CONV_KERNEL), groups=C)
@@ -101,7 +110,11 @@ def project(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Tensor, g
 
 
 def rms_norm_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
-    """o / sqrt(mean_V o^2 + eps) * weight * silu(gate) per head (src/module.rs:501-517); [B,T,HV,V]."""
+    """o / sqrt(mean_V o^2 + eps) * weight * silu(gate) per head (src/module.rs:501-517); [B,T,HV,V].
+    On the GPU group_norm_gate without centering, a group a head."""
+    if _on_kernels(o, gate, weight):
+        rows = lambda t: t.reshape(*t.shape[:-2], -1)
+        return group_norm_gate(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False).view(o.shape)
     return o * torch.rsqrt((o * o).mean(-1, keepdim=True) + eps) * weight * F.silu(gate)
 
 
