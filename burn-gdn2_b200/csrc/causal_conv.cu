@@ -39,6 +39,30 @@ struct ConvParams {
   float* part;  // [gridDim.y][C][4]
 };
 
+// Where a warp is: a run of one of its spans.  `end`: one past the rows that
+// the span walks (the adjoint three more than its own), `s1` past its own.
+struct ConvWalk {
+  int64_t unit;
+  int b, s0, s1, end, t0;
+  bool ok;
+};
+template <bool PACKED>
+__device__ __forceinline__ ConvWalk conv_span(const ConvParams& p, int64_t unit, int behind) {
+  ConvWalk w;
+  w.unit = unit;
+  w.ok = unit < (int64_t)p.spans * (PACKED ? 1 : p.B);
+  w.b = PACKED ? 0 : (int)(unit / p.spans);
+  w.s0 = w.t0 = (int)(PACKED ? unit : unit % p.spans) * p.span;
+  w.s1 = w.s0 + p.span < p.T ? w.s0 + p.span : p.T;
+  w.end = w.s1 + behind;
+  return w;
+}
+template <bool PACKED>
+__device__ __forceinline__ ConvWalk next_run(const ConvParams& p, ConvWalk w, int behind) {
+  w.t0 += RUN;
+  return w.t0 < w.end ? w : conv_span<PACKED>(p, w.unit + (int64_t)gridDim.y * CONV_WARPS, behind);
+}
+
 // What a run's tokens are: one bit a token; lane i holds the sequence and
 // the first row of token i.
 struct ConvRun {
@@ -123,7 +147,7 @@ __device__ __forceinline__ void load_taps(const ConvParams& p, int base, const P
 }
 
 template <typename T, RowMode MODE, bool PACKED>
-__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p) {
+__global__ void __launch_bounds__(32 * CONV_WARPS, 8) k_conv_fwd(const ConvParams p) {
   typedef Rows<T, MODE> R;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -133,57 +157,55 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p
   f32x2 w[HALO + 1];
   load_taps(p, base, ch, w);
 
-  const int64_t units = (int64_t)p.spans * (PACKED ? 1 : p.B);
-  for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < units; unit += (int64_t)gridDim.y * CONV_WARPS) {
-    const int b = PACKED ? 0 : (int)(unit / p.spans);
-    const int s0 = (int)(PACKED ? unit : unit % p.spans) * p.span, s1 = s0 + p.span < p.T ? s0 + p.span : p.T;
-    const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
-    T* y = static_cast<T*>(const_cast<void*>(p.y.p)) + b * p.y.s0 + base;
-    auto rows = [&](int run) { return R{smem + ((run % STAGES) * CONV_WARPS + warp) * R::BYTES}; };
-    auto fetch = [&](int run) {
-      if (s0 + run * RUN < s1) rows(run).fetch(x, p.x.s1, s0 + run * RUN, p.T, p.C - base, lane);
-      cp_async_commit();
-    };
+  auto rows = [&](int n) { return R{smem + ((n % STAGES) * CONV_WARPS + warp) * R::BYTES}; };
+  auto x_of = [&](const ConvWalk& w) { return static_cast<const T*>(p.x.p) + w.b * p.x.s0 + base; };
+  auto fetch = [&](const ConvWalk& w, int n) {
+    if (w.ok) rows(n).fetch(x_of(w), p.x.s1, w.t0, p.T, p.C - base, lane);
+    cp_async_commit();
+  };
+  ConvWalk at = conv_span<PACKED>(p, (int64_t)blockIdx.y * CONV_WARPS + warp, 0);
+  fetch(at, 0);
+  f32x2 win[HALO];
+  for (int turn = 0; at.ok; ++turn) {
+    const ConvWalk next = next_run<PACKED>(p, at, 0);
     __syncwarp();
-    fetch(0);
-    f32x2 win[HALO];
-    for (int run = 0, t0 = s0; t0 < s1; ++run, t0 += RUN) {
-      __syncwarp();
-      fetch(run + 1);
-      const ConvRun k = conv_run<PACKED>(p, b, t0, lane);
-      if (t0 == s0) {  // the tokens in front, of a span that begins inside a sequence
-        #pragma unroll
-        for (int i = 0; i < HALO; ++i) win[i] = f2pk(0.f, 0.f);
-        const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
-        if ((k.valid & 1) && !(k.start & 1)) window_before(p, x, seq, first, t0, base, ch, win);
-      }
-      cp_async_wait<STAGES - 1>();
-      __syncwarp();
-      const auto xs = rows(run).view(x, p.x.s1, t0, lane);
-      T* out = y + (int64_t)t0 * p.y.s1;
-      if (k.inside() && t0 + RUN <= s1) {
-        #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-          const f32x2 xf = xs.get(i), pre = taps(win, xf, w);
-          if (ch.on0) ch.store(out, f2mul(pre, sigmoid2(pre)));
-          out += p.y.s1;
-          slide(win, xf);
-        }
-        continue;
-      }
-      #pragma unroll 1
-      for (int i = 0; i < RUN && t0 + i < s1; ++i) {
-        const int seq = __shfl_sync(0xffffffffu, k.seq, i);
-        const f32x2 xf = xs.get(i);
-        if ((k.start >> i) & 1) window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
-        const f32x2 pre = taps(win, xf, w);
-        if (ch.on0) ch.store(out, (k.valid >> i) & 1 ? f2mul(pre, sigmoid2(pre)) : f2pk(0.f, 0.f));
+    fetch(next, turn + 1);
+    const int t0 = at.t0, s1 = at.s1;
+    const T* x = x_of(at);
+    const ConvRun k = conv_run<PACKED>(p, at.b, t0, lane);
+    if (t0 == at.s0) {  // the tokens in front, of a span that begins inside a sequence
+      #pragma unroll
+      for (int i = 0; i < HALO; ++i) win[i] = f2pk(0.f, 0.f);
+      const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
+      if ((k.valid & 1) && !(k.start & 1)) window_before(p, x, seq, first, t0, base, ch, win);
+    }
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const auto xs = rows(turn).view(x, p.x.s1, t0, lane);
+    T* out = static_cast<T*>(const_cast<void*>(p.y.p)) + at.b * p.y.s0 + base + (int64_t)t0 * p.y.s1;
+    at = next;
+    if (k.inside() && t0 + RUN <= s1) {
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i) {
+        const f32x2 xf = xs.get(i), pre = taps(win, xf, w);
+        if (ch.on0) ch.store(out, f2mul(pre, sigmoid2(pre)));
         out += p.y.s1;
         slide(win, xf);
-        if (((k.last >> i) & 1) && p.cache_out && ch.on0)
-          #pragma unroll
-          for (int s = 0; s < HALO; ++s) ch.store_state(p.cache_out + cache_at(p, seq, s, base), win[s]);
       }
+      continue;
+    }
+    #pragma unroll 1
+    for (int i = 0; i < RUN && t0 + i < s1; ++i) {
+      const int seq = __shfl_sync(0xffffffffu, k.seq, i);
+      const f32x2 xf = xs.get(i);
+      if ((k.start >> i) & 1) window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
+      const f32x2 pre = taps(win, xf, w);
+      if (ch.on0) ch.store(out, (k.valid >> i) & 1 ? f2mul(pre, sigmoid2(pre)) : f2pk(0.f, 0.f));
+      out += p.y.s1;
+      slide(win, xf);
+      if (((k.last >> i) & 1) && p.cache_out && ch.on0)
+        #pragma unroll
+        for (int s = 0; s < HALO; ++s) ch.store_state(p.cache_out + cache_at(p, seq, s, base), win[s]);
     }
   }
 }
@@ -192,7 +214,7 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_fwd(const ConvParams p
 // gradient of the three values before its sequence where s - k lies there;
 // the span that holds the sequence's first token collects those.
 template <typename T, RowMode MODE, bool PACKED>
-__global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p) {
+__global__ void __launch_bounds__(32 * CONV_WARPS, 4) k_conv_bwd(const ConvParams p) {
   typedef Rows<T, MODE> R;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -205,123 +227,119 @@ __global__ void __launch_bounds__(32 * CONV_WARPS) k_conv_bwd(const ConvParams p
   #pragma unroll
   for (int j = 0; j <= HALO; ++j) dw[j] = zero;
 
-  const int64_t units = (int64_t)p.spans * (PACKED ? 1 : p.B);
-  for (int64_t unit = (int64_t)blockIdx.y * CONV_WARPS + warp; unit < units; unit += (int64_t)gridDim.y * CONV_WARPS) {
-    const int b = PACKED ? 0 : (int)(unit / p.spans);
-    const int s0 = (int)(PACKED ? unit : unit % p.spans) * p.span, s1 = s0 + p.span < p.T ? s0 + p.span : p.T;
-    const int end = s1 + HALO;  // rows walked: a token's dx leaves three tokens later
-    const T* x = static_cast<const T*>(p.x.p) + b * p.x.s0 + base;
-    const T* dy = static_cast<const T*>(p.y.p) + b * p.y.s0 + base;
-    T* dx = static_cast<T*>(const_cast<void*>(p.dx.p)) + b * p.dx.s0 + base;
-    auto rows = [&](int run, int which) {
-      return R{smem + (((run % STAGES) * CONV_WARPS + warp) * 2 + which) * R::BYTES};
-    };
-    auto fetch = [&](int run) {
-      const int t0 = s0 + run * RUN;
-      if (t0 < end) {
-        rows(run, 0).fetch(x, p.x.s1, t0, p.T, p.C - base, lane);
-        rows(run, 1).fetch(dy, p.y.s1, t0, p.T, p.C - base, lane);
-      }
-      cp_async_commit();
-    };
+  auto rows = [&](int n, int which) { return R{smem + (((n % STAGES) * CONV_WARPS + warp) * 2 + which) * R::BYTES}; };
+  auto x_of = [&](const ConvWalk& w) { return static_cast<const T*>(p.x.p) + w.b * p.x.s0 + base; };
+  auto dy_of = [&](const ConvWalk& w) { return static_cast<const T*>(p.y.p) + w.b * p.y.s0 + base; };
+  auto fetch = [&](const ConvWalk& w, int n) {
+    if (w.ok) {
+      rows(n, 0).fetch(x_of(w), p.x.s1, w.t0, p.T, p.C - base, lane);
+      rows(n, 1).fetch(dy_of(w), p.y.s1, w.t0, p.T, p.C - base, lane);
+    }
+    cp_async_commit();
+  };
+  ConvWalk at = conv_span<PACKED>(p, (int64_t)blockIdx.y * CONV_WARPS + warp, HALO);
+  fetch(at, 0);
+  f32x2 win[HALO], pend[HALO], before[HALO];
+  int pos = HALO;      // place of the next token in its sequence, as far as the first three count
+  bool owned = false;  // the sequence begins in this span
+  for (int turn = 0; at.ok; ++turn) {
+    const ConvWalk next = next_run<PACKED>(p, at, HALO);
     __syncwarp();
-    fetch(0);
-    f32x2 win[HALO], pend[HALO] = {zero, zero, zero}, before[HALO] = {zero, zero, zero};
-    int pos = HALO;      // place of the next token in its sequence, as far as the first three count
-    bool owned = false;  // the sequence begins in this span
-    for (int run = 0, t0 = s0; t0 < end; ++run, t0 += RUN) {
-      __syncwarp();
-      fetch(run + 1);
-      const ConvRun k = conv_run<PACKED>(p, b, t0, lane);
-      if (t0 == s0) {
-        #pragma unroll
-        for (int i = 0; i < HALO; ++i) win[i] = zero;
-        const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
-        if ((k.valid & 1) && !(k.start & 1)) {
-          window_before(p, x, seq, first, t0, base, ch, win);
-          pos = t0 - first;
-        }
+    fetch(next, turn + 1);
+    const int t0 = at.t0, s0 = at.s0, s1 = at.s1, end = at.end;
+    const T *x = x_of(at), *dy = dy_of(at);
+    const ConvRun k = conv_run<PACKED>(p, at.b, t0, lane);
+    if (t0 == s0) {
+      #pragma unroll
+      for (int i = 0; i < HALO; ++i) win[i] = pend[i] = before[i] = zero;
+      pos = HALO;
+      owned = false;
+      const int seq = __shfl_sync(0xffffffffu, k.seq, 0), first = __shfl_sync(0xffffffffu, k.first, 0);
+      if ((k.valid & 1) && !(k.start & 1)) {
+        window_before(p, x, seq, first, t0, base, ch, win);
+        pos = t0 - first;
       }
-      cp_async_wait<STAGES - 1>();
-      __syncwarp();
-      const auto xs = rows(run, 0).view(x, p.x.s1, t0, lane);
-      const auto ds = rows(run, 1).view(dy, p.y.s1, t0, lane);
-      T* out = dx + (int64_t)(t0 - HALO) * p.dx.s1;
-      // dpre of a token, and its part of dw where the token is the span's own
-      auto adjoint = [&](f32x2 xf, f32x2 df, bool own) {
-        const f32x2 pre = taps(win, xf, w), sig = sigmoid2(pre);
-        const f32x2 dp = f2mul(df, f2mul(sig, f2fma(pre, f2fma(sig, minus, one), one)));
-        if (own) {
-          #pragma unroll
-          for (int j = 0; j < HALO; ++j) dw[j] = f2fma(dp, win[j], dw[j]);
-          dw[HALO] = f2fma(dp, xf, dw[HALO]);
-        }
-        return dp;
-      };
-      if (k.inside() && pos >= HALO) {
+    }
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const auto xs = rows(turn, 0).view(x, p.x.s1, t0, lane);
+    const auto ds = rows(turn, 1).view(dy, p.y.s1, t0, lane);
+    T* out = static_cast<T*>(const_cast<void*>(p.dx.p)) + at.b * p.dx.s0 + base + (int64_t)(t0 - HALO) * p.dx.s1;
+    at = next;
+    // dpre of a token, and its part of dw where the token is the span's own
+    auto adjoint = [&](f32x2 xf, f32x2 df, bool own) {
+      const f32x2 pre = taps(win, xf, w), sig = sigmoid2(pre);
+      const f32x2 dp = f2mul(df, f2mul(sig, f2fma(pre, f2fma(sig, minus, one), one)));
+      if (own) {
         #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-          const f32x2 xf = xs.get(i);
-          const f32x2 dp = adjoint(xf, ds.get(i), i < RUN - HALO || t0 + i < s1);
-          const f32x2 done = f2fma(w[0], dp, pend[2]);
-          if (ch.on0 && (i >= HALO || t0 > s0)) ch.store(out, done);
-          out += p.dx.s1;
-          pend[2] = f2fma(w[1], dp, pend[1]);
-          pend[1] = f2fma(w[2], dp, pend[0]);
-          pend[0] = f2mul(w[3], dp);
-          slide(win, xf);
-        }
-        continue;
+        for (int j = 0; j < HALO; ++j) dw[j] = f2fma(dp, win[j], dw[j]);
+        dw[HALO] = f2fma(dp, xf, dw[HALO]);
       }
-      #pragma unroll 1
-      for (int i = 0; i < RUN && t0 + i < end; ++i) {
-        const int seq = __shfl_sync(0xffffffffu, k.seq, i);
-        const bool opens = (k.start >> i) & 1, closes = (k.last >> i) & 1, in = (k.valid >> i) & 1;
+      return dp;
+    };
+    if (k.inside() && pos >= HALO) {
+      #pragma unroll
+      for (int i = 0; i < RUN; ++i) {
         const f32x2 xf = xs.get(i);
-        if (opens) {
-          pos = 0;
-          owned = t0 + i < s1;
-          window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
-          before[0] = before[1] = before[2] = zero;
+        const f32x2 dp = adjoint(xf, ds.get(i), i < RUN - HALO || t0 + i < s1);
+        const f32x2 done = f2fma(w[0], dp, pend[2]);
+        if (ch.on0 && (i >= HALO || t0 > s0)) ch.store(out, done);
+        out += p.dx.s1;
+        pend[2] = f2fma(w[1], dp, pend[1]);
+        pend[1] = f2fma(w[2], dp, pend[0]);
+        pend[0] = f2mul(w[3], dp);
+        slide(win, xf);
+      }
+      continue;
+    }
+    #pragma unroll 1
+    for (int i = 0; i < RUN && t0 + i < end; ++i) {
+      const int seq = __shfl_sync(0xffffffffu, k.seq, i);
+      const bool opens = (k.start >> i) & 1, closes = (k.last >> i) & 1, in = (k.valid >> i) & 1;
+      const f32x2 xf = xs.get(i);
+      if (opens) {
+        pos = 0;
+        owned = t0 + i < s1;
+        window_before(p, x, seq, t0 + i, t0 + i, base, ch, win);
+        before[0] = before[1] = before[2] = zero;
+      }
+      const f32x2 dp = in ? adjoint(xf, ds.get(i), t0 + i < s1) : zero;
+      f32x2 part[HALO + 1] = {zero, pend[0], pend[1], pend[2]};  // dx of this token and the three before it
+      auto give = [&](int j, f32x2 v) {  // to token s - j, or to what lies before the sequence
+        if (pos >= j) part[j] = f2add(part[j], v);
+        #pragma unroll
+        for (int s = 0; s < HALO; ++s)
+          if (pos < j && pos - j + HALO == s) before[s] = f2add(before[s], v);
+      };
+      if (in) {
+        #pragma unroll
+        for (int j = 0; j <= HALO; ++j) give(j, f2mul(w[HALO - j], dp));
+        if (closes && p.d_cache_out) {  // the new cache holds the last three values
+          #pragma unroll
+          for (int j = 0; j < HALO; ++j)
+            give(j, ch.load(p.d_cache_out + cache_at(p, seq, HALO - 1 - j, base)));
         }
-        const f32x2 dp = in ? adjoint(xf, ds.get(i), t0 + i < s1) : zero;
-        f32x2 part[HALO + 1] = {zero, pend[0], pend[1], pend[2]};  // dx of this token and the three before it
-        auto give = [&](int j, f32x2 v) {  // to token s - j, or to what lies before the sequence
-          if (pos >= j) part[j] = f2add(part[j], v);
-          #pragma unroll
-          for (int s = 0; s < HALO; ++s)
-            if (pos < j && pos - j + HALO == s) before[s] = f2add(before[s], v);
-        };
-        if (in) {
-          #pragma unroll
-          for (int j = 0; j <= HALO; ++j) give(j, f2mul(w[HALO - j], dp));
-          if (closes && p.d_cache_out) {  // the new cache holds the last three values
+        // no later token reaches before the sequence: hand on what does
+        if (owned && (pos == HALO - 1 || (closes && pos < HALO - 1))) {
+          if (p.d_cache_in) {
+            if (ch.on0)
+              #pragma unroll
+              for (int s = 0; s < HALO; ++s) ch.store_state(p.d_cache_in + cache_at(p, seq, s, base), before[s]);
+          } else if (!p.cache_in) {  // copies of the first token
             #pragma unroll
             for (int j = 0; j < HALO; ++j)
-              give(j, ch.load(p.d_cache_out + cache_at(p, seq, HALO - 1 - j, base)));
-          }
-          // no later token reaches before the sequence: hand on what does
-          if (owned && (pos == HALO - 1 || (closes && pos < HALO - 1))) {
-            if (p.d_cache_in) {
-              if (ch.on0)
-                #pragma unroll
-                for (int s = 0; s < HALO; ++s) ch.store_state(p.d_cache_in + cache_at(p, seq, s, base), before[s]);
-            } else if (!p.cache_in) {  // copies of the first token
-              #pragma unroll
-              for (int j = 0; j < HALO; ++j)
-                if (pos == j) part[j] = f2add(part[j], f2add(before[0], f2add(before[1], before[2])));
-            }
+              if (pos == j) part[j] = f2add(part[j], f2add(before[0], f2add(before[1], before[2])));
           }
         }
-        const int row = t0 + i - HALO;
-        if (ch.on0 && row >= s0 && row < s1) ch.store(out, part[HALO]);
-        out += p.dx.s1;
-        pend[0] = part[0];
-        pend[1] = part[1];
-        pend[2] = part[2];
-        slide(win, xf);
-        pos = pos < HALO ? pos + 1 : pos;
       }
+      const int row = t0 + i - HALO;
+      if (ch.on0 && row >= s0 && row < s1) ch.store(out, part[HALO]);
+      out += p.dx.s1;
+      pend[0] = part[0];
+      pend[1] = part[1];
+      pend[2] = part[2];
+      slide(win, xf);
+      pos = pos < HALO ? pos + 1 : pos;
     }
   }
   if (!p.part) return;
@@ -358,29 +376,49 @@ static int check_conv(const gdn2_conv_args* a, const char* fn) {
   return GDN2_OK;
 }
 
+// Blocks that an SM holds: by shared memory, and by registers 32 warps of a
+// forward (64 a thread) and 16 of a backward (128).
+constexpr int conv_resident(int bytes, bool bwd) {
+  const int smem = STAGES * CONV_WARPS * bytes * (bwd ? 2 : 1) + 1024, by_smem = 227 * 1024 / smem;
+  const int by_regs = (bwd ? 16 : 32) / CONV_WARPS;
+  return by_smem < by_regs ? by_smem : by_regs;
+}
+static int conv_resident(RowMode mode, int e, bool bwd) {
+  const bool shifted = mode == ROWS_PAIR || mode == ROWS_ODD;
+  return conv_resident(RUN * (SET * e + (shifted ? 16 : 0)), bwd);
+}
+
 // How a call is cut up: how rows are held, spans of tokens and blocks along them.
 struct ConvPlan {
   RowMode mode;
   int sets, span, spans, blocks;
 };
 
-// Spans of `runs` runs less `less` tokens, down to one run until the warps fill the GPU.  `blocks_per_sm`: blocks
-// along the spans (each leaves a partial row of dw), 0 for all of them.
-static ConvPlan plan_conv(const gdn2_conv_args* a, RowMode mode, int less, int blocks_per_sm) {
+// Spans of whole runs less `less` tokens.  Blocks (along the spans) as many as
+// are resident, so that none waits for a second wave; span and blocks such that
+// the warps with most to do have least: a span costs its runs and about half
+// a run for its beginning.
+static ConvPlan plan_conv(const gdn2_conv_args* a, RowMode mode, int less, int resident) {
   ConvPlan n;
   n.mode = mode;
   n.sets = (a->channels + SET - 1) / SET;
   const int rows = a->cu_seqlens ? 1 : a->batch;
-  int runs = 8;
-  for (;; runs /= 2) {
-    n.span = runs * RUN - less;
-    n.spans = (a->seq_len + n.span - 1) / n.span;
-    if (runs == 1 || (int64_t)n.spans * rows * n.sets >= 148 * 4 * CONV_WARPS) break;
+  const int64_t most = 148 * (int64_t)resident / n.sets;
+  int64_t best = -1;
+  for (int runs = 16; runs >= 1; --runs) {
+    const int span = runs * RUN - less;
+    const int64_t spans = (a->seq_len + span - 1) / span, units = spans * rows;
+    int64_t blocks = (units + CONV_WARPS - 1) / CONV_WARPS;
+    if (blocks > most) blocks = most;
+    if (blocks < 1) blocks = 1;
+    if (blocks > 65535) blocks = 65535;
+    const int64_t rounds = (units + blocks * CONV_WARPS - 1) / (blocks * CONV_WARPS), cost = rounds * (2 * runs + 1);
+    if (best >= 0 && cost >= best) continue;
+    best = cost;
+    n.span = span;
+    n.spans = (int)spans;
+    n.blocks = (int)blocks;
   }
-  const int64_t most = ((int64_t)n.spans * rows + CONV_WARPS - 1) / CONV_WARPS;
-  int64_t want = blocks_per_sm ? (148 * blocks_per_sm + n.sets - 1) / n.sets : most;
-  want = want < most ? want : most;
-  n.blocks = (int)(want < 1 ? 1 : want > 65535 ? 65535 : want);
   return n;
 }
 
@@ -428,7 +466,8 @@ int launch_conv_fwd(const gdn2_conv_args* a, const gdn2_view& y, float* cache_ou
   if (a->seq_len && !y.data) return set_error(GDN2_EINVAL, "%s: null tensor pointer", fn);
   const int e = elem_bytes(a->dtype);
   const RowTensor t[] = {{&a->x, e, true}, {&y, e, false}};
-  const ConvPlan n = plan_conv(a, row_mode(a->channels, t, 2), 0, 0);
+  const RowMode mode = row_mode(a->channels, t, 2);
+  const ConvPlan n = plan_conv(a, mode, 0, conv_resident(mode, e, false));
   ConvParams p;
   fill_conv(p, a, n);
   p.y = make_dview(y);
@@ -441,7 +480,8 @@ static ConvPlan plan_conv_bwd(const gdn2_conv_bwd_args* q) {
   const gdn2_conv_args* a = &q->fwd;
   const int e = elem_bytes(a->dtype);
   const RowTensor t[] = {{&a->x, e, true}, {&q->d_y, e, true}, {&q->dx, e, false}};
-  return plan_conv(a, row_mode(a->channels, t, 3), HALO, 5);
+  const RowMode mode = row_mode(a->channels, t, 3);
+  return plan_conv(a, mode, HALO, conv_resident(mode, e, true));
 }
 
 size_t conv_bwd_workspace_bytes(const gdn2_conv_bwd_args* q) {

@@ -24,18 +24,36 @@ template <typename T, int VEC>
 struct Vec {
   typedef typename RawOf<(int)sizeof(T) * VEC>::type Raw;
   static __device__ __forceinline__ Raw load(const T* p) { return __ldcs(reinterpret_cast<const Raw*>(p)); }
+  // bf16 in pairs: a shift and a mask to f32, one conversion of both back
   static __device__ __forceinline__ void unpack(Raw r, float (&f)[VEC]) {
-    T e[VEC];
-    memcpy(e, &r, sizeof(r));
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) f[v] = to_f32<T>(e[v]);
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+      unsigned w[VEC / 2];
+      memcpy(w, &r, sizeof(r));
+      #pragma unroll
+      for (int v = 0; v < VEC / 2; ++v) {
+        f[2 * v] = __uint_as_float(w[v] << 16);
+        f[2 * v + 1] = __uint_as_float(w[v] & 0xffff0000u);
+      }
+    } else {
+      T e[VEC];
+      memcpy(e, &r, sizeof(r));
+      #pragma unroll
+      for (int v = 0; v < VEC; ++v) f[v] = to_f32<T>(e[v]);
+    }
   }
   static __device__ __forceinline__ Raw pack(const float (&f)[VEC]) {
-    T e[VEC];
-    #pragma unroll
-    for (int v = 0; v < VEC; ++v) e[v] = from_f32<T>(f[v]);
     Raw r;
-    memcpy(&r, e, sizeof(r));
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+      __nv_bfloat162 w[VEC / 2];
+      #pragma unroll
+      for (int v = 0; v < VEC / 2; ++v) w[v] = __floats2bfloat162_rn(f[2 * v], f[2 * v + 1]);
+      memcpy(&r, w, sizeof(r));
+    } else {
+      T e[VEC];
+      #pragma unroll
+      for (int v = 0; v < VEC; ++v) e[v] = from_f32<T>(f[v]);
+      memcpy(&r, e, sizeof(r));
+    }
     return r;
   }
   static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
