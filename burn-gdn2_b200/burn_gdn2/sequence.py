@@ -95,6 +95,11 @@ def _f32(what: str, name: str, t: Optional[torch.Tensor], shape) -> Optional[tor
     return t.contiguous()
 
 
+def _written(tensors) -> None:
+    """Tells autograd that a kernel has written over these tensors."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _workspace(size: int, near: torch.Tensor):
     return (near.new_empty(size, dtype=torch.uint8) if size else None), size
 
@@ -196,6 +201,8 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
         return _GatedScan.apply(x, g, state, cu, bool(complement))
     last = state if inplace else x.new_empty((n, C), dtype=torch.float32)
     h, _ = _scan_forward(x, g, state, cu, complement, last, False)
+    if inplace:
+        _written([state])
     return h, last
 
 
@@ -265,7 +272,7 @@ def causal_conv_silu(x, weight, cache=None, *, cu_seqlens=None) -> Tuple[torch.T
     cache = _f32(what, "cache", cache, (n, SHORT_CONV_CACHE, C))
     x = _rows(x)
     if n == 0 or C == 0 or (T == 0 and cu is None):  # nothing to launch: no token, or nothing in it
-        return x * weight[:, 0], torch.zeros((n, SHORT_CONV_CACHE, C), device=x.device) if cache is None else cache.clone()
+        return x * weight[:, 0].to(x.dtype), torch.zeros((n, SHORT_CONV_CACHE, C), device=x.device) if cache is None else cache.clone()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, cache)):
         return _CausalConv.apply(x, weight, cache, cu)
     return _conv_forward(x, weight, cache, cu)
@@ -460,6 +467,7 @@ def reorder_states(states, index) -> None:
     if index.shape[0] != rows:
         raise ValueError(f"{what}: {index.shape[0]} row numbers for {rows} rows")
     _move_rows(tensors, tensors, index, rows)
+    _written(tensors)
 
 
 def select_states(states, index):

@@ -79,7 +79,7 @@ __device__ __forceinline__ ConvRun conv_run(const ConvParams& p, int b, int t0, 
     if (PACKED) {
       k.seq = find_sequence(p.cu, p.B, t);
       if (k.seq >= 0) {
-        k.first = __ldg(p.cu + k.seq);
+        k.first = max(__ldg(p.cu + k.seq), 0);  // rows before the buffer's are nobody's
         l = t + 1 == p.T || __ldg(p.cu + k.seq + 1) == t + 1;
       }
     } else {
