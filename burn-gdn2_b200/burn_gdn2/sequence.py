@@ -171,8 +171,10 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
 
     T = 1 is the decode step.  ``inplace`` writes the new state over ``state``
     and returns it (serving; no gradients).  g may be anything whose
-    exponential is wanted: -inf cuts off what came before.  Differentiable
-    in x, g and state, once.
+    exponential is wanted: -inf cuts off what came before.  Decays of spans
+    are joined as products in f32: growth (g > 0) is exact as far as the product
+    over a span stays below 3e38; beyond, a state of zero stays zero and any
+    other one becomes infinite.  Differentiable in x, g and state, once.
     """
     what = "gated_scan"
     _check_input(what, x)
@@ -393,7 +395,8 @@ def _pool_like(states, new):
         return next(new)
     if dataclasses.is_dataclass(states):
         return dataclasses.replace(states, **{f.name: next(new) for f in dataclasses.fields(states)})
-    return type(states)([_pool_like(s, new) for s in states])
+    items = [_pool_like(s, new) for s in states]
+    return type(states)(*items) if hasattr(states, "_fields") else type(states)(items)
 
 
 def _checked_pool(what: str, states):

@@ -6,10 +6,12 @@ core (src/forward.rs:44-278) and the gated RMS norm + o_proj
 (src/module.rs:501-517).  ``layer_forward`` is the same graph for torch
 autograd: the projections are torch ops, the recurrence is ``GatedDeltaCore``
 (chunked tensor-core forward, exact-f32 backward kernel), the short conv and
-the gated norm are ``causal_conv_silu`` and ``group_norm_gate`` (torch ops off
-the GPU and in float64), every other elementwise step is a torch op, so ``loss.backward()`` gives the gradient of every weight
-and of the input.  The fused inference path (``GatedDeltaNet2.forward_train``)
-stays the fast forward; this one keeps the intermediates autograd needs.
+the gated norm beside it are ``causal_conv_silu`` and ``group_norm_gate``,
+every other elementwise step is a torch op, so ``loss.backward()`` gives the
+gradient of every weight and of the input.  With another core those two are
+torch ops as well, and the layer is as often differentiable as that core.
+The fused inference path (``GatedDeltaNet2.forward_train``) stays the fast
+forward; this one keeps the intermediates autograd needs.
 
 ``layer_forward(params, cfg, x, gva_mode, core)`` works on any device and
 dtype for its torch part; ``core`` computes (o [B,HV,T,V], final state) from
@@ -34,20 +36,13 @@ PARAM_NAMES = ("q_proj", "k_proj", "v_proj", "f_proj_0", "f_proj_1", "b_proj", "
                "g_proj_1_b", "A_log", "dt_bias", "o_norm_w", "o_proj", "q_conv_w", "k_conv_w", "v_conv_w")
 
 
-def _on_kernels(*tensors: torch.Tensor) -> bool:
-    """Whether the sequence operators take these tensors."""
-    return all(t.is_cuda and t.dtype == torch.float32 for t in tensors)
-
-
 def short_conv_silu(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """Causal depthwise conv (kernel 4) + SiLU from a zero state: the sequence
     start padded by replicating token 0 three times (src/short_conv.rs:22-65).
-    x [B,T,C]; weight [C,4].  On the GPU causal_conv_silu; elsewhere one depthwise conv1d over the replicate-padded
+    x [B,T,C]; weight [C,4].  One depthwise conv1d over the replicate-padded
     [B,C,T+3] sequence (cross-correlation: out[t] = sum_i w[c,i] x_pad[t+i])
     instead of four shifted products, so forward and backward are a few
     kernels, not a few dozen."""
-    if _on_kernels(x, weight):
-        return causal_conv_silu(x, weight)[0]
     C = x.shape[2]
     xp = F.pad(x.transpose(1, 2), (SHORT_CONV_CACHE, 0), mode="replicate")
     out = F.conv1d(xp, weight.reshape(C, 1, SHORT_CONV_KERNEL), groups=C)
@@ -70,7 +65,8 @@ def gva_repeat(x: torch.Tensor, rep: int, gva_mode: str) -> torch.Tensor:
     return x.repeat_interleave(rep, dim=1)
 
 
-def project(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Tensor, gva_mode: str, core_dtype):
+def project(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Tensor, gva_mode: str, core_dtype,
+            conv: Callable = short_conv_silu):
     """src/module.rs:381-498 from a zero conv state.  Returns q, k, g, b
     [B,HV,T,K], v, w [B,HV,T,V] (q, k, v, b, w in core_dtype, g f32) and the
     gate [B,T,HV,V]; activations are computed in f32 or wider."""
@@ -82,9 +78,9 @@ def project(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Tensor, g
     up = lambda t: t.to(wide)
     q_raw, k_raw, v_raw = up(x @ P["q_proj"]), up(x @ P["k_proj"]), up(x @ P["v_proj"])
     if cfg.use_short_conv:
-        q_act = short_conv_silu(q_raw, P["q_conv_w"].to(wide))
-        k_act = short_conv_silu(k_raw, P["k_conv_w"].to(wide))
-        v_act = short_conv_silu(v_raw, P["v_conv_w"].to(wide))
+        q_act = conv(q_raw, P["q_conv_w"].to(wide))
+        k_act = conv(k_raw, P["k_conv_w"].to(wide))
+        v_act = conv(v_raw, P["v_conv_w"].to(wide))
     else:
         q_act, k_act, v_act = F.silu(q_raw), F.silu(k_raw), F.silu(v_raw)
     f_out = up((x @ P["f_proj_0"]) @ P["f_proj_1"])
@@ -110,12 +106,19 @@ def project(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Tensor, g
 
 
 def rms_norm_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
-    """o / sqrt(mean_V o^2 + eps) * weight * silu(gate) per head (src/module.rs:501-517); [B,T,HV,V].
-    On the GPU group_norm_gate without centering, a group a head."""
-    if _on_kernels(o, gate, weight):
-        rows = lambda t: t.reshape(*t.shape[:-2], -1)
-        return group_norm_gate(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False).view(o.shape)
+    """o / sqrt(mean_V o^2 + eps) * weight * silu(gate) per head (src/module.rs:501-517); [B,T,HV,V]."""
     return o * torch.rsqrt((o * o).mean(-1, keepdim=True) + eps) * weight * F.silu(gate)
+
+
+def _conv_kernel(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """short_conv_silu on the B200 kernels."""
+    return causal_conv_silu(x, weight)[0]
+
+
+def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
+    """rms_norm_gate on the B200 kernels: a group a head, not centered."""
+    rows = lambda t: t.reshape(*t.shape[:-2], -1)
+    return group_norm_gate(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False).view(o.shape)
 
 
 def cuda_core(q, k, v, g, b, w, scale, chunk):
@@ -131,8 +134,11 @@ def layer_forward(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Ten
     h, hk, hv, vh = cfg.num_heads, cfg.head_dim, cfg.hv, cfg.v_head
     B, T, _ = x.shape
     cdt = core_dtype if core_dtype is not None else x.dtype
-    q, k, v, g, b, w, gate = project(params, cfg, x, gva_mode, cdt)
+    fused = core is cuda_core and x.is_cuda and params["A_log"].dtype != torch.float64  # f32 activations
+    conv = _conv_kernel if fused else short_conv_silu
+    norm = _norm_kernel if fused and cfg.norm_eps > 0 else rms_norm_gate
+    q, k, v, g, b, w, gate = project(params, cfg, x, gva_mode, cdt, conv)
     o, _ = core(q, k, v, g, b, w, hk ** -0.5, cfg.chunk_size)
     o4 = o.permute(0, 2, 1, 3).to(gate.dtype)  # [B,T,HV,V]
-    normed = rms_norm_gate(o4, gate, params["o_norm_w"].to(gate.dtype), cfg.norm_eps)
+    normed = norm(o4, gate, params["o_norm_w"].to(gate.dtype), cfg.norm_eps)
     return normed.reshape(B, T, hv * vh).to(x.dtype) @ params["o_proj"]

@@ -27,6 +27,9 @@
 // depend on timing.
 #pragma once
 
+#include <cfloat>
+#include <type_traits>
+
 #include "sequence.cuh"
 
 namespace gdn2 {
@@ -74,6 +77,34 @@ struct ScanMaps {
   int cut[2][NW];
 };
 
+// A span's map of the state before it.  A state of zero stays out of the
+// product, which growth (g > 0) may have taken to infinity.
+__device__ __forceinline__ f32x2 through(f32x2 A, f32x2 c, f32x2 H) {
+  float c0, c1, h0, h1, v0, v1;
+  f2un(c, c0, c1);
+  f2un(H, h0, h1);
+  f2un(f2fma(A, c, H), v0, v1);
+  return f2pk(c0 == 0.f ? h0 : v0, c1 == 0.f ? h1 : v1);
+}
+
+// e c + in for an e = e^g (or 1 - e^g) that may be beyond f32 although g is
+// not: nothing grows out of nothing.  SURE: e is a number.
+template <bool SURE>
+__device__ __forceinline__ f32x2 grow(f32x2 e, f32x2 g, f32x2 c, f32x2 in) {
+  const f32x2 v = f2fma(e, c, in);
+  if (SURE) return v;
+  float g0, g1, c0, c1, i0, i1, v0, v1;
+  f2un(g, g0, g1);
+  f2un(c, c0, c1);
+  f2un(in, i0, i1);
+  f2un(v, v0, v1);
+  return f2pk(c0 == 0.f && g0 <= FLT_MAX ? i0 : v0, c1 == 0.f && g1 <= FLT_MAX ? i1 : v1);
+}
+template <bool SURE>
+__device__ __forceinline__ f32x2 grow(f32x2 e, f32x2 g, f32x2 c) {
+  return SURE ? f2mul(e, c) : grow<false>(e, g, c, f2pk(0.f, 0.f));
+}
+
 // From the state `c` before the step's first token (after its last, in the
 // adjoint), the state before this warp's run; c becomes the state after the
 // step, and the maps join to `A` of the whole (with SUM).
@@ -89,7 +120,7 @@ __device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int l
     if (w == warp) cin = c;
     const ulonglong2 m = sh.run[buf][w][lane];
     const bool stop = PACKED && sh.cut[buf][w];
-    c = stop ? m.y : f2fma(m.x, c, m.y);
+    c = stop ? m.y : through(m.x, c, m.y);
     if (SUM) {
       all = f2mul(all, m.x);
       any_cut |= stop;
@@ -199,7 +230,7 @@ __device__ __forceinline__ f32x2 through_segments(const ScanParams& p, int64_t c
   #pragma unroll 8
   for (int s = 0; s < seg; ++s) {
     const ulonglong2 v = m[s * 32];
-    c = PACKED && cut[s] ? v.y : f2fma(v.x, c, v.y);
+    c = PACKED && cut[s] ? v.y : through(v.x, c, v.y);
   }
   return c;
 }
@@ -277,18 +308,19 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
         u[i] = H;
       }
     } else {
-      auto token = [&](int i, f32x2 e, f32x2 r, f32x2& product, f32x2& state) {
-        const f32x2 in = COMP ? f2mul(r, xs.get(i)) : xs.get(i);
+      auto token = [&](auto sure, int i, f32x2 g, f32x2 e, f32x2 r, f32x2& product, f32x2& state) {
+        constexpr bool SURE = decltype(sure)::value;
+        const f32x2 in = COMP ? grow<SURE>(r, g, xs.get(i)) : xs.get(i);
         if (PACKED && ((cuts >> i) & 1)) {
           const int n = k.sequence(i);
           cut = true;
           H = f2pk(0.f, 0.f);
           if ((k.start >> i) & 1) {
             if (p.state_in) H = ch.load(p.state_in + (int64_t)n * p.C + base);
-            H = f2fma(e, H, in);
+            H = grow<SURE>(e, g, H, in);
           }
         } else {
-          H = f2fma(e, H, in);
+          H = grow<SURE>(e, g, H, in);
           if (!cut) A = f2mul(A, e);
         }
         product = A;
@@ -296,20 +328,21 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
       };
       if (PACKED && plain) {
         #pragma unroll
-        for (int i = 0; i < RUN; ++i) token(i, a[i], u[i], a[i], u[i]);
+        for (int i = 0; i < RUN; ++i) token(std::true_type(), i, a[i], a[i], u[i], a[i], u[i]);
       } else {
         #pragma unroll 1
         for (int i = 0; i < RUN; ++i) {
           f32x2 e, r;
-          decay_any<COMP>(gs.get(i), e, r);
-          token(i, e, r, la[i], lu[i]);
+          const f32x2 g = gs.get(i);
+          decay_any<COMP>(g, e, r);
+          token(std::false_type(), i, g, e, r, la[i], lu[i]);
         }
       }
     }
     f32x2 tile = f2pk(1.f, 1.f), before = f2pk(0.f, 0.f);
     const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, MAPS ? before : c, tile, any_cut);
     if (MAPS) {  // this tile, then those behind it
-      c = f2fma(all, before, c);
+      c = through(all, before, c);
       all = f2mul(all, tile);
       if (PACKED && any_cut) break;
       continue;
@@ -317,6 +350,17 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
     if (p.carry && ch.on0 && t0 < p.T) ch.store_state(carry, cin);
     const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
     if (plain) {
+      float a0, a1;
+      f2un(A, a0, a1);
+      if (__any_sync(0xffffffffu, fmaxf(a0, a1) > FLT_MAX)) {  // products beyond f32 (see through())
+        float c0, c1;
+        f2un(cin, c0, c1);
+        #pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+          f2un(a[i], a0, a1);
+          a[i] = f2pk(c0 == 0.f ? 0.f : a0, c1 == 0.f ? 0.f : a1);
+        }
+      }
       if (!cuts) {
         #pragma unroll
         for (int i = 0; i < RUN; ++i) u[i] = f2fma(a[i], cin, u[i]);
@@ -347,7 +391,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
     }
     #pragma unroll 1
     for (int i = 0; i < RUN && t0 + i < p.T; ++i, out += p.h.s1) {
-      const f32x2 v = i < first_cut ? f2fma(la[i], cin, lu[i]) : lu[i];
+      const f32x2 v = i < first_cut ? through(la[i], cin, lu[i]) : lu[i];
       const int n = k.sequence(i);
       if (!ch.on0) continue;
       ch.store(out, v);
@@ -433,28 +477,30 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
     bool cut = false;
     const bool plain = decays<COMP && !MAPS>(gs, a, m);
     // state after token i, from the one before it; its weight in dg
-    auto forward = [&](int i, f32x2 e, f32x2 r) {
+    auto forward = [&](auto sure, int i, f32x2 g, f32x2 e, f32x2 r) {
+      constexpr bool SURE = decltype(sure)::value;
       const f32x2 xf = xs.get(i);
       if (PACKED && ((k.start >> i) & 1)) {
         const int n = k.sequence(i);
         hp = p.state_in ? ch.load(p.state_in + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
       }
       const f32x2 weight = COMP ? f2fma(xf, f2pk(-1.f, -1.f), hp) : hp;
-      hp = f2fma(e, hp, COMP ? f2mul(r, xf) : xf);
+      hp = grow<SURE>(e, g, hp, COMP ? grow<SURE>(r, g, xf) : xf);
       return weight;
     };
     // the run's map, extended to the front by token i
-    auto adjoint = [&](int i, f32x2 e) {
+    auto adjoint = [&](auto sure, int i, f32x2 g, f32x2 e) {
+      constexpr bool SURE = decltype(sure)::value;
       if (PACKED && ((cuts >> i) & 1)) {
         const int n = k.sequence(i);
         cut = true;
         M = f2pk(0.f, 0.f);
         if ((k.last >> i) & 1) {
           if (p.d_state_out) M = ch.load(p.d_state_out + (int64_t)n * p.C + base);
-          M = f2mul(e, f2add(ds.get(i), M));
+          M = grow<SURE>(e, g, f2add(ds.get(i), M));
         }
       } else {
-        M = f2mul(e, f2add(ds.get(i), M));
+        M = grow<SURE>(e, g, f2add(ds.get(i), M));
         if (!cut) A = f2mul(A, e);
       }
     };
@@ -478,22 +524,22 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
     } else if (PACKED && plain) {
       #pragma unroll
       for (int i = 0; i < RUN; ++i)
-        if (!MAPS) w[i] = forward(i, a[i], m[i]);
+        if (!MAPS) w[i] = forward(std::true_type(), i, a[i], a[i], m[i]);
       #pragma unroll
-      for (int i = RUN - 1; i >= 0; --i) adjoint(i, a[i]);
+      for (int i = RUN - 1; i >= 0; --i) adjoint(std::true_type(), i, a[i], a[i]);
     } else {
       #pragma unroll 1
       for (int i = 0; i < RUN; ++i) {
         decay_any<COMP && !MAPS>(gs.get(i), la[i], lm[i]);
-        if (!MAPS) lw[i] = forward(i, la[i], lm[i]);
+        if (!MAPS) lw[i] = forward(std::false_type(), i, gs.get(i), la[i], lm[i]);
       }
       #pragma unroll 1
-      for (int i = RUN - 1; i >= 0; --i) adjoint(i, la[i]);
+      for (int i = RUN - 1; i >= 0; --i) adjoint(std::false_type(), i, gs.get(i), la[i]);
     }
     f32x2 tile = f2pk(1.f, 1.f), behind = f2pk(0.f, 0.f);
     f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, MAPS ? behind : c, tile, any_cut);
     if (MAPS) {  // this tile, then those before it
-      c = f2fma(all, behind, c);
+      c = through(all, behind, c);
       all = f2mul(all, tile);
       if (PACKED && any_cut) break;
       continue;
@@ -510,13 +556,14 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
       if (PACKED && p.d_state_in && k.start) ch.store_state(p.d_state_in + (int64_t)n0 * p.C + base, mu);
       continue;
     }
-    auto write = [&](int i, f32x2 e, f32x2 r, f32x2 weight) {
+    auto write = [&](auto sure, int i, f32x2 g, f32x2 e, f32x2 r, f32x2 weight) {
+      constexpr bool SURE = decltype(sure)::value;
       const int n = PACKED ? k.sequence(i) : 0;
       if (PACKED && ((k.last >> i) & 1))
         mu = p.d_state_out ? ch.load(p.d_state_out + (int64_t)n * p.C + base) : f2pk(0.f, 0.f);
       const f32x2 l = f2add(ds.get(i), mu);
-      f32x2 vx = COMP ? f2mul(r, l) : l;
-      mu = f2mul(e, l);
+      f32x2 vx = COMP ? grow<SURE>(r, g, l) : l;
+      mu = grow<SURE>(e, g, l);
       f32x2 vg = f2mul(mu, weight);
       if (PACKED && !((k.valid >> i) & 1)) vx = vg = mu = f2pk(0.f, 0.f);
       if (ch.on0 && t0 + i < p.T) {
@@ -530,10 +577,10 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
     if (plain) {
       if (!PACKED && t0 >= p.T) continue;  // nothing to write
       #pragma unroll
-      for (int i = RUN - 1; i >= 0; --i) write(i, a[i], m[i], w[i]);
+      for (int i = RUN - 1; i >= 0; --i) write(std::true_type(), i, a[i], a[i], m[i], w[i]);
     } else {
       #pragma unroll 1
-      for (int i = RUN - 1; i >= 0; --i) write(i, la[i], lm[i], lw[i]);
+      for (int i = RUN - 1; i >= 0; --i) write(std::false_type(), i, gs.get(i), la[i], lm[i], lw[i]);
     }
   }
   cp_async_wait<0>();
@@ -556,7 +603,11 @@ __global__ void __launch_bounds__(256) k_scan_step(const ScanParams p) {
   Vec<TX, VEC>::unpack(Vec<TX, VEC>::load(static_cast<const TX*>(p.x.p) + b * p.x.s0 + c0), x);
   if (p.state_in) load_f32<VEC>(p.state_in + b * p.C + c0, s);
   #pragma unroll
-  for (int v = 0; v < VEC; ++v) s[v] = fmaf(expf(g[v]), s[v], COMP ? -expm1f(g[v]) * x[v] : x[v]);
+  for (int v = 0; v < VEC; ++v) {
+    const bool grown = g[v] <= FLT_MAX;  // see grow()
+    const float in = !COMP ? x[v] : x[v] == 0.f && grown ? 0.f : -expm1f(g[v]) * x[v];
+    s[v] = s[v] == 0.f && grown ? in : fmaf(expf(g[v]), s[v], in);
+  }
   if (p.state_out) store_f32<VEC>(p.state_out + b * p.C + c0, s);
   Vec<TX, VEC>::store(static_cast<TX*>(const_cast<void*>(p.h.p)) + b * p.h.s0 + c0, s);
 }

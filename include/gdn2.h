@@ -431,8 +431,8 @@ GDN2_API int gdn2_causal_conv_bwd(const gdn2_conv_bwd_args* args, void* workspac
  *   weight, bias : [groups * width] f32, or [width] for all groups with
  *             weight_shared = 1; NULL = 1 and 0
  *   y       : [rows][groups * width] contiguous (dtype)
- * Up to 1024 * v channels a group, v = 4, 2 or 1 the most elements that width,
- * pointers and pitches are multiples of.
+ * A group of more than 1024 * v channels (v = 4, 2 or 1, the most elements that
+ * width, pointers and pitches are multiples of) is read once per statistic.
  * Backward: d_y [rows][ld_dy]; dx, d_gate contiguous (dtype), d_weight and
  * d_bias f32 as the weights, each NULL where it is not wanted.  The
  * workspace (16-byte aligned, gdn2_group_norm_gate_bwd_workspace_bytes; 0

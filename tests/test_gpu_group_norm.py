@@ -59,6 +59,15 @@ def test_sizes(dtype, rows, groups, width, gate, affine, bias, center):
     _check(_run(*data, groups, 1e-5, center, False), want, bound)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,groups,width", [(3, 1, 1025), (2, 2, 1501), (5, 1, 4104), (700, 1, 4100), (3, 3, 8192), (1, 1, 10240)])
+@pytest.mark.parametrize("gate,affine,bias,center", [(True, "channel", True, True), (False, "group", True, False),
+                                                     (True, "group", False, True), (False, "none", False, True)])
+def test_wide_groups(dtype, rows, groups, width, gate, affine, bias, center):
+    """Groups that a block does not hold at once: 40 values a thread at most, then trees of 8."""
+    test_sizes(dtype, rows, groups, width, gate, affine, bias, center)
+
+
 def test_equals_rms_norm_gate_per_head():
     """The uncentered, gated norm with one weight for all heads is the layer's rms_norm_gate_per_head."""
     import burn_gdn2 as bg
@@ -201,5 +210,3 @@ def test_refusals():
         call(x.half())
     with pytest.raises(ValueError):
         call(x, None, w.cpu())
-    with pytest.raises(bg.Gdn2Error, match="EUNSUPPORTED"):
-        call(torch.zeros(2, 3 * 1025, device="cuda"))

@@ -125,6 +125,36 @@ def test_resets_growth_and_infinities():
         R.check(v.cpu()[at], want[k][at], bound[k][at], k)
 
 
+@pytest.mark.parametrize("rate,T,C", [(20.0, 90, 34), (90.0, 90, 34), (6.0, 40, 64), (0.4, 5000, 12), (3.0, 700, 600)])
+@pytest.mark.parametrize("lens", [None, "packed"])
+def test_growth_of_nothing(rate, T, C, lens):
+    """A decay above one over tokens whose state (adjoint) is zero: its product over a run, a tile or a segment
+    leaves f32's range, and zero times that stays zero."""
+    gen = _gen(int(rate))
+    xs, gs = torch.randn(T, C, generator=gen), _decay(gen, T, C)
+    dh, ds = torch.randn(T, C, generator=gen), torch.zeros(1, C)
+    late = T - 5
+    gs[3:late, ::2] = rate   # every other channel, which neither x nor the gradient of h touches meanwhile
+    xs[:late, ::2], dh[4:, ::2] = 0.0, 0.0
+    cu = None if lens is None else torch.tensor([0, T, T], dtype=torch.int32)
+    st, ds = (None, ds) if lens is None else (torch.zeros(2, C), torch.cat((ds, ds)))
+    def both_ways(lengths, comp):
+        want, bound = R.scan(xs, gs, st, lengths, comp, dh, ds)
+        got = _run(xs, gs, st, dh, ds, (1, T), cu, comp, True)
+        if rate > 88.8:  # e^90 dh[3] > 2^128 for dh[3] > 0.28: no f32 adjoint before token 3, and none in its dg (or 1 - e^90 times it)
+            for k, rows in (("dx", 4 if comp else 3), ("dg", 4), ("d_state", 1)):
+                if k in got:
+                    got[k], want[k] = got[k].clone(), want[k].clone()
+                    got[k][:rows, ::2] = want[k][:rows, ::2] = 0.0
+        _check(got, want, bound)
+
+    both_ways([T] if lens is None else [T, 0], False)
+    if lens is None and T == 90:  # a leaky average of nothing, and token by token
+        both_ways([T], True)
+        want, bound = R.scan(xs, gs, None, [1] * T, True)
+        _check(_run(xs, gs, torch.zeros(T, C), None, None, (T, 1), None, True, False), want, bound)
+
+
 def test_strided_and_broadcast_inputs():
     """Column slices, a batch-transposed buffer, an odd offset, gradients of broadcast inputs."""
     import burn_gdn2 as bg

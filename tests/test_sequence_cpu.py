@@ -128,8 +128,7 @@ def _norm_args(**over):
 
 @pytest.mark.parametrize("over,status", [
     (dict(rows=0), 1), (dict(groups=0), 1), (dict(width=-4), 1), (dict(dtype=2), 1), (dict(eps=0.0), 1),
-    (dict(eps=float("nan")), 1), (dict(x=None), 1), (dict(width=4100), 2), (dict(width=1025), 2),
-    (dict(groups=1 << 20, width=1 << 12), 2),
+    (dict(eps=float("nan")), 1), (dict(x=None), 1), (dict(groups=1 << 20, width=1 << 12), 2),
 ])
 def test_group_norm_argument_errors(over, status):
     from burn_gdn2 import LIB, _lib
