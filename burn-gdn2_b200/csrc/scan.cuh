@@ -107,20 +107,23 @@ __device__ __forceinline__ f32x2 grow(f32x2 e, f32x2 g, f32x2 c) {
 
 // From the state `c` before the step's first token (after its last, in the
 // adjoint), the state before this warp's run; c becomes the state after the
-// step, and the maps join to `A` of the whole (with SUM).
+// step, and the maps join to `A` of the whole (with SUM).  wild: a product of
+// the step is beyond f32.
 template <int NW, bool PACKED, bool SUM>
 __device__ __forceinline__ f32x2 join(ScanMaps<NW>& sh, int buf, int warp, int lane, f32x2 A, f32x2 H, bool cut,
-                                      f32x2& c, f32x2& all, bool& any_cut) {
+                                      f32x2& c, f32x2& all, bool& any_cut, bool& wild) {
+  float a0, a1;
+  f2un(A, a0, a1);
   sh.run[buf][warp][lane] = make_ulonglong2(A, H);
   if (PACKED && lane == 0) sh.cut[buf][warp] = cut;
-  __syncthreads();
+  wild = __syncthreads_or(!(a0 <= FLT_MAX && a1 <= FLT_MAX));
   f32x2 cin = c;
   #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w == warp) cin = c;
     const ulonglong2 m = sh.run[buf][w][lane];
     const bool stop = PACKED && sh.cut[buf][w];
-    c = stop ? m.y : through(m.x, c, m.y);
+    c = stop ? m.y : wild ? through(m.x, c, m.y) : f2fma(m.x, c, m.y);
     if (SUM) {
       all = f2mul(all, m.x);
       any_cut |= stop;
@@ -340,7 +343,8 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
       }
     }
     f32x2 tile = f2pk(1.f, 1.f), before = f2pk(0.f, 0.f);
-    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, MAPS ? before : c, tile, any_cut);
+    bool wild;
+    const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, MAPS ? before : c, tile, any_cut, wild);
     if (MAPS) {  // this tile, then those behind it
       c = through(all, before, c);
       all = f2mul(all, tile);
@@ -350,10 +354,8 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
     if (p.carry && ch.on0 && t0 < p.T) ch.store_state(carry, cin);
     const int first_cut = cuts ? __ffs(cuts) - 1 : RUN;
     if (plain) {
-      float a0, a1;
-      f2un(A, a0, a1);
-      if (__any_sync(0xffffffffu, fmaxf(a0, a1) > FLT_MAX)) {  // products beyond f32 (see through())
-        float c0, c1;
+      if (wild) {  // see through()
+        float a0, a1, c0, c1;
         f2un(cin, c0, c1);
         #pragma unroll
         for (int i = 0; i < RUN; ++i) {
@@ -537,7 +539,8 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
       for (int i = RUN - 1; i >= 0; --i) adjoint(std::false_type(), i, gs.get(i), la[i]);
     }
     f32x2 tile = f2pk(1.f, 1.f), behind = f2pk(0.f, 0.f);
-    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, MAPS ? behind : c, tile, any_cut);
+    bool wild;
+    f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, MAPS ? behind : c, tile, any_cut, wild);
     if (MAPS) {  // this tile, then those before it
       c = through(all, behind, c);
       all = f2mul(all, tile);
