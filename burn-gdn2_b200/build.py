@@ -1,5 +1,6 @@
 #!/usr/bin/env python3
-"""Build libgdn2_b200.so (all sm_100a kernels + the C ABI of include/gdn2.h).
+"""Build libgdn2_b200.so (all sm_100a kernels + the C ABI of include/gdn2.h)
+and _torch_calls.so (csrc/torch_calls.cpp: the sequence operators on torch tensors).
 
     python burn-gdn2_b200/build.py [--force] [--verbose]
 
@@ -14,6 +15,7 @@ import concurrent.futures as cf
 import hashlib
 import os
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -21,6 +23,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "burn_gdn2", "libgdn2_b200.so")
+
+CALLS = os.path.join(HERE, "burn_gdn2", "_torch_calls.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -35,6 +39,32 @@ def _digest(paths, extra):
             h.update(f.read())
     h.update(" ".join(extra).encode())
     return h.hexdigest()[:16]
+
+
+def build_torch_calls(force=False):
+    """The extension for the installed torch and Python; links libgdn2_b200.so beside it."""
+    import torch
+
+    src = os.path.join(CSRC, "torch_calls.cpp")
+    home = os.path.dirname(torch.__file__)
+    include = [INCLUDE, sysconfig.get_paths()["include"], os.path.join(home, "include"),
+               os.path.join(home, "include", "torch", "csrc", "api", "include"),
+               os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    libs = os.path.join(home, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [a for d in include for a in ("-isystem", d)] + [src, "-o", CALLS]
+    cmd += ["-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath," + libs]
+    cmd += ["-L" + os.path.dirname(LIB), "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    tag = _digest([src, os.path.join(INCLUDE, "gdn2.h")], cmd + [torch.__version__, sysconfig.get_python_version()])
+    stamp = CALLS + ".stamp"
+    if force or not os.path.exists(CALLS) or not os.path.exists(stamp) or open(stamp).read() != tag:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+        with open(stamp, "w") as f:
+            f.write(tag)
+    return CALLS
 
 
 def build(force=False, verbose=False):
@@ -82,6 +112,7 @@ def build(force=False, verbose=False):
         p = os.path.join(BUILD, f)
         if f.endswith(".o") and p not in keep:
             os.remove(p)
+    build_torch_calls(force)
     return LIB
 
 
