@@ -210,3 +210,5 @@ def test_refusals():
         call(x.half())
     with pytest.raises(ValueError):
         call(x, None, w.cpu())
+    with pytest.raises(bg.Gdn2Error, match="EUNSUPPORTED"):  # 2^31 channels, all the same stored one
+        call(torch.zeros(1, device="cuda").as_strided((1, 1 << 31), (0, 0)), num_groups=1)
