@@ -60,11 +60,12 @@ def test_sizes(dtype, rows, groups, width, gate, affine, bias, center):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,groups,width", [(3, 1, 1025), (2, 2, 1501), (5, 1, 4104), (700, 1, 4100), (3, 3, 8192), (1, 1, 10240)])
+@pytest.mark.parametrize("rows,groups,width", [(3, 1, 1025), (2, 2, 1501), (5, 1, 4104), (700, 1, 4100), (3, 3, 8192), (1, 1, 10240), (3, 1, 30000)])
 @pytest.mark.parametrize("gate,affine,bias,center", [(True, "channel", True, True), (False, "group", True, False),
                                                      (True, "group", False, True), (False, "none", False, True)])
 def test_wide_groups(dtype, rows, groups, width, gate, affine, bias, center):
-    """Groups that a block does not hold at once: 40 values a thread at most, then trees of 8."""
+    """Groups that a block does not hold at once: the sums of weights' gradients in shared memory or, for the
+    widest, not; at most 20 additions a thread, then trees."""
     test_sizes(dtype, rows, groups, width, gate, affine, bias, center)
 
 
