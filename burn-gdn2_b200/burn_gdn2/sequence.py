@@ -14,6 +14,10 @@ in the rows cu_seqlens[n] .. cu_seqlens[n+1].  A ``cu_seqlens`` on the CPU is
 checked and copied to the device; one on the device is taken as it is (the
 kernels stay inside the buffers whatever it holds).  Rows behind the last
 sequence come out as zero, in outputs and gradients.
+
+A backward captured into a CUDA graph wants no eager graph of the same leaves
+alive: torch would wait on the eager graph's stream in the middle of the
+capture.
 """
 from __future__ import annotations
 
@@ -23,8 +27,12 @@ from typing import Tuple
 import torch
 
 from . import _lib  # loads the library that the calls below are linked to
-from . import _torch_calls as _calls
 from .ops import _DT
+
+try:
+    from . import _torch_calls as _calls
+except ImportError as e:
+    raise ImportError("_torch_calls.so not built for this torch: run `python burn-gdn2_b200/build.py`") from e
 
 _calls.set_error_class(_lib.Gdn2Error)
 
