@@ -84,9 +84,10 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
     T = 1 is the decode step.  ``inplace`` writes the new state over ``state``
     and returns it (serving; no gradients).  g may be anything whose
     exponential is wanted: -inf cuts off what came before.  Decays of spans
-    are joined as products in f32: growth (g > 0) is exact as far as the product
-    over a span stays below 3e38; beyond, a state of zero stays zero and any
-    other one becomes infinite.  Differentiable in x, g and state, once.
+    are joined as products in f32: growth (g > 0) is exact as far as the products
+    over spans of the sequence stay inside f32 (1e-38 to 3e38); beyond, a state
+    of zero stays zero and any other one need not stay finite (or come back).
+    Differentiable in x, g and state, once.
     """
     return _calls.gated_scan(x, g, state, _packed("gated_scan", cu_seqlens, x), complement, inplace)
 
