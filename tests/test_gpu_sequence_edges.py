@@ -64,6 +64,22 @@ def test_second_derivatives_are_refused():
             g.sum().backward()
 
 
+def test_the_layer_with_another_core_is_as_often_differentiable():
+    import burn_gdn2 as bg
+    from burn_gdn2 import training
+
+    def core(q, k, v, g, b, w, scale, chunk):  # any torch core: all its inputs in a product
+        return g.exp() * scale * (q + b * k) * v * w, None
+
+    cfg = bg.Gdn2Config(mode=bg.Gdn2Mode.Chunk, chunk_size=64, hidden_size=64, num_heads=1, head_dim=32)
+    m = bg.GatedDeltaNet2.new(cfg, device="cuda", dtype=torch.float32, seed=2)
+    x = torch.randn(1, 6, 64, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).requires_grad_(True)
+    y = training.layer_forward(m.parameters(), cfg, x, core=core)
+    (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    (gg,) = torch.autograd.grad(g.square().sum(), x)
+    assert torch.isfinite(gg).all() and gg.any()
+
+
 def test_inference_mode_and_in_place_versions():
     import burn_gdn2 as bg
 

@@ -1,5 +1,6 @@
 """CPU: what the sequence operators refuse, before any launch, and their C
 entries' argument errors."""
+import collections
 import ctypes
 
 import pytest
@@ -23,7 +24,7 @@ def test_packed_offsets_are_checked_on_the_host():
     from burn_gdn2 import sequence
 
     x = _fake(1, 10, 4)
-    for bad in ([1, 5], [0, 7, 3], [0, 11], [0, 4, 3, 9]):
+    for bad in ([1, 5], [0, 7, 3], [0, 11], [0, 4, 3, 9], [0, 2147483647, -2, 1]):
         with pytest.raises(ValueError, match="ascend"):
             sequence._cu_seqlens("op", torch.tensor(bad, dtype=torch.int32), x)
     for bad in (torch.tensor([0], dtype=torch.int32), torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([0.0, 1.0])):
@@ -246,6 +247,9 @@ def test_pool_structures():
     assert [a is b for a, b in zip(flat, t)] == [True] * 6 and len(flat) == 6
     again = sequence._pool_like(nested, iter(flat))
     assert isinstance(again[0], bg.Gdn2State) and again[0].conv_v is t[3] and again[1][1][0] is t[5]
+    pair = collections.namedtuple("Pair", "cache state")(t[0], t[1])
+    again = sequence._pool_like(pair, iter(sequence._pool_tensors("op", pair)))
+    assert type(again) is type(pair) and again.cache is t[0] and again.state is t[1]
     with pytest.raises(TypeError):
         sequence._pool_tensors("op", {"a": 1})
     with pytest.raises(RuntimeError, match="CPU tensor"):
