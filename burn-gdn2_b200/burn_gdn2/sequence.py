@@ -86,7 +86,8 @@ def gated_scan(x, g, state=None, *, cu_seqlens=None, complement: bool = False,
     exponential is wanted: -inf cuts off what came before.  Decays of spans
     are joined as products in f32: growth (g > 0) is exact as far as the products
     over spans of the sequence stay inside f32 (1e-38 to 3e38); beyond, a state
-    of zero stays zero and any other one need not stay finite (or come back).
+    of zero stays zero, also one that a reset has cut off in the same span, and
+    any other one need not stay finite (or come back).
     Differentiable in x, g and state, once.
     """
     return _calls.gated_scan(x, g, state, _packed("gated_scan", cu_seqlens, x), complement, inplace)

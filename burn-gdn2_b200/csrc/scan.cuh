@@ -90,6 +90,34 @@ __device__ __forceinline__ f32x2 through(f32x2 A, f32x2 c, f32x2 H) {
   return f2pk(c0 == 0.f ? h0 : v0, c1 == 0.f ? h1 : v1);
 }
 
+__device__ __forceinline__ bool not_number(f32x2 v) {
+  float v0, v1;
+  f2un(v, v0, v1);
+  return v0 != v0 || v1 != v1;
+}
+
+// Product of the decays of two neighbouring spans.  A reset leaves zero beside
+// growth beyond f32 as well: a state that it cut off has nothing to grow from.
+__device__ __forceinline__ f32x2 chained(f32x2 a, f32x2 b) {
+  const f32x2 v = f2mul(a, b);
+  if (!not_number(v)) return v;
+  float v0, v1, s0, s1;
+  f2un(v, v0, v1);
+  f2un(f2add(a, b), s0, s1);  // NaN where a factor is: both are at least 0
+  return f2pk(v0 != v0 && s0 == s0 ? 0.f : v0, v1 != v1 && s1 == s1 ? 0.f : v1);
+}
+
+// The same of a segment's tiles, the latest one's runs being in `sh` and their
+// product `tile`; a product of all that is a number has met no such pair.
+template <int NW>
+__device__ __forceinline__ f32x2 chained(const ScanMaps<NW>& sh, int buf, int lane, f32x2 all, f32x2 tile) {
+  const f32x2 v = f2mul(all, tile);
+  if (!not_number(v)) return v;
+  #pragma unroll 1
+  for (int w = 0; w < NW; ++w) all = chained(all, sh.run[buf][w][lane].x);
+  return all;
+}
+
 // e c + in for an e = e^g (or 1 - e^g) that may be beyond f32 although g is
 // not: nothing grows out of nothing.  SURE: e is a number.
 template <bool SURE>
@@ -327,7 +355,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
           }
         } else {
           H = grow<SURE>(e, g, H, in);
-          if (!cut) A = f2mul(A, e);
+          if (!cut) A = SURE ? f2mul(A, e) : chained(A, e);
         }
         product = A;
         state = H;
@@ -350,7 +378,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, fal
     const f32x2 cin = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, H, cut, MAPS ? before : c, tile, any_cut, wild);
     if (MAPS) {  // this tile, then those behind it
       c = through(all, before, c);
-      all = f2mul(all, tile);
+      all = chained(sh, step & 1, lane, all, tile);
       if (PACKED && any_cut) break;
       continue;
     }
@@ -506,7 +534,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
         }
       } else {
         M = grow<SURE>(e, g, f2add(ds.get(i), M));
-        if (!cut) A = f2mul(A, e);
+        if (!cut) A = SURE ? f2mul(A, e) : chained(A, e);
       }
     };
     if (plain && !cuts) {
@@ -546,7 +574,7 @@ __global__ void __launch_bounds__(32 * NW, resident_blocks<TX, TG, MODE>(NW, tru
     f32x2 mu = join<NW, PACKED, MAPS>(sh, step & 1, warp, lane, A, M, cut, MAPS ? behind : c, tile, any_cut, wild);
     if (MAPS) {  // this tile, then those before it
       c = through(all, behind, c);
-      all = f2mul(all, tile);
+      all = chained(sh, step & 1, lane, all, tile);
       if (PACKED && any_cut) break;
       continue;
     }
