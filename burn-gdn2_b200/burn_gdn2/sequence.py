@@ -7,13 +7,14 @@
   select_states     the same into a new pool of another size
 
 Every operator takes CUDA tensors on any device and launches on that device's
-current stream; it is differentiable where an input requires a gradient, and
-deterministic.  Sequences come as a dense batch [B,T,C], or packed: one
-buffer [1,R,C] with ``cu_seqlens`` (int32 [N+1], ascending from 0), sequence n
-in the rows cu_seqlens[n] .. cu_seqlens[n+1].  A ``cu_seqlens`` on the CPU is
-checked and copied to the device; one on the device is taken as it is (the
-kernels stay inside the buffers whatever it holds).  Rows behind the last
-sequence come out as zero, in outputs and gradients.
+current stream; it is differentiable where an input requires a gradient (in
+reverse mode; a tangent of forward mode is refused), and deterministic.
+Sequences come as a dense batch [B,T,C], or packed: one buffer [1,R,C] with
+``cu_seqlens`` (int32 [N+1], ascending from 0), sequence n in the rows
+cu_seqlens[n] .. cu_seqlens[n+1].  A ``cu_seqlens`` on the CPU is checked and
+copied to the device; one on the device is taken as it is (the kernels stay
+inside the buffers whatever it holds).  Rows behind the last sequence come
+out as zero, in outputs and gradients.
 
 A backward captured into a CUDA graph wants no eager graph of the same leaves
 alive: torch would wait on the eager graph's stream in the middle of the

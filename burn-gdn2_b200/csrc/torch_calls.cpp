@@ -3,8 +3,9 @@
 // because a call of a decode step runs for 3 us on the device: the same work in
 // Python took 15 to 20 us of the host, and 120 us with a gradient.
 //
-// Gradients are given once: an output's gradient with create_graph = True
-// raises when it is differentiated again.
+// Gradients are given once, in reverse: an output's gradient with create_graph
+// = True raises when it is differentiated again, a tangent of forward-mode
+// differentiation is refused.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
@@ -98,6 +99,12 @@ bool wants_grad(std::initializer_list<Tensor> list) {
   for (const Tensor& t : list)
     if (t.defined() && t.requires_grad()) return true;
   return false;
+}
+
+// A dual tensor does not require a gradient, so its tangent would be lost.
+void no_tangents(const char* what, std::initializer_list<Tensor> list) {
+  for (const Tensor& t : list)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
 
 // What a second derivative meets.
@@ -206,6 +213,7 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor g, const std::optional<Te
                    ": g must be float32 or x's dtype ", x.scalar_type(), ", got ", g.scalar_type());
   check_sizes(what, x);
   const Tensor cu = given(cu_in), given_state = given(state_in);
+  no_tangents(what, {x, g, given_state});
   same_device(what, x, g);
   same_device(what, x, given_state);
   const int64_t n = cu.defined() ? cu.numel() - 1 : x.size(0), T = x.size(1), C = x.size(2);
@@ -299,6 +307,7 @@ std::tuple<Tensor, Tensor> causal_conv_silu(Tensor x, const Tensor& weight_in, c
   TORCH_CHECK_VALUE(x.dim() == 3, what, ": x must be [B,T,C], got ", x.sizes());
   check_sizes(what, x);
   const Tensor cu = given(cu_in);
+  no_tangents(what, {x, weight_in, given(cache_in)});
   same_device(what, x, weight_in);
   same_device(what, x, given(cache_in));
   const int64_t n = cu.defined() ? cu.numel() - 1 : x.size(0), T = x.size(1), C = x.size(2);
@@ -418,6 +427,7 @@ Tensor group_norm_gate(const Tensor& x, const std::optional<Tensor>& gate_in, co
   if (chan > kMaxInt) throw Failure(GDN2_EUNSUPPORTED, "group_norm_gate: more than 2^31 - 1 channels");
   const Tensor gate = given(gate_in);
   Tensor affine[2] = {given(weight_in), given(bias_in)};
+  no_tangents(what, {x, gate, affine[0], affine[1]});
   same_device(what, x, gate);
   TORCH_CHECK_VALUE(!gate.defined() || (gate.sizes() == x.sizes() && gate.scalar_type() == x.scalar_type()), what,
                     ": gate must be ", x.sizes(), " ", x.scalar_type(), ", got ", gate.sizes(), " ", gate.scalar_type());
@@ -448,6 +458,7 @@ void check_pool(const char* what, const std::vector<Tensor>& pool) {
                       "many, got ", t.sizes(), " beside ", pool[0].sizes());
     TORCH_CHECK_VALUE(t.is_contiguous(), what, ": the tensors of a pool must be contiguous");
     TORCH_CHECK_VALUE(!t.requires_grad(), what, ": the rows of a pool move without gradients; detach its tensors");
+    no_tangents(what, {t});
     same_device(what, pool[0], t);
   }
   TORCH_CHECK_VALUE(pool[0].size(0) <= GDN2_MAX_STATE_ROWS, what, ": ", pool[0].size(0), " rows, at most ",
