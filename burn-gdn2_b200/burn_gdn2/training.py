@@ -23,6 +23,7 @@ from typing import Callable, Dict, Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 
 from .config import Gdn2Config
 from .ops import GatedDeltaCore
@@ -116,7 +117,11 @@ def _conv_kernel(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 
 
 def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
-    """rms_norm_gate on the B200 kernels: a group a head, not centered."""
+    """rms_norm_gate on the B200 kernels: a group a head, not centered.  A
+    forward-mode tangent (of the gate's or the norm's weights: the core lets
+    none through) takes the torch ops."""
+    if any(unpack_dual(t).tangent is not None for t in (o, gate, weight)):
+        return rms_norm_gate(o, gate, weight, eps)
     rows = lambda t: t.reshape(*t.shape[:-2], -1)
     return group_norm_gate(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False).view(o.shape)
 
