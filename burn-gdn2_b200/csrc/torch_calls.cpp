@@ -11,6 +11,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TensorUtils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -115,15 +116,16 @@ struct Twice : torch::autograd::Node {
     TORCH_CHECK(false, what, ": trying to differentiate twice; its gradients are once_differentiable");
   }
 };
-// Gradients from a backward without a graph of its own.
-variable_list once(const char* what, const variable_list& incoming, variable_list out) {
+// Gradients from a backward without a graph of its own: with create_graph they
+// hang on all that they depend on (the incoming gradients, the inputs) by a
+// node that refuses, else a penalty on a gradient would drop out in silence.
+variable_list once(const char* what, const variable_list& incoming, const variable_list& inputs, variable_list out) {
   if (!at::GradMode::is_enabled()) return out;
-  bool graph = false;
-  for (const Tensor& t : incoming) graph = graph || (t.defined() && t.requires_grad());
-  if (!graph) return out;
   auto node = std::shared_ptr<Twice>(new Twice(what), torch::autograd::deleteNode);
-  for (const Tensor& t : incoming)
-    if (t.defined() && t.requires_grad()) node->add_next_edge(torch::autograd::impl::gradient_edge(t));
+  for (const variable_list* list : {&incoming, &inputs})
+    for (const Tensor& t : *list)
+      if (t.defined() && t.requires_grad()) node->add_next_edge(torch::autograd::impl::gradient_edge(t));
+  if (!node->num_outputs()) return out;
   for (Tensor& t : out)
     if (t.defined()) {
       t = t.detach();
@@ -199,7 +201,7 @@ struct Scan : torch::autograd::Function<Scan> {
       const Tensor ws = workspace(size, x);
       check(gdn2_gated_scan_bwd(&a, ptr(ws), size, on.stream));
     }
-    return once("gated_scan", grads, std::move(out));
+    return once("gated_scan", grads, {x, g, state}, std::move(out));
   }
 };
 
@@ -296,7 +298,7 @@ struct Conv : torch::autograd::Function<Conv> {
       const Tensor ws = workspace(size, x);
       check(gdn2_causal_conv_bwd(&a, ptr(ws), size, on.stream));
     }
-    return once("causal_conv_silu", grads, std::move(out));
+    return once("causal_conv_silu", grads, {x, weight, cache}, std::move(out));
   }
 };
 
@@ -332,6 +334,13 @@ struct NormRest {
 // [..., C] as rows; a copy where the rows are not evenly spaced or their channels not contiguous.
 Tensor norm_rows(const Tensor& t, int64_t chan) {
   return t.defined() ? rows(t.dim() == 2 ? t : t.reshape({-1, chan})) : t;
+}
+// t such that norm_rows makes no copy of it: a copy made once, for forward and backward.
+Tensor evenly(const Tensor& t, int64_t chan) {
+  if (!t.defined() || t.is_contiguous()) return t;
+  const bool lined = t.stride(-1) == 1 || t.size(-1) == 1;
+  const int64_t sizes[] = {t.numel() / chan, chan};
+  return lined && at::detail::computeStride(t.sizes(), t.strides(), at::IntArrayRef(sizes)) ? t : t.contiguous();
 }
 
 gdn2_group_norm_args norm_args(const Tensor& x, const Tensor& gate, const Tensor& weight, const Tensor& bias,
@@ -369,27 +378,27 @@ struct Norm : torch::autograd::Function<Norm> {
                         const std::optional<Tensor>& weight_in, const std::optional<Tensor>& bias_in, int64_t groups,
                         double eps, bool center) {
     const Tensor gate = given(gate_in), weight = given(weight_in), bias = given(bias_in);
+    const int64_t chan = x.size(-1);
+    ctx->save_for_backward({x, gate, weight, bias});
     ctx->saved_data["needs"] = needs({x, gate, weight, bias});
-    const Tensor xr = norm_rows(x, x.size(-1)), gr = norm_rows(gate, x.size(-1));
-    ctx->save_for_backward({xr, gr, weight, bias});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["center"] = center;
-    ctx->saved_data["shape"] = x.sizes().vec();
-    Tensor y = norm_forward(xr, gr, weight, bias, {groups, eps, center});
+    Tensor y = norm_forward(norm_rows(x, chan), norm_rows(gate, chan), weight, bias, {groups, eps, center});
     return x.dim() == 2 ? y : y.view(x.sizes());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &gate = saved[1], &weight = saved[2], &bias = saved[3];
+    const Tensor &weight = saved[2], &bias = saved[3];
     variable_list out(7);
     {
       at::NoGradGuard none;
-      On on(x);
-      const int64_t wanted = ctx->saved_data["needs"].toInt();
-      const Tensor d_y = norm_rows(grads[0], x.size(1));
+      On on(saved[0]);
+      const int64_t wanted = ctx->saved_data["needs"].toInt(), chan = saved[0].size(-1);
+      const Tensor x = norm_rows(saved[0], chan), gate = norm_rows(saved[1], chan), d_y = norm_rows(grads[0], chan);
+      const Tensor* of[] = {&x, &gate, &weight, &bias};
       for (int k = 0; k < 4; ++k)
-        if ((wanted >> k) & 1) out[k] = like(saved[k]);
+        if ((wanted >> k) & 1) out[k] = like(*of[k]);
       if (x.size(0)) {
         gdn2_group_norm_bwd_args a{};
         a.fwd = norm_args(x, gate, weight, bias,
@@ -408,11 +417,10 @@ struct Norm : torch::autograd::Function<Norm> {
         for (int k = 2; k < 4; ++k)
           if (out[k].defined()) out[k].zero_();
       }
-      const auto shape = ctx->saved_data["shape"].toIntVector();
       for (int k = 0; k < 2; ++k)
-        if (out[k].defined() && shape.size() != 2) out[k] = out[k].view(shape);
+        if (out[k].defined() && saved[0].dim() != 2) out[k] = out[k].view(saved[0].sizes());
     }
-    return once("group_norm_gate", grads, std::move(out));
+    return once("group_norm_gate", grads, {saved[0], saved[1], weight, bias}, std::move(out));
   }
 };
 
@@ -444,7 +452,8 @@ Tensor group_norm_gate(const Tensor& x, const std::optional<Tensor>& gate_in, co
   const Tensor &weight = affine[0], &bias = affine[1];
   TORCH_CHECK_VALUE(!bias.defined() || (weight.defined() && weight.sizes() == bias.sizes()), what,
                     ": a bias goes with a weight of its shape");
-  if (wants_grad({x, gate, weight, bias})) return Norm::apply(x, maybe(gate), maybe(weight), maybe(bias), groups, eps, center);
+  if (wants_grad({x, gate, weight, bias}))
+    return Norm::apply(evenly(x, chan), maybe(evenly(gate, chan)), maybe(weight), maybe(bias), groups, eps, center);
   Tensor y = norm_forward(norm_rows(x, chan), norm_rows(gate, chan), weight, bias, {groups, eps, center});
   return x.dim() == 2 ? y : y.view(x.sizes());
 }
