@@ -121,7 +121,13 @@ def group_norm_gate(x, gate=None, weight=None, bias=None, *, num_groups: int, ep
     rms_norm_gate_per_head on [..., HV*V], with gradients.  f32 arithmetic;
     differentiable in x, gate, weight and bias, once.
     """
-    return _calls.group_norm_gate(x, gate, weight, bias, num_groups, eps, center)
+    return _calls.group_norm_gate(x, gate, weight, bias, num_groups, eps, center, False)
+
+
+def group_norm_gate_again(x, gate, weight, *, num_groups: int, eps: float, center: bool):
+    """group_norm_gate for a graph that may be differentiated more often: a
+    backward with create_graph runs the formula in torch operations."""
+    return _calls.group_norm_gate(x, gate, weight, None, num_groups, eps, center, True)
 
 
 # -- state pools ---------------------------------------------------------------

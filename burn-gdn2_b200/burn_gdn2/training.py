@@ -8,8 +8,10 @@ autograd: the projections are torch ops, the recurrence is ``GatedDeltaCore``
 (chunked tensor-core forward, exact-f32 backward kernel), the short conv and
 the gated norm beside it are ``causal_conv_silu`` and ``group_norm_gate``,
 every other elementwise step is a torch op, so ``loss.backward()`` gives the
-gradient of every weight and of the input.  With another core those two are
-torch ops as well, and the layer is as often differentiable as that core.
+gradient of every weight and of the input.  What the recurrence takes no part
+in (the gate's, the norm's and the output projection's weights) has second and
+forward-mode derivatives too.  With another core those two are torch ops as
+well, and the layer is as often differentiable as that core.
 The fused inference path (``GatedDeltaNet2.forward_train``) stays the fast
 forward; this one keeps the intermediates autograd needs.
 
@@ -27,7 +29,7 @@ from torch.autograd.forward_ad import unpack_dual
 
 from .config import Gdn2Config
 from .ops import GatedDeltaCore
-from .sequence import causal_conv_silu, group_norm_gate
+from .sequence import causal_conv_silu, group_norm_gate_again
 
 SHORT_CONV_KERNEL = 4  # src/short_conv.rs:5
 SHORT_CONV_CACHE = 3  # src/short_conv.rs:7
@@ -123,7 +125,8 @@ def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps:
     if any(unpack_dual(t).tangent is not None for t in (o, gate, weight)):
         return rms_norm_gate(o, gate, weight, eps)
     rows = lambda t: t.reshape(*t.shape[:-2], -1)
-    return group_norm_gate(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False).view(o.shape)
+    y = group_norm_gate_again(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False)
+    return y.view(o.shape)
 
 
 def cuda_core(q, k, v, g, b, w, scale, chunk):

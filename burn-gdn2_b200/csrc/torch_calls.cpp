@@ -4,8 +4,9 @@
 // Python took 15 to 20 us of the host, and 120 us with a gradient.
 //
 // Gradients are given once, in reverse: an output's gradient with create_graph
-// = True raises when it is differentiated again, a tangent of forward-mode
-// differentiation is refused.
+// = True raises when it is differentiated again (but for the norm of the
+// training layer), a tangent of forward-mode differentiation is refused.
+#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
@@ -331,6 +332,28 @@ struct NormRest {
   bool center;
 };
 
+// The gradients of the inputs of which `wanted` has a bit, by the formula in
+// torch operations and with a graph of their own.
+variable_list norm_backward_again(const variable_list& saved, const Tensor& d_y, int64_t wanted, const NormRest& r) {
+  const Tensor &x = saved[0], &gate = saved[1], &weight = saved[2], &bias = saved[3];
+  const int64_t chan = x.size(-1), width = chan / r.groups;
+  const auto split = [&](const Tensor& t) { return t.to(at::kFloat).reshape({-1, r.groups, width}); };
+  const auto affine = [&](const Tensor& t) { return t.numel() == chan ? t.reshape({r.groups, width}) : t; };
+  Tensor v = split(x);
+  if (r.center) v = v - v.mean(-1, true);
+  v = v * (v.square().mean(-1, true) + r.eps).rsqrt();
+  if (weight.defined()) v = v * affine(weight);
+  if (bias.defined()) v = v + affine(bias);
+  const Tensor y = (gate.defined() ? v * at::silu(split(gate)) : at::silu(v)).reshape(x.sizes()).to(x.scalar_type());
+  variable_list inputs, out(4);
+  for (int k = 0; k < 4; ++k)
+    if ((wanted >> k) & 1) inputs.push_back(saved[k]);
+  variable_list grads = torch::autograd::grad({y}, inputs, {d_y}, true, true);
+  for (int k = 0, at = 0; k < 4; ++k)
+    if ((wanted >> k) & 1) out[k] = grads[at++];
+  return out;
+}
+
 // [..., C] as rows; a copy where the rows are not evenly spaced or their channels not contiguous.
 Tensor norm_rows(const Tensor& t, int64_t chan) {
   return t.defined() ? rows(t.dim() == 2 ? t : t.reshape({-1, chan})) : t;
@@ -376,7 +399,7 @@ Tensor norm_forward(const Tensor& x, const Tensor& gate, const Tensor& weight, c
 struct Norm : torch::autograd::Function<Norm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& gate_in,
                         const std::optional<Tensor>& weight_in, const std::optional<Tensor>& bias_in, int64_t groups,
-                        double eps, bool center) {
+                        double eps, bool center, bool twice) {
     const Tensor gate = given(gate_in), weight = given(weight_in), bias = given(bias_in);
     const int64_t chan = x.size(-1);
     ctx->save_for_backward({x, gate, weight, bias});
@@ -384,26 +407,32 @@ struct Norm : torch::autograd::Function<Norm> {
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["center"] = center;
+    ctx->saved_data["twice"] = twice;
     Tensor y = norm_forward(norm_rows(x, chan), norm_rows(gate, chan), weight, bias, {groups, eps, center});
     return x.dim() == 2 ? y : y.view(x.sizes());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &weight = saved[2], &bias = saved[3];
-    variable_list out(7);
+    const int64_t wanted = ctx->saved_data["needs"].toInt(), chan = saved[0].size(-1);
+    const NormRest r{ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
+                     ctx->saved_data["center"].toBool()};
+    variable_list out(8);
+    if (at::GradMode::is_enabled() && ctx->saved_data["twice"].toBool()) {
+      variable_list again = norm_backward_again(saved, grads[0], wanted, r);
+      std::copy(again.begin(), again.end(), out.begin());
+      return out;
+    }
     {
       at::NoGradGuard none;
       On on(saved[0]);
-      const int64_t wanted = ctx->saved_data["needs"].toInt(), chan = saved[0].size(-1);
       const Tensor x = norm_rows(saved[0], chan), gate = norm_rows(saved[1], chan), d_y = norm_rows(grads[0], chan);
       const Tensor* of[] = {&x, &gate, &weight, &bias};
       for (int k = 0; k < 4; ++k)
         if ((wanted >> k) & 1) out[k] = like(*of[k]);
       if (x.size(0)) {
         gdn2_group_norm_bwd_args a{};
-        a.fwd = norm_args(x, gate, weight, bias,
-                          {ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
-                           ctx->saved_data["center"].toBool()});
+        a.fwd = norm_args(x, gate, weight, bias, r);
         a.d_y = ptr(d_y);
         a.ld_dy = d_y.stride(0);
         a.dx = ptr(out[0]);
@@ -424,8 +453,9 @@ struct Norm : torch::autograd::Function<Norm> {
   }
 };
 
+// twice: a backward with create_graph takes norm_backward_again.
 Tensor group_norm_gate(const Tensor& x, const std::optional<Tensor>& gate_in, const std::optional<Tensor>& weight_in,
-                       const std::optional<Tensor>& bias_in, int64_t groups, double eps, bool center) {
+                       const std::optional<Tensor>& bias_in, int64_t groups, double eps, bool center, bool twice) {
   const char* what = "group_norm_gate";
   check_input(what, x);
   const int64_t chan = x.dim() ? x.size(-1) : 0;
@@ -453,7 +483,7 @@ Tensor group_norm_gate(const Tensor& x, const std::optional<Tensor>& gate_in, co
   TORCH_CHECK_VALUE(!bias.defined() || (weight.defined() && weight.sizes() == bias.sizes()), what,
                     ": a bias goes with a weight of its shape");
   if (wants_grad({x, gate, weight, bias}))
-    return Norm::apply(evenly(x, chan), maybe(evenly(gate, chan)), maybe(weight), maybe(bias), groups, eps, center);
+    return Norm::apply(evenly(x, chan), maybe(evenly(gate, chan)), maybe(weight), maybe(bias), groups, eps, center, twice);
   Tensor y = norm_forward(norm_rows(x, chan), norm_rows(gate, chan), weight, bias, {groups, eps, center});
   return x.dim() == 2 ? y : y.view(x.sizes());
 }
