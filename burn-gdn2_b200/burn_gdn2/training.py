@@ -144,7 +144,7 @@ def layer_forward(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Ten
     cdt = core_dtype if core_dtype is not None else x.dtype
     fused = core is cuda_core and x.is_cuda and params["A_log"].dtype != torch.float64  # f32 activations
     conv = _conv_kernel if fused else short_conv_silu
-    norm = _norm_kernel if fused and cfg.norm_eps > 0 else rms_norm_gate
+    norm = _norm_kernel if fused and cfg.norm_eps >= torch.finfo(torch.float32).tiny else rms_norm_gate
     q, k, v, g, b, w, gate = project(params, cfg, x, gva_mode, cdt, conv)
     o, _ = core(q, k, v, g, b, w, hk ** -0.5, cfg.chunk_size)
     o4 = o.permute(0, 2, 1, 3).to(gate.dtype)  # [B,T,HV,V]
