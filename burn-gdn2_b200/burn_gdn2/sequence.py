@@ -30,12 +30,30 @@ import torch
 from . import _lib  # loads the library that the calls below are linked to
 from .ops import _DT
 
+
+class _NotBuilt:
+    """Stands for the extension where it cannot be loaded: the rest of the package needs no torch extension."""
+
+    def __init__(self, error):
+        self._error = error
+
+    def __getattr__(self, name):
+        raise ImportError("_torch_calls.so not built for this torch: run `python burn-gdn2_b200/build.py`") from self._error
+
+
 try:
     from . import _torch_calls as _calls
-except ImportError as e:
-    raise ImportError("_torch_calls.so not built for this torch: run `python burn-gdn2_b200/build.py`") from e
 
-_calls.set_error_class(_lib.Gdn2Error)
+    if _calls.torch_version != torch.__version__.split("+")[0]:
+        raise ImportError(f"_torch_calls.so is built for torch {_calls.torch_version}, this is {torch.__version__}")
+    _calls.set_error_class(_lib.Gdn2Error)
+except ImportError as e:
+    _calls = _NotBuilt(e)
+
+
+def available() -> bool:
+    """Whether the extension that the operators run on is there."""
+    return not isinstance(_calls, _NotBuilt)
 
 
 def _check_input(what: str, x: torch.Tensor):

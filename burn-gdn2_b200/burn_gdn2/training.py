@@ -21,12 +21,14 @@ dtype for its torch part; ``core`` computes (o [B,HV,T,V], final state) from
 """
 from __future__ import annotations
 
+import warnings
 from typing import Callable, Dict, Optional
 
 import torch
 import torch.nn.functional as F
 from torch.autograd.forward_ad import unpack_dual
 
+from . import sequence
 from .config import Gdn2Config
 from .ops import GatedDeltaCore
 from .sequence import causal_conv_silu, group_norm_gate_again
@@ -129,6 +131,14 @@ def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps:
     return y.view(o.shape)
 
 
+def on_operators() -> bool:
+    """Whether the short convs and the norm can run on the sequence operators; a warning where they cannot."""
+    if not sequence.available():
+        warnings.warn("forward_train_autograd runs its short convs and its norm as torch ops: _torch_calls.so is not built "
+                      "for this torch (python burn-gdn2_b200/build.py)")
+    return sequence.available()
+
+
 def cuda_core(q, k, v, g, b, w, scale, chunk):
     """The recurrence from a zero state on the B200 kernels: GatedDeltaCore."""
     return GatedDeltaCore.apply(q, k, v, g, b, w, None, scale, chunk)
@@ -142,7 +152,7 @@ def layer_forward(params: Dict[str, torch.Tensor], cfg: Gdn2Config, x: torch.Ten
     h, hk, hv, vh = cfg.num_heads, cfg.head_dim, cfg.hv, cfg.v_head
     B, T, _ = x.shape
     cdt = core_dtype if core_dtype is not None else x.dtype
-    fused = core is cuda_core and x.is_cuda and params["A_log"].dtype != torch.float64  # f32 activations
+    fused = core is cuda_core and x.is_cuda and params["A_log"].dtype != torch.float64 and on_operators()  # f32 activations
     conv = _conv_kernel if fused else short_conv_silu
     norm = _norm_kernel if fused and cfg.norm_eps >= torch.finfo(torch.float32).tiny else rms_norm_gate
     q, k, v, g, b, w, gate = project(params, cfg, x, gva_mode, cdt, conv)

@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/version.h>
 
 #include <ATen/ATen.h>
 #include <ATen/TensorUtils.h>
@@ -570,6 +571,7 @@ std::vector<Tensor> select_states(const std::vector<Tensor>& pool, const Tensor&
 
 PYBIND11_MODULE(_torch_calls, m) {
   static py::handle error;  // burn_gdn2's Gdn2Error
+  m.attr("torch_version") = TORCH_VERSION;
   m.def("set_error_class", [](py::object cls) { error = cls.release(); });
   py::register_exception_translator([](std::exception_ptr p) {
     try {
