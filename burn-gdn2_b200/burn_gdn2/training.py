@@ -117,7 +117,7 @@ def rms_norm_gate(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps
 
 def _conv_kernel(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """short_conv_silu on the B200 kernels."""
-    return causal_conv_silu(x, weight)[0]
+    return causal_conv_silu(x, weight.reshape(-1, SHORT_CONV_KERNEL))[0]
 
 
 def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -127,7 +127,7 @@ def _norm_kernel(o: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps:
     if any(unpack_dual(t).tangent is not None for t in (o, gate, weight)):
         return rms_norm_gate(o, gate, weight, eps)
     rows = lambda t: t.reshape(*t.shape[:-2], -1)
-    y = group_norm_gate_again(rows(o), rows(gate), weight, num_groups=o.shape[-2], eps=eps, center=False)
+    y = group_norm_gate_again(rows(o), rows(gate), weight.reshape(-1), num_groups=o.shape[-2], eps=eps, center=False)
     return y.view(o.shape)
 
 
