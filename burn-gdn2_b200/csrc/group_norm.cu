@@ -511,7 +511,8 @@ static int launch_norm_wide(const NormParams& p, const NormPlan& n, cudaStream_t
   q.wide_smem = bytes > 0 && bytes <= WIDE_SMEM;
   const int smem = q.wide_smem ? (int)bytes : 0;
   auto run = [&](auto kernel) {
-    int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
+    // the limit is the function's, not the launch's: one value, so that calls of several threads cannot lower it for each other
+    int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BWD ? WIDE_SMEM : 0), fn);
     if (rc) return rc;
     kernel<<<dim3(n.gx, n.gy), WIDE_THREADS, smem, st>>>(q);
     return check_cuda(cudaGetLastError(), fn);

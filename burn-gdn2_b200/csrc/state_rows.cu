@@ -167,7 +167,8 @@ int launch_state_rows(const gdn2_state_rows* t, int32_t count, const int32_t* in
   // where nothing is staged: 18.7 us (20.3, 22.6).
   const int want = dst_rows * (int)(sizeof(int2) + 64) + 16;
   const int smem = want < ROWS_SMEM_MIN ? ROWS_SMEM_MIN : want > ROWS_SMEM_MAX ? ROWS_SMEM_MAX : want / 16 * 16;
-  int rc = check_cuda(cudaFuncSetAttribute(k_state_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), fn);
+  // the limit is the function's, not the launch's: one value, so that calls of several threads cannot lower it for each other
+  int rc = check_cuda(cudaFuncSetAttribute(k_state_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM_MAX), fn);
   for (int first = 0; !rc && first < count; first += MAX_POOL) {
     RowsParams p;
     p.count = count - first < MAX_POOL ? count - first : MAX_POOL;
