@@ -517,10 +517,14 @@ typedef struct gdn2_config {
 GDN2_API int gdn2_config_validate(const gdn2_config* cfg, char* msg, size_t msg_len);
 
 /* Device-side error bits accumulated since the last call (and cleared):
- * bit 0 = a bounded wait inside a kernel gave up (a bulk copy that never
- * completed); the kernel finished without hanging but its results are
- * invalid; bit 1 = gdn2_move_state_rows met a row number outside its pool.
- * Synchronises the current device. */
+ * GDN2_DEVERR_WAIT: a bounded wait inside a kernel gave up (a bulk copy that
+ * never completed); the kernel finished without hanging but its results are
+ * invalid.  GDN2_DEVERR_STATE_INDEX: gdn2_move_state_rows met a row number
+ * outside its pool; no other result is touched by it.  Synchronises the
+ * current device. */
+#define GDN2_DEVERR_WAIT 1u
+#define GDN2_DEVERR_STATE_INDEX 2u
+
 GDN2_API int gdn2_read_device_errors(uint32_t* flags);
 
 /* Diagnostic (no counterpart in the reference): one tcgen05 MMA tile,

@@ -21,6 +21,10 @@ pub const GDN2_DTYPE_BF16: i32 = 1;
 pub const GDN2_PRECISION_F32: i32 = 0;
 pub const GDN2_PRECISION_BF16: i32 = 1;
 
+/// Bits of `gdn2_read_device_errors`.
+pub const GDN2_DEVERR_WAIT: u32 = 1;
+pub const GDN2_DEVERR_STATE_INDEX: u32 = 2;
+
 pub const GDN2_NOALLOC_SCRATCH_BYTES: usize = 32 << 20;
 
 /// 4-D view `[d0][d1][d2][d3]`, `d3` contiguous, strides in elements.

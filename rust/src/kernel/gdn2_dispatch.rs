@@ -17,6 +17,7 @@
 //! one place that depends on the cubecl release's accessor of a handle's device address.
 use std::any::{Any, TypeId};
 use std::ffi::c_void;
+use std::sync::atomic::{AtomicU32, Ordering};
 
 use burn::tensor::{backend::Backend, Tensor};
 use burn_cubecl::tensor::CubeTensor;
@@ -47,6 +48,15 @@ fn view(t: &CubeTensor<cubecl::cuda::CudaRuntime>) -> Gdn2View {
     Gdn2View { data: raw_ptr(t), stride0: s[0] as i64, stride1: s[1] as i64, stride2: s[2] as i64 }
 }
 
+/// GDN2_DEVERR_STATE_INDEX as the core calls below met it: reading the error word clears it, and the bit belongs to
+/// the caller of `gdn2_move_state_rows`.
+static POOL_ERRORS: AtomicU32 = AtomicU32::new(0);
+
+/// Panics on the bit of a bounded wait that gave up: the results of the kernel are invalid.
+fn stop_on_wait(flags: u32) {
+    assert!(flags & GDN2_DEVERR_WAIT == 0, "libgdn2_b200: device error bits {flags:#x}");
+}
+
 /// cubecl launches on its own stream: finish its queued work, run the library on the default stream, and wait
 /// for it before cubecl continues.
 fn run_on_device(client_sync: impl Fn(), launch: impl FnOnce(*mut c_void) -> i32) {
@@ -60,7 +70,20 @@ fn run_on_device(client_sync: impl Fn(), launch: impl FnOnce(*mut c_void) -> i32
     if let Err(e) = check(unsafe { gdn2_read_device_errors(&mut flags) }) {
         panic!("libgdn2_b200: {e}");
     }
-    assert!(flags == 0, "libgdn2_b200: device error bits {flags:#x}");
+    POOL_ERRORS.fetch_or(flags & GDN2_DEVERR_STATE_INDEX, Ordering::Relaxed);
+    stop_on_wait(flags);
+}
+
+/// Whether a `gdn2_move_state_rows` since the last call met a row number outside its pool, also where a core call has
+/// read the error word in between.  Synchronises the device.
+pub fn take_state_index_error() -> bool {
+    let mut flags = 0u32;
+    if let Err(e) = check(unsafe { gdn2_read_device_errors(&mut flags) }) {
+        panic!("libgdn2_b200: {e}");
+    }
+    let kept = POOL_ERRORS.swap(0, Ordering::Relaxed);
+    stop_on_wait(flags);
+    (flags | kept) & GDN2_DEVERR_STATE_INDEX != 0
 }
 
 /// `fused_recurrent_gdn2` with `update_state = true` on kernel (3): q,k,g,b `[B,HV,T,K]`, v,w `[B,HV,T,V]`,
