@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Build libgdn2_b200.so (all sm_100a kernels + the C ABI of include/gdn2.h)
-and _torch_calls.so (csrc/torch_calls.cpp: the sequence operators on torch tensors).
+and, where torch is installed, _torch_calls.so (csrc/torch_calls.cpp: the sequence operators on torch tensors).
 
     python burn-gdn2_b200/build.py [--force] [--verbose]
 
@@ -42,8 +42,13 @@ def _digest(paths, extra):
 
 
 def build_torch_calls(force=False):
-    """The extension for the installed torch and Python; links libgdn2_b200.so beside it."""
-    import torch
+    """The extension for the installed torch and Python; links libgdn2_b200.so beside it.  None without a torch: the
+    library's C and Rust callers need none."""
+    try:
+        import torch
+    except ImportError:
+        print("torch is not installed: _torch_calls.so (the Python sequence operators) is left out")
+        return None
 
     src = os.path.join(CSRC, "torch_calls.cpp")
     home = os.path.dirname(torch.__file__)
