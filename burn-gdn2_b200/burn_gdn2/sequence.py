@@ -172,8 +172,14 @@ def _pool_like(states, new):
     return type(states)(*items) if hasattr(states, "_fields") else type(states)(items)
 
 
-def _index(index) -> torch.Tensor:
-    return index if isinstance(index, torch.Tensor) else torch.tensor(index, dtype=torch.int64)
+def _index(what: str, index) -> torch.Tensor:
+    """index as a tensor; numbers given as a sequence must be whole ones (a mask or a fraction would pass for some)."""
+    if isinstance(index, torch.Tensor):
+        return index
+    t = torch.as_tensor(index)
+    if t.numel() and (t.dtype == torch.bool or t.is_floating_point() or t.is_complex()):
+        raise ValueError(f"{what}: index must be whole numbers, got {index!r}")
+    return t.to(torch.int64)
 
 
 def reorder_states(states, index) -> None:
@@ -192,7 +198,7 @@ def reorder_states(states, index) -> None:
     """
     tensors = _pool_tensors("reorder_states", states)
     if tensors:
-        _calls.reorder_states(tensors, _index(index))
+        _calls.reorder_states(tensors, _index("reorder_states", index))
 
 
 def select_states(states, index):
@@ -201,4 +207,4 @@ def select_states(states, index):
     result has the structure of ``states``; numbers as in reorder_states, but a
     row whose number on the device is outside the pool is zeros."""
     tensors = _pool_tensors("select_states", states)
-    return _pool_like(states, iter(_calls.select_states(tensors, _index(index)) if tensors else ()))
+    return _pool_like(states, iter(_calls.select_states(tensors, _index("select_states", index)) if tensors else ()))
