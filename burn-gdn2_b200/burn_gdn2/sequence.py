@@ -13,8 +13,10 @@ Sequences come as a dense batch [B,T,C], or packed: one buffer [1,R,C] with
 ``cu_seqlens`` (int32 [N+1], ascending from 0), sequence n in the rows
 cu_seqlens[n] .. cu_seqlens[n+1].  A ``cu_seqlens`` on the CPU is checked and
 copied to the device; one on the device is taken as it is (the kernels stay
-inside the buffers whatever it holds).  Rows behind the last sequence come
-out as zero, in outputs and gradients.
+inside the buffers whatever it holds).  Offsets and row numbers from the host
+are copied from pageable memory, for which the call waits on its stream: a
+serving loop and a capture pass them on the device.  Rows behind the last
+sequence come out as zero, in outputs and gradients.
 
 A backward captured into a CUDA graph wants no eager graph of the same leaves
 alive: torch would wait on the eager graph's stream in the middle of the
@@ -137,7 +139,8 @@ def group_norm_gate(x, gate=None, weight=None, bias=None, *, num_groups: int, ep
     weight, bias: f32 [C], or [C / num_groups] for all groups alike, or None.
     With ``center=False``, a gate and a weight per head this is
     rms_norm_gate_per_head on [..., HV*V], with gradients.  f32 arithmetic;
-    differentiable in x, gate, weight and bias, once.
+    eps must be above 0 in f32; differentiable in x, gate, weight and bias,
+    once.
     """
     return _calls.group_norm_gate(x, gate, weight, bias, num_groups, eps, center, False)
 

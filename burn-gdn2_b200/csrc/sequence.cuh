@@ -79,8 +79,12 @@ __device__ __forceinline__ void store_pairs(T* p, const f32x2 (&f)[VEC == 1 ? 1 
 }
 
 // Sigmoid of a pair: 1 / (1 + 2^(-t log2 e)) by the approximate exponential
-// and reciprocal (2 ulp and 1 ulp), far below the rounding of a bf16 result
-// and near f32's own.
+// and reciprocal (2 ulp and 1 ulp).  The rounded product t log2 e adds up to
+// 2 |t| half-steps, relative, where the exponential counts (t < 0), so an f32
+// silu is off by (16 + 2 |t|) 2^-24 of its value at most: below the rounding of
+// a bf16 result, a few times expf's own error near t = 0 and more on the left.
+// From about t = -87.3 down the reciprocal is below the smallest normal f32 and
+// counts as zero (silu's true value there is 1e-36 and less).
 __device__ __forceinline__ f32x2 sigmoid2(f32x2 t) {
   float e0, e1;
   f2un(f2mul(t, f2pk(-1.44269504088896f, -1.44269504088896f)), e0, e1);

@@ -7,7 +7,8 @@
 // touched (43 of 256 rows of 1.1 MB: 18.8 us, 79 % of what a copy reaches).
 // Each block packs the list of moved rows.  Where no move's source
 // is overwritten by another one (a compaction, a fork, rows gathered into
-// another pool) the blocks copy pieces of rows in no particular order.
+// another pool) the blocks copy pieces of rows in no particular order (256 rows
+// of 1 MB into another pool: 80 us, all of what a copy reaches).
 // Otherwise a block owns a span of byte columns across all rows, reads that
 // span of every source into shared memory and writes it only after the last
 // of them has been read, so no order of moves can go wrong; the span is
