@@ -179,7 +179,7 @@ def _index(what: str, index) -> torch.Tensor:
     """index as a tensor; numbers given as a sequence must be whole ones (a mask or a fraction would pass for some)."""
     if isinstance(index, torch.Tensor):
         return index
-    t = torch.as_tensor(index)
+    t = torch.tensor(index)
     if t.numel() and (t.dtype == torch.bool or t.is_floating_point() or t.is_complex()):
         raise ValueError(f"{what}: index must be whole numbers, got {index!r}")
     return t.to(torch.int64)
