@@ -25,6 +25,7 @@ capture.
 from __future__ import annotations
 
 import dataclasses
+import re
 from typing import Tuple
 
 import torch
@@ -43,10 +44,15 @@ class _NotBuilt:
         raise ImportError("_torch_calls.so not built for this torch: run `python burn-gdn2_b200/build.py`") from self._error
 
 
+def _release(version: str) -> str:
+    """The numbers of a torch version: what its headers give, without a pre-release's or a build's name."""
+    return re.match(r"\d+(\.\d+)*", version).group()
+
+
 try:
     from . import _torch_calls as _calls
 
-    if _calls.torch_version != torch.__version__.split("+")[0]:
+    if _calls.torch_version != _release(torch.__version__):
         raise ImportError(f"_torch_calls.so is built for torch {_calls.torch_version}, this is {torch.__version__}")
     _calls.set_error_class(_lib.Gdn2Error)
 except ImportError as e:

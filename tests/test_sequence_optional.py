@@ -62,3 +62,10 @@ except ImportError as e:
     print("1.0.0" in str(e.__cause__))
 """)
     assert out.strip() == "True"
+
+
+def test_release_numbers():
+    from burn_gdn2 import sequence
+
+    for version, want in (("2.11.0+cu128", "2.11.0"), ("2.12.0a0+gitabc", "2.12.0"), ("2.12.0.dev20260101", "2.12.0"), ("2.11.1", "2.11.1")):
+        assert sequence._release(version) == want
